@@ -9,7 +9,7 @@ for f in nerfool_amd/csrc/*.hip; do
   o=build/variants/$name/$(basename $f).o
   if [ "$(basename $f)" = ${NF_VARIANT_SRC:-nf_cnn.hip} ] || [ ! -f $o ]; then
     extra=""; [ "$(basename $f)" = nf_wino_bf.hip ] && extra="-fno-slp-vectorize"       # as __graft_entry__.HIPCC_EXTRA
-    /opt/rocm/bin/hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -munsafe-fp-atomics -fPIC -std=c++17 -Iinclude -Inerfool_amd/csrc $extra "$@" -c $f -o $o &
+    /opt/rocm/bin/hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -munsafe-fp-atomics -fPIC -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude -Inerfool_amd/csrc $extra "$@" -c $f -o $o &
   fi
 done
 wait
