@@ -423,6 +423,38 @@ int nf_in_act_pad_bwd(const float* dy_padded, const float* d_extra, const float*
                       int H, int W, const float* gamma, const float* beta, const float* mean, const float* rstd, int act, int pad,
                       float* d_res, float* dx, void* scratch, int64_t dy_n_stride, const float* d_extra_sub, nf_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * The feed-forward half of a transformer layer at any width (ref: gnt/transformer_network.py:38-50 is the ungated block, :175-202 the norm
+ * in front of it; here the norm has no mean and the block a gate).  dtype: 0 float32, 1 bfloat16, 2 float16 -- one type for all tensors of a
+ * call.  activation: 0 silu, 1 gelu (the error function), 2 relu.  Rows are contiguous; weights are [out, in].
+ *
+ * nf_rms_norm_fwd: h = x + residual (nullable: h = x, nothing is written), y = weight h / sqrt(mean(h^2) + eps); weight nullable (1).
+ *   Either y (the inputs' type), or q + scale: 8 bits in blocks of 32 values of a row -- scale [rows, ceil(dim / 32)] bytes e + 127, e the least
+ *   whole number with max|block| <= 448 2^e; q [rows, dim] e4m3 of v / 2^e (a block with an infinity or NaN: byte 255, q NaN).
+ *   rstd (nullable, [rows] float): what nf_rms_norm_bwd reads.
+ * nf_rms_norm_bwd: dx = rstd (w dy - xhat mean(w dy xhat)) + dh (nullable), the gradient of x and of residual alike; dweight (nullable) =
+ *   sum over rows of dy xhat, which needs a workspace of nf_rms_norm_bwd_workspace_floats(dim) floats.  Sums are in a fixed order.
+ * nf_quantize_8bit: x itself in that 8-bit form.
+ *
+ * nf_gated_ff_fwd: out [rows, dim] = (act(x Wg^T) * (x Wu^T)) Wd^T; Wg, Wu [hidden, dim], Wd [dim, hidden].  g_save, u_save (nullable, together):
+ *   x Wg^T and x Wu^T in float, [rows, hidden], for the backward pass.  Operand pointers must be 16-byte aligned.
+ * nf_gated_ff_bwd: the gradients that are not NULL of dx [rows, dim], dw_gate, dw_up [hidden, dim], dw_down [dim, hidden] from dy, g, u.
+ * workspace: as many bytes as the *_workspace_bytes call of the same sizes says (-1: sizes out of range), 256-byte aligned.
+ * ---------------------------------------------------------------------------------------------------------------- */
+int nf_rms_norm_fwd(const void* x, const void* residual, const void* weight, int64_t rows, int dim, int dtype, float eps, void* h, void* y,
+                    uint8_t* q, uint8_t* scale, float* rstd, nf_stream_t stream);
+int64_t nf_rms_norm_bwd_workspace_floats(int dim);
+int nf_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, const float* rstd, int64_t rows, int dim, int dtype,
+                    void* dx, void* dweight, float* workspace, nf_stream_t stream);
+int nf_quantize_8bit(const void* x, int64_t rows, int dim, int dtype, uint8_t* q, uint8_t* scale, nf_stream_t stream);
+int64_t nf_gated_ff_fwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype);
+int nf_gated_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, int64_t rows, int dim, int hidden, int dtype,
+                    int activation, void* out, float* g_save, float* u_save, void* workspace, nf_stream_t stream);
+int64_t nf_gated_ff_bwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, int want_dx, int want_dw_gate_up, int want_dw_down);
+int nf_gated_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* dy, const float* g, const float* u,
+                    int64_t rows, int dim, int hidden, int dtype, int activation, void* dx, void* dw_gate, void* dw_up, void* dw_down,
+                    void* workspace, nf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,97 @@
+// Shared by the feed-forward operators (nf_rms_norm.hip, nf_gated_ff*.hip): element types, 16-byte vectors of a row, the 8-bit block format.
+#pragma once
+
+#include "nf_common.h"
+
+typedef __bf16 ff_bf16;
+typedef _Float16 ff_half;
+typedef ff_bf16 ff_bf16x8 __attribute__((ext_vector_type(8)));
+typedef ff_half ff_half8 __attribute__((ext_vector_type(8)));
+typedef float ff_f32x16 __attribute__((ext_vector_type(16)));
+typedef float ff_f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned ff_u32x4 __attribute__((ext_vector_type(4)));
+
+// a row's 16-byte vectors need not start at a 16-byte address (odd row lengths): the hardware loads and stores them at any element's address
+template <typename T>
+struct FfVec;
+template <>
+struct FfVec<float> {
+    static constexpr int N = 4;
+    typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <>
+struct FfVec<ff_bf16> {
+    static constexpr int N = 8;
+    typedef ff_bf16 V __attribute__((ext_vector_type(8), aligned(2)));
+};
+template <>
+struct FfVec<ff_half> {
+    static constexpr int N = 8;
+    typedef ff_half V __attribute__((ext_vector_type(8), aligned(2)));
+};
+
+// elements c .. c + N - 1 of a row of `dim` as float; those behind the row's end are 0
+template <typename T>
+__device__ __forceinline__ void ff_load_row(const T* row, int c, int dim, float* v) {
+    constexpr int N = FfVec<T>::N;
+    if (c + N <= dim) {
+        const typename FfVec<T>::V t = *reinterpret_cast<const typename FfVec<T>::V*>(row + c);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = (float)t[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = c + j < dim ? (float)row[c + j] : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void ff_store_row(T* row, int c, int dim, const float* v) {
+    constexpr int N = FfVec<T>::N;
+    if (c + N <= dim) {
+        typename FfVec<T>::V t;
+#pragma unroll
+        for (int j = 0; j < N; ++j) t[j] = (T)v[j];
+        *reinterpret_cast<typename FfVec<T>::V*>(row + c) = t;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (c + j < dim) row[c + j] = (T)v[j];
+    }
+}
+
+// ---- the 8-bit form: 32 consecutive values of a row share the scale 2^e, e the least whole number with max|block| <= 448 * 2^e (448 is
+//      e4m3's largest value), stored as the byte e + 127; a block of zeros has e = -127, one with an infinity or a NaN the byte 255 and all
+//      its values are NaN.  This is the format that the matrix instruction scales by itself (v_mfma_scale_f32_*_f8f6f4).
+__device__ __forceinline__ unsigned ff_scale_byte(float top) {
+    const unsigned u = __float_as_uint(top) & 0x7fffffffu;
+    if (u >= 0x7f800000u) return 255u;
+    // 448 * 2^e = 1.75 * 2^(e + 8): the exponent field says floor(log2), the mantissa whether 1.75 is enough.  Subnormal maxima are below
+    // 448 * 2^-127 and take the least exponent.
+    const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e <= -127 ? 0u : (unsigned)(e + 127);
+}
+// 2^-e of a scale byte below 255: 2^127 .. 2^-127, the last of them (byte 254) subnormal
+__device__ __forceinline__ float ff_scale_inverse(unsigned byte) { return __uint_as_float(byte < 254u ? (254u - byte) << 23 : 0x400000u); }
+
+// float -> e4m3, nearest, ties to even, |v| <= 448 or NaN
+__device__ __forceinline__ unsigned ff_e4m3_soft(float v) {
+    const unsigned u = __float_as_uint(v), sign = (u >> 24) & 0x80u;
+    const float a = __uint_as_float(u & 0x7fffffffu);
+    if (!(a <= 464.f)) return sign | 0x7fu;
+    int e = (int)((u >> 23) & 0xffu) - 127;
+    if (e < -6) e = -6;
+    const float m = rintf(ldexpf(a, 3 - e));          // in steps of 2^(e - 3): 8 .. 16 for a normal value, 0 .. 8 below
+    const int n = (int)m;
+    return sign | (unsigned)(((e + 7) << 3) + n - 8);
+}
+// four floats -> four e4m3 bytes, the first in the low byte
+__device__ __forceinline__ unsigned ff_e4m3x4(float a, float b, float c, float d) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+    return (unsigned)r;
+#else
+    return ff_e4m3_soft(a) | ff_e4m3_soft(b) << 8 | ff_e4m3_soft(c) << 16 | ff_e4m3_soft(d) << 24;
+#endif
+}
+
+enum { FF_F32 = 0, FF_BF16 = 1, FF_F16 = 2 };

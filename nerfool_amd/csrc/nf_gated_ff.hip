@@ -1,0 +1,419 @@
+// The gated feed-forward block, forward and backward (gnt/transformer_network.py:38-50 is the ungated one: two projections with a ReLU between).
+//
+//   g = x Wg^T, u = x Wu^T, h = act(g) u, out = h Wd^T                                     x [M, D]; Wg, Wu [F, D]; Wd [D, F]
+//   dh = dy Wd, dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// Forward: one product makes g and u of the same features in one wave's registers and stores h (and, for a backward pass, g and u in float32:
+// their rounding to 16 bits would put an error of a bf16 half step into dg and du each, beside the one of dg and du themselves); a second
+// makes out.  Backward: dh's product stores [dg | du] (one [M, 2F] tensor) and h again; then dx (k = 2F over [Wg; Wu]), [dWg; dWu] and dWd.
+// h, dg and du are rounded once, to the inputs' type, because they are operands of a matrix product in that type.  float32 inputs are split into
+// three bf16 parts (8 + 8 + 8 bits, exact) and multiplied as six products of order <= 2^-16: float32-grade sums at 16 / 6 of the float32 pipe's rate.
+#include "nf_ff_gemm.h"
+
+namespace {
+
+enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
+
+// act(g) and act'(g)
+__device__ __forceinline__ void ff_act(int act, float g, float& a, float& slope) {
+    if (act == ACT_SILU) {
+        const float s = 1.f / (1.f + expf(-g));
+        a = g * s;
+        slope = s * (1.f + g * (1.f - s));
+    } else if (act == ACT_GELU) {
+        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+        a = g * cdf;
+        slope = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
+    } else {
+        a = g > 0.f ? g : (g != g ? g : 0.f);
+        slope = g > 0.f ? 1.f : 0.f;
+    }
+}
+
+// ---- stores of 4 consecutive values of a row (`left`: how many the row still has); pitch and address allow one store where `wide`
+template <typename T>
+__device__ __forceinline__ void ff_put(T* p, int left, const float* v) {
+    if (left >= 4) {
+        typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        *reinterpret_cast<V4*>(p) = V4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    } else {
+        for (int c = 0; c < left; ++c) p[c] = (T)v[c];
+    }
+}
+// the three bf16 parts of 4 floats.  The first is cut off, not rounded: near the largest float the rounded part would be infinite; the others are
+// rounded, which makes the third exact.  An infinity or a NaN keeps its value in the first part and zeros in the others.
+__device__ __forceinline__ void ff_split3(float v, ff_bf16* part) {
+    const unsigned u = __float_as_uint(v);
+    float hi = (float)(ff_bf16)v;
+    if (!(fabsf(hi) <= 3.4028235e38f)) hi = __uint_as_float(u & 0xffff0000u);
+    if (v != v) hi = v;
+    float rest = v - hi;
+    if (!(fabsf(v) <= 3.4028235e38f)) rest = 0.f;
+    const float mid = (float)(ff_bf16)rest;
+    part[0] = (ff_bf16)hi;
+    part[1] = (ff_bf16)mid;
+    part[2] = (ff_bf16)(rest - mid);
+}
+__device__ __forceinline__ void ff_put3(ff_bf16* p, int64_t plane, int left, const float* v) {
+    ff_bf16 t[4][3];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) ff_split3(v[c], t[c]);
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+        if (left >= 4) {
+            typedef ff_bf16 V4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<V4*>(p + e * plane) = V4{t[0][e], t[1][e], t[2][e], t[3][e]};
+        } else {
+            for (int c = 0; c < 4; ++c) p[e * plane + c] = c < left ? t[c][e] : (ff_bf16)0.f;          // the padding of the row: zeros
+        }
+    }
+}
+// an operand of a later product: 16-bit values, or three planes of bf16 parts (T = float); rows padded to `pitch`, a multiple of 8
+template <typename T>
+struct FfMid {
+    T* p;
+    int64_t pitch;
+    __device__ __forceinline__ void put(int64_t m, int n, int left, const float* v) const {
+        T* d = p + m * pitch + n;
+        if (left >= 4) {
+            typedef T V4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<V4*>(d) = V4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+        } else
+            for (int c = 0; c < 4; ++c) d[c] = (T)(c < left ? v[c] : 0.f);
+    }
+};
+template <>
+struct FfMid<float> {
+    ff_bf16* p;
+    int64_t pitch, plane;
+    __device__ __forceinline__ void put(int64_t m, int n, int left, const float* v) const { ff_put3(p + m * pitch + n, plane, left, v); }
+};
+
+template <typename T>
+struct EpiStore {
+    T *out, *out2;          // nullable
+    int64_t pitch;
+    int len, split_m;          // rows m < len go to out, rows m >= split_m to out2, at most len of them
+    __device__ __forceinline__ void plain(int, int m, int n, int left, const float* v) const {
+        const bool second = m >= split_m;
+        const int r = second ? m - split_m : m;
+        T* o = second ? out2 : out;
+        if (o && r < len) ff_put(o + r * pitch + n, left, v);
+    }
+    __device__ __forceinline__ void gated(int, int, int, int, const float*, const float*) const {}
+};
+template <typename T>
+struct EpiGate {
+    FfMid<T> h;
+    float *g_save, *u_save;          // [M, F], nullable
+    int64_t F;
+    int act;
+    __device__ __forceinline__ void gated(int, int m, int n, int left, const float* g, const float* u) const {
+        float v[4], a, slope;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            ff_act(act, g[c], a, slope);
+            v[c] = a * u[c];
+        }
+        h.put(m, n, left, v);
+        if (g_save) {
+            ff_put(g_save + m * F + n, left, g);
+            ff_put(u_save + m * F + n, left, u);
+        }
+    }
+    __device__ __forceinline__ void plain(int, int, int, int, const float*) const {}
+};
+template <typename T>
+struct EpiGateBwd {
+    FfMid<T> dgu, h;          // dgu: [M, 2 Fp], dg in columns 0 .., du in columns Fp ..
+    const float *g, *u;
+    int64_t F, Fp;
+    int act, want_h;
+    __device__ __forceinline__ void plain(int, int m, int n, int left, const float* dh) const {
+        float gv[4], uv[4], dg[4], du[4], hv[4];
+        const float *gp = g + m * F + n, *up = u + m * F + n;
+        if (left >= 4) {
+            typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
+            const F4 a = *reinterpret_cast<const F4*>(gp), b = *reinterpret_cast<const F4*>(up);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) gv[c] = a[c], uv[c] = b[c];
+        } else
+            for (int c = 0; c < 4; ++c) gv[c] = c < left ? gp[c] : 0.f, uv[c] = c < left ? up[c] : 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            float a, slope;
+            ff_act(act, gv[c], a, slope);
+            hv[c] = a * uv[c];
+            dg[c] = dh[c] * uv[c] * slope;
+            du[c] = dh[c] * a;
+        }
+        dgu.put(m, n, left, dg);
+        dgu.put(m, (int)Fp + n, left, du);
+        if (want_h) h.put(m, n, left, hv);
+    }
+    __device__ __forceinline__ void gated(int, int, int, int, const float*, const float*) const {}
+};
+
+// rows [R, C] -> rows padded with zeros to `pitch` (a multiple of 8); float -> three planes of bf16 parts
+template <typename T>
+__global__ void __launch_bounds__(256) k_ff_pack(const T* __restrict__ src, int64_t rows, int cols, FfMid<T> dst) {
+    const int per_row = (int)(dst.pitch / 4);
+    const int64_t n = rows * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per_row;
+        const int c = (int)(i - r * per_row) * 4, left = cols - c;
+        float v[4];
+        const T* s = src + r * cols + c;
+        if (left >= 4) {
+            typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+            const V4 t = *reinterpret_cast<const V4*>(s);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = (float)t[j];
+        } else
+            for (int j = 0; j < 4; ++j) v[j] = j < left ? (float)s[j] : 0.f;
+        dst.put(r, c, left > 0 ? left : 0, v);
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------------------
+template <typename T>
+struct FfElem {
+    typedef T E;
+    static constexpr int NP = 1;
+};
+template <>
+struct FfElem<float> {
+    typedef ff_bf16 E;
+    static constexpr int NP = 3;
+};
+
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// carves a workspace; with base = nullptr it only counts
+struct Carve {
+    char* base;
+    int64_t used = 0;
+    void* take(int64_t bytes) {
+        const int64_t at = used;
+        used += (bytes + 255) / 256 * 256;
+        return base ? base + at : nullptr;
+    }
+};
+
+template <typename T>
+FfMid<T> mid_at(Carve& ws, int64_t rows, int64_t pitch) {
+    FfMid<T> m;
+    m.p = (T*)ws.take(rows * pitch * sizeof(T));
+    m.pitch = pitch;
+    return m;
+}
+template <>
+FfMid<float> mid_at<float>(Carve& ws, int64_t rows, int64_t pitch) {
+    FfMid<float> m;
+    m.plane = rows * pitch;
+    m.p = (ff_bf16*)ws.take(3 * m.plane * 2);
+    m.pitch = pitch;
+    return m;
+}
+template <typename T>
+FfOperand as_operand(const FfMid<T>& m, int rows) {
+    return FfOperand{(const uint16_t*)m.p, (const uint16_t*)m.p, 0, m.pitch, rows, 0x7fffffff, 0x7fffffff};
+}
+FfOperand as_operand(const FfMid<float>& m, int rows) {
+    return FfOperand{(const uint16_t*)m.p, (const uint16_t*)m.p, m.plane, m.pitch, rows, 0x7fffffff, 0x7fffffff};
+}
+
+// a tensor [rows, cols] as an operand: itself where the kernel can read it, else a padded (and for float32 split) copy
+template <typename T>
+struct FfPacked {
+    FfMid<T> mid;
+    bool copy;
+};
+template <typename T>
+FfPacked<T> pack_at(Carve& ws, int64_t rows, int cols) {
+    FfPacked<T> p;
+    p.copy = sizeof(T) == 4 || cols % 8 != 0;
+    if (p.copy)
+        p.mid = mid_at<T>(ws, rows, pad8(cols));
+    else {
+        p.mid.p = nullptr;
+        p.mid.pitch = cols;
+    }
+    return p;
+}
+template <typename T>
+void pack_run(const void* src, int64_t rows, int cols, FfPacked<T>& p, hipStream_t st) {
+    if (!p.copy) {
+        p.mid.p = (decltype(p.mid.p))const_cast<void*>(src);
+        return;
+    }
+    int64_t blocks = (rows * (p.mid.pitch / 4) + 255) / 256;
+    if (blocks > 256 * 16) blocks = 256 * 16;
+    hipLaunchKernelGGL((k_ff_pack<T>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)src, rows, cols, p.mid);
+}
+
+template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, bool PO, bool QO, bool GATED, typename Epi>
+int launch(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
+    constexpr int LDS = 2 * NP * (BP + BQ) * BK * 2, COLS = GATED ? BP / 2 : BP;
+    static bool set[NF_MAX_DEVICES];
+    const int dev = nf_current_device();
+    const auto kernel = k_ff_gemm<E, NP, BP, BQ, WP, WQ, BK, PO, QO, GATED, Epi>;
+    if (!set[dev]) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) {
+            nf_set_error("gated feed-forward: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
+            return 2;
+        }
+        set[dev] = true;
+    }
+    FfShape s;
+    s.M = M, s.N = N, s.K = K, s.n_end = n_end;
+    s.tiles_m = (M + BQ - 1) / BQ, s.tiles_n = (N + COLS - 1) / COLS;
+    s.k_split = 1, s.k_part = (K + BK - 1) / BK * BK;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.tiles_m * s.tiles_n)), dim3(WP * WQ * 64), LDS, st, p, q, s, epi);
+    return 0;
+}
+
+// tile: 256 x 256 where that gives most of the 256 CUs a tile, else 128 x 128 (float32 parts: 128 x 128, whose three planes fill the LDS)
+template <typename T, bool PO, bool QO, bool GATED, typename Epi>
+int product(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
+    typedef typename FfElem<T>::E E;
+    if constexpr (FfElem<T>::NP == 3) {
+        return launch<E, 3, 128, 128, 2, 4, 32, PO, QO, GATED>(p, q, M, N, n_end, K, epi, st);
+    } else {
+        const int64_t big = (int64_t)((M + 255) / 256) * ((N * (GATED ? 2 : 1) + 255) / 256);
+        if (big >= 160) return launch<E, 1, 256, 256, 2, 4, 64, PO, QO, GATED>(p, q, M, N, n_end, K, epi, st);
+        return launch<E, 1, 128, 128, 2, 2, 64, PO, QO, GATED>(p, q, M, N, n_end, K, epi, st);
+    }
+}
+
+#define FF_TRY(call)            \
+    do {                        \
+        const int rc_ = (call); \
+        if (rc_) return rc_;    \
+    } while (0)
+
+template <typename T>
+struct FwdPlan {
+    FfPacked<T> x, wg, wu, wd;
+    FfMid<T> h;
+    int64_t bytes;
+    FwdPlan(char* base, int64_t M, int D, int F) {
+        Carve ws{base};
+        x = pack_at<T>(ws, M, D);
+        wg = pack_at<T>(ws, F, D);
+        wu = pack_at<T>(ws, F, D);
+        wd = pack_at<T>(ws, D, F);
+        h = mid_at<T>(ws, M, pad8(F));
+        bytes = ws.used;
+    }
+};
+
+template <typename T>
+int ff_fwd(const void* x, const void* wg, const void* wu, const void* wd, int M, int D, int F, int act, void* out, float* g_save, float* u_save,
+           void* workspace, hipStream_t st) {
+    FwdPlan<T> f((char*)workspace, M, D, F);
+    pack_run<T>(x, M, D, f.x, st);
+    pack_run<T>(wg, F, D, f.wg, st);
+    pack_run<T>(wu, F, D, f.wu, st);
+    pack_run<T>(wd, D, F, f.wd, st);
+    FfOperand p = as_operand(f.wg.mid, F);
+    p.b = (const uint16_t*)f.wu.mid.p;
+    const EpiGate<T> gate = {f.h, g_save, u_save, F, act};
+    FF_TRY((product<T, false, false, true>(p, as_operand(f.x.mid, M), M, F, (int)f.h.pitch, (int)f.x.mid.pitch, gate, st)));
+    const EpiStore<T> store = {(T*)out, nullptr, D, M, 0x7fffffff};
+    FF_TRY((product<T, false, false, false>(as_operand(f.wd.mid, D), as_operand(f.h, M), M, D, D, (int)f.h.pitch, store, st)));
+    return 0;
+}
+
+template <typename T>
+struct BwdPlan {
+    FfPacked<T> x, wg, wu, wd, dy;
+    FfMid<T> dgu, h;
+    int64_t bytes;
+    BwdPlan(char* base, int64_t M, int D, int F, bool dx, bool dwgu, bool dwd) {
+        Carve ws{base};
+        dy = pack_at<T>(ws, M, D);
+        wd = pack_at<T>(ws, D, F);
+        if (dwgu) x = pack_at<T>(ws, M, D);
+        if (dx) wg = pack_at<T>(ws, F, D), wu = pack_at<T>(ws, F, D);
+        dgu = mid_at<T>(ws, M, 2 * pad8(F));
+        if (dwd) h = mid_at<T>(ws, M, pad8(F));
+        bytes = ws.used;
+    }
+};
+
+template <typename T>
+int ff_bwd(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, const float* g, const float* u, int M, int D, int F,
+           int act, void* dx, void* dwg, void* dwu, void* dwd, void* workspace, hipStream_t st) {
+    const bool dwgu = dwg || dwu;
+    BwdPlan<T> f((char*)workspace, M, D, F, dx != nullptr, dwgu, dwd != nullptr);
+    const int Fp = (int)pad8(F);
+    pack_run<T>(dy, M, D, f.dy, st);
+    pack_run<T>(wd, D, F, f.wd, st);
+    // dh[m][f] = sum over d of dy[m][d] Wd[d][f]
+    const EpiGateBwd<T> gate = {f.dgu, f.h, g, u, F, Fp, act, dwd != nullptr};
+    FfOperand p = as_operand(f.wd.mid, (int)f.wd.mid.pitch);
+    FF_TRY((product<T, true, false, false>(p, as_operand(f.dy.mid, M), M, F, Fp, D, gate, st)));
+    if (dx) {          // dx[m][d] = sum over k of dgu[m][k] [Wg; zeros up to Fp; Wu][k][d]
+        pack_run<T>(wg, F, D, f.wg, st);
+        pack_run<T>(wu, F, D, f.wu, st);
+        p = as_operand(f.wg.mid, (int)f.wg.mid.pitch);
+        p.b = (const uint16_t*)f.wu.mid.p;
+        p.len = F, p.seg = Fp;
+        const EpiStore<T> store = {(T*)dx, nullptr, D, M, 0x7fffffff};
+        FF_TRY((product<T, true, false, false>(p, as_operand(f.dgu, M), M, D, D, Fp + F, store, st)));
+    }
+    if (dwgu) {          // [dWg; dWu][f][d] = sum over m of dgu[m][f] x[m][d]
+        pack_run<T>(x, M, D, f.x, st);
+        const EpiStore<T> store = {(T*)dwg, (T*)dwu, D, F, Fp};
+        FF_TRY((product<T, true, true, false>(as_operand(f.x.mid, (int)f.x.mid.pitch), as_operand(f.dgu, 2 * Fp), 2 * Fp, D, D, M, store, st)));
+    }
+    if (dwd) {          // dWd[d][f] = sum over m of dy[m][d] h[m][f]
+        const EpiStore<T> store = {(T*)dwd, nullptr, F, D, 0x7fffffff};
+        FF_TRY((product<T, true, true, false>(as_operand(f.h, Fp), as_operand(f.dy.mid, (int)f.dy.mid.pitch), D, F, F, M, store, st)));
+    }
+    return 0;
+}
+
+bool ff_sizes_ok(const char* what, int64_t M, int D, int F, int dtype, int act) {
+    if (M >= 1 && M <= (1 << 30) && D >= 1 && F >= 1 && D <= (1 << 20) && F <= (1 << 20) && dtype >= FF_F32 && dtype <= FF_F16 && act >= ACT_SILU && act <= ACT_RELU)
+        return true;
+    nf_set_error("%s: need 1 <= rows <= 2^30, 1 <= dim, hidden <= 2^20, dtype and activation in 0 .. 2 (got rows %lld dim %d hidden %d dtype %d activation %d)",
+                 what, (long long)M, D, F, dtype, act);
+    return false;
+}
+
+}  // namespace
+
+extern "C" int64_t nf_gated_ff_fwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype) {
+    if (!ff_sizes_ok("nf_gated_ff_fwd_workspace_bytes", rows, dim, hidden, dtype, 0)) return -1;
+    if (dtype == FF_F32) return FwdPlan<float>(nullptr, rows, dim, hidden).bytes;
+    return FwdPlan<ff_bf16>(nullptr, rows, dim, hidden).bytes;
+}
+
+extern "C" int nf_gated_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, int64_t rows, int dim, int hidden, int dtype,
+                               int activation, void* out, float* g_save, float* u_save, void* workspace, nf_stream_t stream) {
+    if (!ff_sizes_ok("nf_gated_ff_fwd", rows, dim, hidden, dtype, activation)) return 1;
+    NF_REQUIRE((g_save != nullptr) == (u_save != nullptr), "nf_gated_ff_fwd: g_save and u_save go together");
+    const auto f = dtype == FF_F32 ? ff_fwd<float> : dtype == FF_BF16 ? ff_fwd<ff_bf16> : ff_fwd<ff_half>;
+    FF_TRY(f(x, w_gate, w_up, w_down, (int)rows, dim, hidden, activation, out, g_save, u_save, workspace, (hipStream_t)stream));
+    NF_LAUNCH_CHECK("nf_gated_ff_fwd");
+    return 0;
+}
+
+extern "C" int64_t nf_gated_ff_bwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, int want_dx, int want_dw_gate_up, int want_dw_down) {
+    if (!ff_sizes_ok("nf_gated_ff_bwd_workspace_bytes", rows, dim, hidden, dtype, 0)) return -1;
+    if (dtype == FF_F32) return BwdPlan<float>(nullptr, rows, dim, hidden, want_dx, want_dw_gate_up, want_dw_down).bytes;
+    return BwdPlan<ff_bf16>(nullptr, rows, dim, hidden, want_dx, want_dw_gate_up, want_dw_down).bytes;
+}
+
+extern "C" int nf_gated_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* dy, const float* g, const float* u,
+                               int64_t rows, int dim, int hidden, int dtype, int activation, void* dx, void* dw_gate, void* dw_up, void* dw_down,
+                               void* workspace, nf_stream_t stream) {
+    if (!ff_sizes_ok("nf_gated_ff_bwd", rows, dim, hidden, dtype, activation)) return 1;
+    const auto f = dtype == FF_F32 ? ff_bwd<float> : dtype == FF_BF16 ? ff_bwd<ff_bf16> : ff_bwd<ff_half>;
+    FF_TRY(f(x, w_gate, w_up, w_down, dy, g, u, (int)rows, dim, hidden, activation, dx, dw_gate, dw_up, dw_down, workspace, (hipStream_t)stream));
+    NF_LAUNCH_CHECK("nf_gated_ff_bwd");
+    return 0;
+}

@@ -1,0 +1,134 @@
+"""The feed-forward half of a transformer layer as operators of its own, at any width and in float32, bfloat16 or float16: the
+root-mean-square norm with the residual's addition, and the gated feed-forward block.  GNT's own layers (LayerNorm and a ReLU block of
+width 64, gnt/transformer_network.py:38-50, :121-202) run inside the whole-network kernels of `GNT`; these stand beside them for networks with
+other layers.
+
+    y, h = rms_norm(x, weight, residual=r)                      # h = x + r, y = weight * h / sqrt(mean(h^2) + eps)
+    out = gated_feed_forward(y, w_gate, w_up, w_down)           # (act(y Wg^T) * (y Wu^T)) Wd^T
+
+Both have a backward pass (not a second one: differentiating a gradient raises).  On 8 bits, for inference:
+
+    q, scale, h = rms_norm_8bit(x, weight, residual=r)
+    out = gated_feed_forward_8bit((q, scale), quantize_8bit(w_gate), quantize_8bit(w_up), quantize_8bit(w_down), dtype=torch.bfloat16)
+
+An 8-bit tensor is a pair: the values, float8_e4m3fn [..., n], and the scales, float8_e8m0fnu [..., ceil(n / 32)] -- 32 consecutive values of the
+last axis share a power of two, the least 2^e with max|block| <= 448 * 2^e.  A block that holds an infinity or a NaN is NaN as a whole.
+
+Any number of leading axes; a call's tensors are of one type and on one device; tensors that are not contiguous are copied.  Work is enqueued on the
+current stream; results do not depend on scheduling (no atomics).  In float32 an infinity in an operand of a product gives NaN where the exact sum
+would be infinite: operands are split into parts, and the parts that are zero meet the infinity."""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from .. import ops
+
+
+def _rows(t, name):
+    if t.dim() < 1 or not t.shape[-1]:
+        raise ValueError('%s must have a last axis of at least one value (got the shape %s)' % (name, tuple(t.shape)))
+    return t.reshape(-1, t.shape[-1])
+
+
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        need = any(ctx.needs_input_grad[:3])
+        h, y, rstd = ops.rms_norm_fwd(x, weight, residual, eps, want_rstd=need)
+        ctx.set_materialize_grads(False)
+        if need:
+            ctx.save_for_backward(x if h is None else h, weight, rstd)
+        return (y, h) if h is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        if dy is None:          # only the sum was used
+            return (dh if need_x else None, torch.zeros_like(weight) if need_w else None, dh if need_r else None, None)
+        dx, dw = ops.rms_norm_bwd(dy, dh, h, weight, rstd, need_w)
+        return dx if need_x else None, dw, dx if need_r else None, None
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-6):
+    """x, residual [..., dim], weight [dim] -> y, or (y, h) with a residual: h = x + residual in the inputs' type, y from the sum before that rounding"""
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError('residual has the shape %s, x %s' % (tuple(residual.shape), tuple(x.shape)))
+    got = _RMSNorm.apply(_rows(x, 'x'), weight, None if residual is None else _rows(residual, 'residual'), float(eps))
+    if residual is None:
+        return got.reshape(x.shape)
+    return got[0].reshape(x.shape), got[1].reshape(x.shape)
+
+
+def _no_gradient(what, tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError('%s has no backward pass: call it under torch.no_grad(), or on tensors that do not require a gradient' % what)
+
+
+def rms_norm_8bit(x, weight=None, residual=None, eps=1e-6):
+    """rms_norm with y in 8 bits -> (q, scale), or (q, scale, h) with a residual; no backward pass"""
+    _no_gradient('rms_norm_8bit', (x, weight, residual))
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError('residual has the shape %s, x %s' % (tuple(residual.shape), tuple(x.shape)))
+    h, (q, scale), _ = ops.rms_norm_fwd(_rows(x, 'x'), weight, None if residual is None else _rows(residual, 'residual'), float(eps), quantize=True)
+    q, scale = q.reshape(x.shape), scale.reshape(*x.shape[:-1], scale.shape[-1])
+    return (q, scale) if residual is None else (q, scale, h.reshape(x.shape))
+
+
+def quantize_8bit(x):
+    """x [..., n] -> (q, scale); no backward pass"""
+    _no_gradient('quantize_8bit', (x,))
+    q, scale = ops.quantize_8bit(_rows(x, 'x'))
+    return q.reshape(x.shape), scale.reshape(*x.shape[:-1], scale.shape[-1])
+
+
+class _GatedFeedForward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation):
+        need = any(ctx.needs_input_grad[:4])
+        out, g, u = ops.gated_ff_fwd(x, w_gate, w_up, w_down, activation, save=need)
+        ctx.activation = activation
+        if need:
+            ctx.save_for_backward(x, w_gate, w_up, w_down, g, u)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w_gate, w_up, w_down, g, u = ctx.saved_tensors
+        return (*ops.gated_ff_bwd(x, w_gate, w_up, w_down, dy, g, u, ctx.activation, ctx.needs_input_grad[:4]), None)
+
+
+def gated_feed_forward(x, w_gate, w_up, w_down, activation='silu'):
+    """x [..., dim], w_gate, w_up [hidden, dim], w_down [dim, hidden] -> [..., dim]; activation: 'silu', 'gelu' (the error function), 'relu'.
+    Constant weights (requires_grad False, as everywhere in an attack) cost no gradient of their own."""
+    ops.ff_activation(activation)
+    return _GatedFeedForward.apply(_rows(x, 'x'), w_gate, w_up, w_down, activation).reshape(x.shape)
+
+
+class RMSNorm(nn.Module):
+    """`rms_norm` with its weight; called with a residual it returns (y, h)"""
+
+    def __init__(self, dim, eps=1e-6):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.eps = eps
+
+    def forward(self, x, residual=None):
+        return rms_norm(x, self.weight, residual, self.eps)
+
+
+class GatedFeedForward(nn.Module):
+    """`gated_feed_forward` with its weights, `[out, in]` as nn.Linear keeps them and under nn.Linear's names"""
+
+    def __init__(self, dim, hid, activation='silu'):
+        super().__init__()
+        ops.ff_activation(activation)
+        self.activation = activation
+        self.gate = nn.Linear(dim, hid, bias=False)
+        self.up = nn.Linear(dim, hid, bias=False)
+        self.down = nn.Linear(hid, dim, bias=False)
+
+    def forward(self, x):
+        return gated_feed_forward(x, self.gate.weight, self.up.weight, self.down.weight, self.activation)

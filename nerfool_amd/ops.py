@@ -969,3 +969,146 @@ def gnt_bwd(blob, ray_diff, mask, d_rgb, ws, shape, depth, dropout=None):
             _launch(_lib.lib().nf_gnt_bwd, 'nf_gnt_bwd', d_rgb, _ptr(blob), _ptr(ray_diff), _ptr(mask), _ptr(d_rgb), R, S, V, depth, _ptr(d_rgb_feat),
                     _ptr(ws))
     return d_rgb_feat
+
+
+# ---- the feed-forward half of a transformer layer (csrc/nf_rms_norm.hip, csrc/nf_gated_ff.hip): float32, bfloat16 or float16, one type a call ----
+_FF_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FF_ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
+
+
+def _ff(t, name, like=None):
+    """contiguous, 16-byte aligned, of a supported type; with `like`: of its type and on its device"""
+    if t.dtype not in _FF_DTYPES:
+        raise TypeError('%s must be float32, bfloat16 or float16 (got %s)' % (name, t.dtype))
+    if not t.is_cuda and not _lib.emulated():
+        raise RuntimeError('%s is on %s: the nerfool_amd kernels run on the GPU only (no CPU fallback)' % (name, t.device))
+    if like is not None and t.dtype != like.dtype:
+        raise TypeError('%s is %s, but the call is in %s' % (name, t.dtype, like.dtype))
+    if like is not None and t.device != like.device:
+        raise ValueError('%s is on %s, but the call is on %s' % (name, t.device, like.device))
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _ff_shape(t, shape, name):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError('%s has the shape %s, not %s' % (name, tuple(t.shape), tuple(shape)))
+    return t
+
+
+def ff_activation(name):
+    if name not in _FF_ACTIVATIONS:
+        raise ValueError('activation must be one of %s (got %r)' % (sorted(_FF_ACTIVATIONS), name))
+    return _FF_ACTIVATIONS[name]
+
+
+def rms_norm_fwd(x, weight, residual, eps, quantize=False, want_rstd=False):
+    """x, residual [rows, dim], weight [dim] (residual, weight: or None) -> (h or None, y, rstd or None); quantize: y is (q, scale), float8_e4m3fn
+    [rows, dim] and float8_e8m0fnu [rows, ceil(dim / 32)]"""
+    x = _ff(x, 'x')
+    rows, dim = x.shape
+    if residual is not None:
+        residual = _ff_shape(_ff(residual, 'residual', x), x.shape, 'residual')
+    if weight is not None:
+        weight = _ff_shape(_ff(weight, 'weight', x), (dim,), 'weight')
+    h = torch.empty_like(x) if residual is not None else None
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
+    y = q = scale = None
+    if quantize:
+        q, scale = _empty_8bit(rows, dim, x.device)
+    else:
+        y = torch.empty_like(x)
+    if rows:
+        with prof.launch('nf_rms_norm_fwd', x, rows=rows, dim=dim):
+            _launch(_lib.lib().nf_rms_norm_fwd, 'nf_rms_norm_fwd', x, _ptr(x), _ptr(residual), _ptr(weight), rows, dim, _FF_DTYPES[x.dtype], float(eps),
+                    _ptr(h), _ptr(y), _ptr(q), _ptr(scale), _ptr(rstd))
+    return h, (q, scale) if quantize else y, rstd
+
+
+def _empty_8bit(rows, dim, device):
+    return (torch.empty(rows, dim, dtype=torch.float8_e4m3fn, device=device),
+            torch.empty(rows, (dim + 31) // 32, dtype=torch.float8_e8m0fnu, device=device))
+
+
+def rms_norm_bwd(dy, dh, h, weight, rstd, want_dweight):
+    """-> (dx, dweight or None); dh: or None"""
+    h = _ff(h, 'h')
+    dy = _ff_shape(_ff(dy, 'dy', h), h.shape, 'dy')
+    if dh is not None:
+        dh = _ff_shape(_ff(dh, 'dh', h), h.shape, 'dh')
+    if weight is not None:
+        weight = _ff(weight, 'weight', h)
+    rows, dim = h.shape
+    dx = torch.empty_like(h)
+    if rows == 0:
+        return dx, torch.zeros(dim, dtype=h.dtype, device=h.device) if want_dweight else None
+    dw = ws = None
+    if want_dweight:
+        dw = torch.empty(dim, dtype=h.dtype, device=h.device)
+        ws = torch.empty(_lib.lib().nf_rms_norm_bwd_workspace_floats(dim), dtype=torch.float32, device=h.device)
+    with prof.launch('nf_rms_norm_bwd', h, rows=rows, dim=dim):
+        _launch(_lib.lib().nf_rms_norm_bwd, 'nf_rms_norm_bwd', h, _ptr(dy), _ptr(dh), _ptr(h), _ptr(weight), _ptr(rstd), rows, dim, _FF_DTYPES[h.dtype],
+                _ptr(dx), _ptr(dw), _ptr(ws))
+    return dx, dw
+
+
+def quantize_8bit(x):
+    """x [rows, dim] -> (q, scale) as rms_norm_fwd(quantize=True) gives them"""
+    x = _ff(x, 'x')
+    rows, dim = x.shape
+    q, scale = _empty_8bit(rows, dim, x.device)
+    if rows:
+        with prof.launch('nf_quantize_8bit', x, rows=rows, dim=dim):
+            _launch(_lib.lib().nf_quantize_8bit, 'nf_quantize_8bit', x, _ptr(x), rows, dim, _FF_DTYPES[x.dtype], _ptr(q), _ptr(scale))
+    return q, scale
+
+
+def _gated_ff_weights(x, w_gate, w_up, w_down):
+    if w_gate.dim() != 2 or w_gate.shape[1] != x.shape[1] or not w_gate.shape[0]:
+        raise ValueError('w_gate has the shape %s, not [hidden, %d]' % (tuple(w_gate.shape), x.shape[1]))
+    hidden, dim = w_gate.shape
+    return (_ff(w_gate, 'w_gate', x), _ff_shape(_ff(w_up, 'w_up', x), (hidden, dim), 'w_up'),
+            _ff_shape(_ff(w_down, 'w_down', x), (dim, hidden), 'w_down'))
+
+
+def gated_ff_fwd(x, w_gate, w_up, w_down, activation, save=False):
+    """x [rows, dim] -> (out, g, u); g, u (float32 [rows, hidden]) are None unless `save`"""
+    x = _ff(x, 'x')
+    act = ff_activation(activation)
+    w_gate, w_up, w_down = _gated_ff_weights(x, w_gate, w_up, w_down)
+    (rows, dim), hidden = x.shape, w_gate.shape[0]
+    out = torch.empty_like(x)
+    g = torch.empty(rows, hidden, dtype=torch.float32, device=x.device) if save else None
+    u = torch.empty_like(g) if save else None
+    if rows:
+        L = _lib.lib()
+        ws = _workspace_bytes(L.nf_gated_ff_fwd_workspace_bytes(rows, dim, hidden, _FF_DTYPES[x.dtype]), 'nf_gated_ff_fwd', x)
+        with prof.launch('nf_gated_ff_fwd', x, rows=rows, dim=dim, hidden=hidden):
+            _launch(L.nf_gated_ff_fwd, 'nf_gated_ff_fwd', x, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), rows, dim, hidden, _FF_DTYPES[x.dtype], act,
+                    _ptr(out), _ptr(g), _ptr(u), _ptr(ws))
+    return out, g, u
+
+
+def _workspace_bytes(n, name, like):
+    if n < 0:
+        raise RuntimeError('%s failed: %s' % (name, _lib.lib().nf_last_error().decode()))
+    return torch.empty(n, dtype=torch.uint8, device=like.device)
+
+
+def gated_ff_bwd(x, w_gate, w_up, w_down, dy, g, u, activation, want):
+    """want: four truth values, which of (dx, dw_gate, dw_up, dw_down) to compute -> those, None for the others"""
+    x = _ff(x, 'x')
+    act = ff_activation(activation)
+    w_gate, w_up, w_down = _gated_ff_weights(x, w_gate, w_up, w_down)
+    dy = _ff_shape(_ff(dy, 'dy', x), x.shape, 'dy')
+    (rows, dim), hidden = x.shape, w_gate.shape[0]
+    make = torch.empty_like if rows else torch.zeros_like
+    grads = [make(t) if w else None for t, w in zip((x, w_gate, w_up, w_down), want)]
+    if rows and any(want):
+        L = _lib.lib()
+        ws = _workspace_bytes(L.nf_gated_ff_bwd_workspace_bytes(rows, dim, hidden, _FF_DTYPES[x.dtype], int(bool(want[0])), int(bool(want[1] or want[2])),
+                                                                int(bool(want[3]))), 'nf_gated_ff_bwd', x)
+        with prof.launch('nf_gated_ff_bwd', x, rows=rows, dim=dim, hidden=hidden):
+            _launch(L.nf_gated_ff_bwd, 'nf_gated_ff_bwd', x, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(dy), _ptr(g), _ptr(u), rows, dim, hidden,
+                    _FF_DTYPES[x.dtype], act, *[_ptr(t) for t in grads], _ptr(ws))
+    return grads

@@ -12,6 +12,7 @@
 // collective (true on the GPU for the kernels in this repo as well).  __shared__ variables are per worker thread, i.e. per
 // block in flight.
 #pragma once
+#define NF_HIP_EMU 1
 
 #include <math.h>
 #include <pthread.h>
@@ -213,6 +214,32 @@ static inline nf_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_bf16(nf_emu_bf16x
         d[r] = acc;
     }
     return d;
+}
+
+// the same shape with float16 operands
+typedef _Float16 nf_emu_f16x8 __attribute__((ext_vector_type(8)));
+static inline nf_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_f16(nf_emu_f16x8 a, nf_emu_f16x8 b, nf_emu_f32x16 c, int, int, int) {
+    float A[8][64], B[8][64];
+    for (int j = 0; j < 8; ++j) nf_emu_publish_ab((float)a[j], (float)b[j], A[j], B[j]);
+    nf_emu_f32x16 d = c;
+    int l = hip_emu::lane(), col = l & 31, hi = l >> 5;
+    for (int r = 0; r < 16; ++r) {
+        int row = (r & 3) + 8 * (r >> 2) + 4 * hi;
+        float acc = c[r];
+        for (int h = 0; h < 2; ++h)
+            for (int j = 0; j < 8; ++j) acc = fmaf(A[j][row + 32 * h], B[j][col + 32 * h], acc);
+        d[r] = acc;
+    }
+    return d;
+}
+// ds_read_b64_tr_b16: each lane reads 8 bytes at its own address; within 16 lanes, lane i gets element i % 4 of lanes 4 j + i / 4, j = 0 .. 3
+static inline uint64_t nf_emu_read_tr16(const char* p) {
+    uint64_t raw;
+    memcpy(&raw, p, 8);
+    const int l = hip_emu::lane(), g = l & ~15, i = l & 15;
+    uint64_t out = 0;
+    for (int j = 0; j < 4; ++j) out |= ((hip_emu::exchange(raw, g + 4 * j + (i >> 2)) >> (16 * (i & 3))) & 0xffffull) << (16 * j);
+    return out;
 }
 
 // D = A(16x4) * B(4x16) + C.  lane l: a = A[l&15][l>>4], b = B[l>>4][l&15]; c[r] = C[row = 4*(l>>4) + r][col = l&15]
