@@ -439,6 +439,8 @@ int nf_in_act_pad_bwd(const float* dy_padded, const float* d_extra, const float*
  * nf_gated_ff_fwd: out [rows, dim] = (act(x Wg^T) * (x Wu^T)) Wd^T; Wg, Wu [hidden, dim], Wd [dim, hidden].  g_save, u_save (nullable, together):
  *   x Wg^T and x Wu^T in float, [rows, hidden], for the backward pass.  Operand pointers must be 16-byte aligned.
  * nf_gated_ff_bwd: the gradients that are not NULL of dx [rows, dim], dw_gate, dw_up [hidden, dim], dw_down [dim, hidden] from dy, g, u.
+ * nf_gated_ff_fwd_8bit: the block on operands in the 8-bit form above (dim, hidden multiples of 32; scales [rows of the operand, k / 32] bytes); h in
+ *   the middle is brought to that form from its float values; out in out_dtype.
  * workspace: as many bytes as the *_workspace_bytes call of the same sizes says (-1: sizes out of range), 256-byte aligned.
  * ---------------------------------------------------------------------------------------------------------------- */
 int nf_rms_norm_fwd(const void* x, const void* residual, const void* weight, int64_t rows, int dim, int dtype, float eps, void* h, void* y,
@@ -454,6 +456,10 @@ int64_t nf_gated_ff_bwd_workspace_bytes(int64_t rows, int dim, int hidden, int d
 int nf_gated_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* dy, const float* g, const float* u,
                     int64_t rows, int dim, int hidden, int dtype, int activation, void* dx, void* dw_gate, void* dw_up, void* dw_down,
                     void* workspace, nf_stream_t stream);
+int64_t nf_gated_ff_fwd_8bit_workspace_bytes(int64_t rows, int hidden);
+int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const void* w_gate, const uint8_t* gate_scale, const void* w_up,
+                         const uint8_t* up_scale, const void* w_down, const uint8_t* down_scale, int64_t rows, int dim, int hidden, int out_dtype,
+                         int activation, void* out, void* workspace, nf_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -10,6 +10,8 @@ typedef ff_half ff_half8 __attribute__((ext_vector_type(8)));
 typedef float ff_f32x16 __attribute__((ext_vector_type(16)));
 typedef float ff_f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned ff_u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned ff_u32x2 __attribute__((ext_vector_type(2)));
+typedef ff_bf16 ff_bf16x2 __attribute__((ext_vector_type(2)));
 
 // a row's 16-byte vectors need not start at a 16-byte address (odd row lengths): the hardware loads and stores them at any element's address
 template <typename T>
@@ -94,4 +96,42 @@ __device__ __forceinline__ unsigned ff_e4m3x4(float a, float b, float c, float d
 #endif
 }
 
+// eight e4m3 bytes (the first in lo's low byte) times 2^(byte - 127), in bfloat16: exact, but for what lies below its least value, 2^-133
+__device__ __forceinline__ ff_bf16x8 ff_from_e4m3x8(unsigned lo, unsigned hi, unsigned byte) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const float s = __uint_as_float(byte << 23);          // the instruction takes the exponent field: 2^(byte - 127)
+    ff_bf16x2 v[4];
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false);
+    v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false);
+    v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
+    return __builtin_bit_cast(ff_bf16x8, v);
+#else
+    ff_bf16x8 v;
+    for (int j = 0; j < 8; ++j) {
+        const unsigned b = ((j < 4 ? lo : hi) >> (8 * (j & 3))) & 255u, e = (b >> 3) & 15u, m = b & 7u;
+        float f = (b & 127u) == 127u || byte == 255u ? NAN : ldexpf(e ? (float)(8 + m) : (float)m, (e ? (int)e : 1) - 10 + (int)byte - 127);
+        v[j] = (ff_bf16)(b & 128u ? -f : f);
+    }
+    return v;
+#endif
+}
+
 enum { FF_F32 = 0, FF_BF16 = 1, FF_F16 = 2 };
+enum { FF_SILU = 0, FF_GELU = 1, FF_RELU = 2 };
+
+// act(g) and act'(g)
+__device__ __forceinline__ void ff_act(int act, float g, float& a, float& slope) {
+    if (act == FF_SILU) {
+        const float s = 1.f / (1.f + expf(-g));
+        a = g * s;
+        slope = s * (1.f + g * (1.f - s));
+    } else if (act == FF_GELU) {
+        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+        a = g * cdf;
+        slope = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
+    } else {
+        a = g > 0.f ? g : (g != g ? g : 0.f);
+        slope = g > 0.f ? 1.f : 0.f;
+    }
+}

@@ -12,24 +12,6 @@
 
 namespace {
 
-enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
-
-// act(g) and act'(g)
-__device__ __forceinline__ void ff_act(int act, float g, float& a, float& slope) {
-    if (act == ACT_SILU) {
-        const float s = 1.f / (1.f + expf(-g));
-        a = g * s;
-        slope = s * (1.f + g * (1.f - s));
-    } else if (act == ACT_GELU) {
-        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-        a = g * cdf;
-        slope = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
-    } else {
-        a = g > 0.f ? g : (g != g ? g : 0.f);
-        slope = g > 0.f ? 1.f : 0.f;
-    }
-}
-
 // ---- stores of 4 consecutive values of a row (`left`: how many the row still has); pitch and address allow one store where `wide`
 template <typename T>
 __device__ __forceinline__ void ff_put(T* p, int left, const float* v) {
@@ -377,7 +359,7 @@ int ff_bwd(const void* x, const void* wg, const void* wu, const void* wd, const 
 }
 
 bool ff_sizes_ok(const char* what, int64_t M, int D, int F, int dtype, int act) {
-    if (M >= 1 && M <= (1 << 30) && D >= 1 && F >= 1 && D <= (1 << 20) && F <= (1 << 20) && dtype >= FF_F32 && dtype <= FF_F16 && act >= ACT_SILU && act <= ACT_RELU)
+    if (M >= 1 && M <= (1 << 30) && D >= 1 && F >= 1 && D <= (1 << 20) && F <= (1 << 20) && dtype >= FF_F32 && dtype <= FF_F16 && act >= FF_SILU && act <= FF_RELU)
         return true;
     nf_set_error("%s: need 1 <= rows <= 2^30, 1 <= dim, hidden <= 2^20, dtype and activation in 0 .. 2 (got rows %lld dim %d hidden %d dtype %d activation %d)",
                  what, (long long)M, D, F, dtype, act);

@@ -1,0 +1,270 @@
+// The gated feed-forward block on 8-bit operands (e4m3 with a power-of-two scale per 32 values along k: nf_ff.h), forward only:
+// h = act(x Wg^T) * (x Wu^T) is brought to the same form in the output stage of its product -- 32 consecutive features of a row are one 32 x 32
+// block's rows, so that a block's maximum is a lane's 16 registers and one exchange -- and out = h Wd^T is made from it.
+//
+// v_mfma_scale_f32_32x32x64_f8f6f4 multiplies the scales in: lane l holds row l mod 32, k = 16 (l / 32) .. + 15 and 32 + 16 (l / 32) .. + 15 of the
+// instruction's 64, and its scale operand is that of the row's block l / 32 (k 0 .. 31 or 32 .. 63).  A k step of the tile is 128 values: 128
+// bytes of a row, as in the 16-bit kernels, whose loader moves them (two values as one 16-bit element), and 4 scale bytes of a row, one word.
+//
+// That instruction aligns the products of 16 consecutive k to the largest of them and drops what lies below 2^-12 of it (probed: beside a product
+// of 2^16 one of 2^4 counts, one of 2^2 does not): about 1e-4 of a sum of products like a network's, which moves a few of h's values to a
+// neighbouring step.  Beside a bfloat16 result's rounding that is small (0.0020 against 0.0017 from the exact sums at 4096 x 4096 x 8192); beside a float16
+// or float32 result's it is not.  For those the values are multiplied as bfloat16, which holds value and scale exactly, on
+// v_mfma_f32_32x32x16_bf16: float32 sums, at half the rate; v_cvt_scalef32_pk_bf16_fp8 makes two operands of two values and their scale.
+#include "nf_ff_gemm.h"
+
+typedef int ff_i32x8 __attribute__((ext_vector_type(8)));
+
+namespace {
+
+struct FfScales {
+    const uint8_t *a, *b;          // gated: gate and up
+    int64_t pitch;                 // bytes: k / 32
+    int rows;
+};
+
+// the 4 scale bytes of blocks blk .. blk + 3 of a row; blocks behind the last have the scale 1 (their values are zeros)
+__device__ __forceinline__ unsigned ff_scale_word(const uint8_t* row, int blk, int blocks) {
+    if (blk + 4 <= blocks) {
+        typedef unsigned U __attribute__((aligned(1)));
+        return *reinterpret_cast<const U*>(row + blk);
+    }
+    unsigned w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (blk + i < blocks ? (unsigned)row[blk + i] : 127u) << (8 * i);
+    return w;
+}
+
+// EXACT: the products in bfloat16
+template <int BP, int BQ, int WP, int WQ, bool GATED, bool EXACT, typename Epi>
+__global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand q, FfScales sp, FfScales sq, FfShape s, Epi epi) {
+    constexpr int BK = 64;          // in pairs of values
+    constexpr int WAVES = WP * WQ, SP = BP / WP, SQ = BQ / WQ, TP = SP / 32, TQ = SQ / 32;
+    typedef FfLoader<1, BP, BK, WAVES, false, GATED, SP> LP;
+    typedef FfLoader<1, BQ, BK, WAVES, false, false, SQ> LQ;
+    constexpr int BUF = LP::BYTES + LQ::BYTES;
+    HIP_DYNAMIC_SHARED(char, lds)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
+    const int wp = wave % WP, wq = wave / WP;
+    int tm, tn;
+    ff_tile_of(s, blockIdx.x, tm, tn);
+    const int m0 = tm * BQ, n0 = tn * (GATED ? BP / 2 : BP);
+    const int K = s.K;          // pairs
+    const int blocks = K / 16;
+    LP lp;
+    LQ lq;
+    lp.init(p, n0, 0, wave, lane);
+    lq.init(q, m0, 0, wave, lane);
+    const uint8_t *prow[TP], *qrow[TQ];
+#pragma unroll
+    for (int i = 0; i < TP; ++i) {
+        int row = GATED ? n0 + wp * (SP / 2) + 32 * (i % (TP > 1 ? TP / 2 : 1)) + r32 : n0 + wp * SP + 32 * i + r32;
+        if (row >= sp.rows) row = sp.rows - 1;
+        prow[i] = (GATED && i >= TP / 2 ? sp.b : sp.a) + row * sp.pitch;
+    }
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        int row = m0 + wq * SQ + 32 * j + r32;
+        if (row >= sq.rows) row = sq.rows - 1;
+        qrow[j] = sq.a + row * sq.pitch;
+    }
+    ff_f32x16 acc[TP][TQ];
+#pragma unroll
+    for (int i = 0; i < TP; ++i)
+#pragma unroll
+        for (int j = 0; j < TQ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    unsigned pn[TP], qn[TQ];
+#pragma unroll
+    for (int i = 0; i < TP; ++i) pn[i] = ff_scale_word(prow[i], 0, blocks);
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) qn[j] = ff_scale_word(qrow[j], 0, blocks);
+    lp.load(lds, 0, K, wave, lane);
+    lq.load(lds + LP::BYTES, 0, K, wave, lane);
+    int cur = 0;
+    for (int k0 = 0; k0 < K; k0 += BK) {
+        ff_dma_wait();
+        __syncthreads();
+        unsigned pc[TP], qc[TQ];          // the lane's scales of this step: byte 0 for its first 64 values, byte 2 for the others
+#pragma unroll
+        for (int i = 0; i < TP; ++i) pc[i] = EXACT ? pn[i] : pn[i] >> (8 * half);
+#pragma unroll
+        for (int j = 0; j < TQ; ++j) qc[j] = EXACT ? qn[j] : qn[j] >> (8 * half);
+        if (k0 + BK < K) {
+            const int blk = (k0 + BK) / 16;
+#pragma unroll
+            for (int i = 0; i < TP; ++i) pn[i] = ff_scale_word(prow[i], blk, blocks);
+#pragma unroll
+            for (int j = 0; j < TQ; ++j) qn[j] = ff_scale_word(qrow[j], blk, blocks);
+            char* nb = lds + (cur ^ 1) * BUF;
+            lp.load(nb, k0 + BK, K, wave, lane);
+            lq.load(nb + LP::BYTES, k0 + BK, K, wave, lane);
+        }
+        const char* bp = lds + cur * BUF;
+        const char* bq = bp + LP::BYTES;
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+                ff_bf16x8 a[TP], b[TQ];
+                auto fragment = [&](const char* tile, int row32, unsigned scales) {
+                    const int r = row32 + r32;
+                    const ff_u32x2 v = *reinterpret_cast<const ff_u32x2*>(tile + r * (BK * 2) + ((kk ^ ff_swz_inner<8>(r)) << 4) + 8 * half);
+                    return ff_from_e4m3x8(v.x, v.y, (scales >> (8 * (kk / 2))) & 255u);
+                };
+#pragma unroll
+                for (int i = 0; i < TP; ++i) a[i] = fragment(bp, wp * SP + 32 * i, pc[i]);
+#pragma unroll
+                for (int j = 0; j < TQ; ++j) b[j] = fragment(bq, wq * SQ + 32 * j, qc[j]);
+#pragma unroll
+                for (int i = 0; i < TP; ++i)
+#pragma unroll
+                    for (int j = 0; j < TQ; ++j) acc[i][j] = FfMfma<ff_bf16>::mul(a[i], b[j], acc[i][j]);
+            }
+        } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            ff_i32x8 a[TP], b[TQ];
+            auto fragment = [&](const char* tile, int row32) {
+                const int r = row32 + r32;
+                ff_u32x4 v[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    v[c] = *reinterpret_cast<const ff_u32x4*>(tile + r * (BK * 2) + (((4 * t + 2 * c + half) ^ ff_swz_inner<8>(r)) << 4));
+                return __builtin_bit_cast(ff_i32x8, v);
+            };
+#pragma unroll
+            for (int i = 0; i < TP; ++i) a[i] = fragment(bp, wp * SP + 32 * i);
+#pragma unroll
+            for (int j = 0; j < TQ; ++j) b[j] = fragment(bq, wq * SQ + 32 * j);
+#pragma unroll
+            for (int i = 0; i < TP; ++i)
+#pragma unroll
+                for (int j = 0; j < TQ; ++j)
+                    acc[i][j] = t == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 0, 0, 0, (int)pc[i], 0, (int)qc[j])
+                                       : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 0, 0, 2, (int)pc[i], 2, (int)qc[j]);
+        }
+        }
+        cur ^= 1;
+    }
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        const int m = m0 + wq * SQ + 32 * j + r32;
+        if (GATED) {
+#pragma unroll
+            for (int i = 0; i < TP / 2; ++i) epi.gated(m, n0 + wp * (SP / 2) + 32 * i, half, s, acc[i][j], acc[(i + TP / 2) % TP][j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < TP; ++i) epi.plain(m, n0 + wp * SP + 32 * i, half, s, acc[i][j]);
+        }
+    }
+}
+
+template <typename T>
+struct Epi8Store {
+    T* out;
+    int64_t pitch;
+    __device__ __forceinline__ void plain(int m, int n0, int half, const FfShape& s, const ff_f32x16& v) const {
+        if (m >= s.M) return;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int n = n0 + 8 * g + 4 * half;          // N is a multiple of 32
+            typedef T V4 __attribute__((ext_vector_type(4)));
+            if (n < s.N) *reinterpret_cast<V4*>(out + m * pitch + n) = V4{(T)v[4 * g], (T)v[4 * g + 1], (T)v[4 * g + 2], (T)v[4 * g + 3]};
+        }
+    }
+    __device__ __forceinline__ void gated(int, int, int, const FfShape&, const ff_f32x16&, const ff_f32x16&) const {}
+};
+
+struct Epi8Gate {
+    uint8_t *q, *scale;
+    int64_t F;
+    int act;
+    __device__ __forceinline__ void gated(int m, int n0, int half, const FfShape& s, const ff_f32x16& g, const ff_f32x16& u) const {
+        float v[16], top = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float a, slope;
+            ff_act(act, g[r], a, slope);
+            v[r] = a * u[r];
+            top = fmaxf(top, fabsf(v[r]));
+            bad |= !(fabsf(v[r]) <= 3.4028235e38f);
+        }
+        if (bad) top = INFINITY;
+        top = nf_half_max(top);
+        if (m >= s.M || n0 >= s.N) return;
+        const unsigned byte = ff_scale_byte(top);
+        const float inv = byte == 255u ? NAN : ff_scale_inverse(byte);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<unsigned*>(q + m * F + n0 + 8 * c + 4 * half) =
+                ff_e4m3x4(v[4 * c] * inv, v[4 * c + 1] * inv, v[4 * c + 2] * inv, v[4 * c + 3] * inv);
+        if (half == 0) scale[m * (F / 32) + n0 / 32] = (uint8_t)byte;
+    }
+    __device__ __forceinline__ void plain(int, int, int, const FfShape&, const ff_f32x16&) const {}
+};
+
+template <int BP, int BQ, int WP, int WQ, bool GATED, bool EXACT, typename Epi>
+int launch8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const FfScales& sq, int M, int N, int K, const Epi& epi, hipStream_t st) {
+    constexpr int LDS = 2 * (BP + BQ) * 128, COLS = GATED ? BP / 2 : BP;
+    static bool set[NF_MAX_DEVICES];
+    const int dev = nf_current_device();
+    const auto kernel = k_ff_gemm8<BP, BQ, WP, WQ, GATED, EXACT, Epi>;
+    if (!set[dev]) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) {
+            nf_set_error("gated feed-forward in 8 bits: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
+            return 2;
+        }
+        set[dev] = true;
+    }
+    FfShape s;
+    s.M = M, s.N = N, s.K = K / 2, s.n_end = N;
+    s.tiles_m = (M + BQ - 1) / BQ, s.tiles_n = (N + COLS - 1) / COLS;
+    s.k_split = 1, s.k_part = K / 2;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.tiles_m * s.tiles_n)), dim3(WP * WQ * 64), LDS, st, p, q, sp, sq, s, epi);
+    return 0;
+}
+
+// tile: 256 x 256 where that gives most of the 256 CUs a tile, else 128 x 128
+template <bool GATED, bool EXACT, typename Epi>
+int product8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const FfScales& sq, int M, int N, int K, const Epi& epi, hipStream_t st) {
+    const int64_t big = (int64_t)((M + 255) / 256) * ((N * (GATED ? 2 : 1) + 255) / 256);
+    if (big >= 160) return launch8<256, 256, 2, 4, GATED, EXACT>(p, q, sp, sq, M, N, K, epi, st);
+    return launch8<128, 128, 2, 2, GATED, EXACT>(p, q, sp, sq, M, N, K, epi, st);
+}
+
+FfOperand operand8(const void* a, const void* b, int rows, int K) {
+    return FfOperand{(const uint16_t*)a, (const uint16_t*)b, 0, K / 2, rows, 0x7fffffff, 0x7fffffff};
+}
+
+}  // namespace
+
+extern "C" int64_t nf_gated_ff_fwd_8bit_workspace_bytes(int64_t rows, int hidden) { return rows * hidden + rows * (hidden / 32) + 512; }
+
+extern "C" int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const void* w_gate, const uint8_t* gate_scale, const void* w_up,
+                                    const uint8_t* up_scale, const void* w_down, const uint8_t* down_scale, int64_t rows, int dim, int hidden,
+                                    int out_dtype, int activation, void* out, void* workspace, nf_stream_t stream) {
+    NF_REQUIRE(rows >= 1 && rows <= (1 << 30) && dim >= 32 && hidden >= 32 && dim % 32 == 0 && hidden % 32 == 0 && dim <= (1 << 20) &&
+                   hidden <= (1 << 20) && out_dtype >= FF_F32 && out_dtype <= FF_F16 && activation >= FF_SILU && activation <= FF_RELU,
+               "nf_gated_ff_fwd_8bit: need 1 <= rows <= 2^30, dim and hidden multiples of 32 up to 2^20, dtype and activation in 0 .. 2 (got rows %lld dim %d "
+               "hidden %d dtype %d activation %d)", (long long)rows, dim, hidden, out_dtype, activation);
+    hipStream_t st = (hipStream_t)stream;
+    const int M = (int)rows, D = dim, F = hidden;
+    uint8_t* hq = (uint8_t*)workspace;
+    uint8_t* hs = hq + (rows * hidden + 255) / 256 * 256;
+    const Epi8Gate gate = {hq, hs, F, activation};
+    const FfOperand pg = operand8(w_gate, w_up, F, D), qx = operand8(x, x, M, D);
+    const FfScales spg = {gate_scale, up_scale, D / 32, F}, sqx = {x_scale, x_scale, D / 32, M};
+    int rc = out_dtype == FF_BF16 ? product8<true, false>(pg, qx, spg, sqx, M, F, D, gate, st) : product8<true, true>(pg, qx, spg, sqx, M, F, D, gate, st);
+    if (rc) return rc;
+    const FfOperand p = operand8(w_down, w_down, D, F), q = operand8(hq, hq, M, F);
+    const FfScales sp = {down_scale, down_scale, F / 32, D}, sq = {hs, hs, F / 32, M};
+    if (out_dtype == FF_F32) rc = product8<false, true>(p, q, sp, sq, M, D, F, Epi8Store<float>{(float*)out, D}, st);
+    else if (out_dtype == FF_BF16) rc = product8<false, false>(p, q, sp, sq, M, D, F, Epi8Store<ff_bf16>{(ff_bf16*)out, D}, st);
+    else rc = product8<false, true>(p, q, sp, sq, M, D, F, Epi8Store<ff_half>{(ff_half*)out, D}, st);
+    if (rc) return rc;
+    NF_LAUNCH_CHECK("nf_gated_ff_fwd_8bit");
+    return 0;
+}

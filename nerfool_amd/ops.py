@@ -1112,3 +1112,42 @@ def gated_ff_bwd(x, w_gate, w_up, w_down, dy, g, u, activation, want):
             _launch(L.nf_gated_ff_bwd, 'nf_gated_ff_bwd', x, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(dy), _ptr(g), _ptr(u), rows, dim, hidden,
                     _FF_DTYPES[x.dtype], act, *[_ptr(t) for t in grads], _ptr(ws))
     return grads
+
+
+def _pair_8bit(pair, rows, dim, name, like=None):
+    """(q, scale) checked against [rows, dim] (rows or dim None: any) -> contiguous, q 16-byte aligned"""
+    q, scale = pair
+    if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.float8_e8m0fnu:
+        raise TypeError('%s must be a pair of float8_e4m3fn values and float8_e8m0fnu scales (got %s, %s)' % (name, q.dtype, scale.dtype))
+    if not q.is_cuda and not _lib.emulated():
+        raise RuntimeError('%s is on %s: the nerfool_amd kernels run on the GPU only (no CPU fallback)' % (name, q.device))
+    if scale.device != q.device or (like is not None and q.device != like.device):
+        raise ValueError('%s: values and scales must be on the device of the call' % name)
+    if q.dim() != 2 or q.shape[1] % 32 or not q.shape[1]:
+        raise ValueError('%s: the last axis must be a multiple of 32 (got the shape %s)' % (name, tuple(q.shape)))
+    _ff_shape(q, (q.shape[0] if rows is None else rows, q.shape[1] if dim is None else dim), name)
+    _ff_shape(scale, (q.shape[0], q.shape[1] // 32), name + "'s scales")
+    q, scale = q.contiguous(), scale.contiguous()
+    return (q if q.data_ptr() % 16 == 0 else q.clone()), scale
+
+
+def gated_ff_fwd_8bit(x, w_gate, w_up, w_down, activation, dtype):
+    """pairs (q, scale): x [rows, dim], w_gate, w_up [hidden, dim], w_down [dim, hidden] -> out [rows, dim] in dtype"""
+    act = ff_activation(activation)
+    if dtype not in _FF_DTYPES:
+        raise TypeError('dtype must be float32, bfloat16 or float16 (got %s)' % (dtype,))
+    x = _pair_8bit(x, None, None, 'x')
+    rows, dim = x[0].shape
+    w_gate = _pair_8bit(w_gate, None, dim, 'w_gate', x[0])
+    hidden = w_gate[0].shape[0]
+    if not hidden:
+        raise ValueError('w_gate has no rows')
+    w_up, w_down = _pair_8bit(w_up, hidden, dim, 'w_up', x[0]), _pair_8bit(w_down, dim, hidden, 'w_down', x[0])
+    out = torch.empty(rows, dim, dtype=dtype, device=x[0].device)
+    if rows:
+        L = _lib.lib()
+        ws = _workspace_bytes(L.nf_gated_ff_fwd_8bit_workspace_bytes(rows, hidden), 'nf_gated_ff_fwd_8bit', out)
+        with prof.launch('nf_gated_ff_fwd_8bit', out, rows=rows, dim=dim, hidden=hidden):
+            _launch(L.nf_gated_ff_fwd_8bit, 'nf_gated_ff_fwd_8bit', out, *[_ptr(t) for pair in (x, w_gate, w_up, w_down) for t in pair], rows, dim, hidden,
+                    _FF_DTYPES[dtype], act, _ptr(out), _ptr(ws))
+    return out

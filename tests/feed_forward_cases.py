@@ -63,3 +63,82 @@ def check_gated(rows, dim, hidden, dtype, device, act='silu', frozen=False, seed
     leaves = [x] if frozen else [x, *ws]
     for key, got in zip(('dx', 'dw_gate', 'dw_up', 'dw_down'), torch.autograd.grad(out, leaves, dy)):
         near(got, want[key], key)
+
+
+# ---- 8 bits ----------------------------------------------------------------------------------------------------------------------
+def value_of(q, scale):
+    s = torch.exp2(scale.view(torch.uint8).double() - 127)
+    return q.double() * s.repeat_interleave(32, dim=-1)[..., :q.shape[-1]]
+
+
+def grid_step(v, scale):
+    """spacing of e4m3 at |v|, given 2^e per block"""
+    s = scale.repeat_interleave(32, dim=1)[:, :v.shape[1]]
+    return s * torch.exp2(torch.floor(torch.log2((v.abs() / s).clamp(min=2.0 ** -6))) - 3)
+
+
+def check_norm_8bit(rows, dim, dtype, device, residual=True, seed=0):
+    """every value within half a grid step (of the neighbouring grid point) of the float64 norm, up to what float32 can be off; the scales are the least
+    that hold the block, up to the same"""
+    gen = torch.Generator().manual_seed(seed + 11 * rows + dim)
+    x = normal(gen, rows, dim, dtype=dtype, device=device, scale=3.0)
+    r = normal(gen, rows, dim, dtype=dtype, device=device) if residual else None
+    w = (1 + 0.2 * torch.randn(dim, generator=gen)).to(dtype).to(device)
+    got = ff.rms_norm_8bit(x, w, r, eps=1e-5)
+    q, scale = got[:2]
+    assert q.dtype == torch.float8_e4m3fn and scale.dtype == torch.float8_e8m0fnu and q.shape == x.shape and scale.shape == (rows, -(-dim // 32))
+    want = ref.norm(x, w, r, 1e-5, dtype=dtype)
+    if residual:
+        near(got[2], want['h'], 'h')
+    y = want['y'][0]
+    off = (96 + dim // 256 + 4) * ref.U
+    lo, hi = ref.to_8bit(y * (1 - off))[1], ref.to_8bit(y * (1 + off))[1]
+    s = torch.exp2(scale.view(torch.uint8).double() - 127)
+    assert ((s == lo) | (s == hi)).all()
+    v = value_of(q, scale)
+    assert ((v - y).abs() <= 0.5 * torch.maximum(grid_step(v, s), grid_step(y, s)) + off * y.abs()).all()
+
+
+def check_quantize(rows, dim, dtype, device, seed=0):
+    """exact: the inputs are what is brought to 8 bits"""
+    gen = torch.Generator().manual_seed(seed + rows + dim)
+    x = normal(gen, rows, dim) * torch.exp2(torch.randint(-20, 12, (rows, 1), generator=gen).float())
+    if rows > 2:
+        x[1] = 0
+        x[2, ::3] = x[2, ::3].sign() * 448 * 2.0 ** -3          # a maximum on the border of two scales
+        x[2, 1::3] *= 1e-3
+    x = x.to(dtype).to(device)
+    q, scale = ff.quantize_8bit(x)
+    vq, vs = ref.to_8bit(x.double())
+    assert torch.equal(q.double(), vq) and torch.equal(torch.exp2(scale.view(torch.uint8).double() - 127), vs)
+
+
+def check_gated_8bit(rows, dim, hidden, device, act='silu', dtype=BF16, seed=0):
+    gen = torch.Generator().manual_seed(seed + rows + 3 * dim + 5 * hidden)
+    pairs = [ff.quantize_8bit(normal(gen, *s, device=device, scale=c)) for s, c in
+             (((rows, dim), 1.0), ((hidden, dim), dim ** -0.5), ((hidden, dim), dim ** -0.5), ((dim, hidden), hidden ** -0.5))]
+    out = ff.gated_feed_forward_8bit(*pairs, activation=act, dtype=dtype)
+    x, wg, wu, wd = (value_of(*p) for p in pairs)
+
+    def product8(p, q, e=None):
+        # for a bfloat16 result the matrix instruction multiplies e4m3 itself: of 16 consecutive products it drops what lies below 2^-12 of the power of
+        # two of the largest.  A product is below 4 times its power of two (mantissas below 2 each), so each of the 15 others loses less than
+        # 2^-12 times that power, at most 2^-12 of the largest; 15 * 2^-12 of the largest is at most 15 * 2^-12 of the 16 magnitudes' sum.
+        v, b = ref._product(p, e, q, None, False)
+        return v, b + (15 * 2.0 ** -12 * (p.abs() @ q.abs()) if dtype == BF16 else 0)
+
+    (g, eg), (u, eu) = (product8(x, w.t()) for w in (wg, wu))
+    a, _ = ref.act(act, g)
+    h = a * u
+    eh = ref.LIPSCHITZ[act][0] * eg * u.abs() + (a.abs() + eg) * eu + 20 * ref.U * (h.abs() + ref.U)
+    hq, s = ref.to_8bit(h)
+    hq = hq * s.repeat_interleave(32, dim=1)
+    # what a value that close to a border of the grid, or of two scales, may be off by: a step of the grid
+    tops = [ref.to_8bit(h.abs() + e)[1] for e in (eh, -eh.clamp(max=0))] + [ref.to_8bit((h.abs() - eh).clamp(min=0))[1]]
+    unsure = ((tops[0] != s) | (tops[2] != s)).repeat_interleave(32, dim=1)
+    step = grid_step(h, s)
+    frac = (h - hq).abs() / step
+    eq = torch.where((0.5 - frac) * step <= eh, step, torch.zeros_like(step))
+    eq = torch.where(unsure, 2 * step + 2.0 ** -9 * s.repeat_interleave(32, dim=1), eq)
+    v, e = product8(hq, wd.t(), eq)
+    near(out, (v, ref.rounded(v, e, dtype)), 'out')

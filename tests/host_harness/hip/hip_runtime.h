@@ -232,6 +232,53 @@ static inline nf_emu_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_f16(nf_emu_f16x8 
     }
     return d;
 }
+// D = A(32x64) * B(64x32) + C, e4m3 operands with a scale byte 2^(b - 127) per lane (byte `op` of the scale word).  lane l (r = l & 31, g = l >> 5) holds
+// k = 16 g + j in byte j < 16 and k = 32 + 16 g + j - 16 in byte j >= 16; its scale is that of k 32 g .. 32 g + 31.  (Formats 0, 0: e4m3.)
+typedef int nf_emu_i32x8 __attribute__((ext_vector_type(8)));
+static inline float nf_emu_e4m3(unsigned b) {
+    const unsigned e = (b >> 3) & 15, m = b & 7;
+    float v = e ? ldexpf((float)(8 + m), (int)e - 10) : ldexpf((float)m, -9);
+    if (e == 15 && m == 7) v = NAN;
+    return b & 0x80 ? -v : v;
+}
+static inline nf_emu_f32x16 __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(nf_emu_i32x8 a, nf_emu_i32x8 b, nf_emu_f32x16 c, int, int, int opa, int sa,
+                                                                             int opb, int sb) {
+    float own[2][32][64];
+    unsigned scale[2][64];
+    for (int w = 0; w < 2; ++w) {
+        const nf_emu_i32x8& src = w ? b : a;
+        for (int q = 0; q < 4; ++q) {
+            const uint64_t raw = (uint64_t)(unsigned)src[2 * q] | (uint64_t)(unsigned)src[2 * q + 1] << 32;
+            uint64_t* sl = hip_emu::wave_slots();
+            sl[hip_emu::lane()] = raw;
+            hip_emu::wave_barrier();
+            for (int l = 0; l < 64; ++l)
+                for (int j = 0; j < 8; ++j) {
+                    const int byte = 8 * q + j, g = l >> 5, k = byte < 16 ? 16 * g + byte : 32 + 16 * g + byte - 16;
+                    own[w][l & 31][k] = nf_emu_e4m3((unsigned)(sl[l] >> (8 * j)) & 255u);
+                }
+            hip_emu::wave_barrier();
+        }
+        uint64_t* sl = hip_emu::wave_slots();
+        sl[hip_emu::lane()] = (uint64_t)(((unsigned)(w ? sb : sa) >> (8 * (w ? opb : opa))) & 255u);
+        hip_emu::wave_barrier();
+        for (int l = 0; l < 64; ++l) scale[w][l] = (unsigned)sl[l];
+        hip_emu::wave_barrier();
+    }
+    nf_emu_f32x16 d = c;
+    const int l = hip_emu::lane(), col = l & 31, hi = l >> 5;
+    for (int r = 0; r < 16; ++r) {
+        const int row = (r & 3) + 8 * (r >> 2) + 4 * hi;
+        float acc = c[r];
+        for (int k = 0; k < 64; ++k) {
+            const int g = k >> 5;
+            const unsigned x = scale[0][row + 32 * g], y = scale[1][col + 32 * g];
+            acc += x == 255 || y == 255 ? NAN : ldexpf(own[0][row][k] * own[1][col][k], (int)x + (int)y - 254);
+        }
+        d[r] = acc;
+    }
+    return d;
+}
 // ds_read_b64_tr_b16: each lane reads 8 bytes at its own address; within 16 lanes, lane i gets element i % 4 of lanes 4 j + i / 4, j = 0 .. 3
 static inline uint64_t nf_emu_read_tr16(const char* p) {
     uint64_t raw;

@@ -68,3 +68,33 @@ def test_gated(rows, dim, hidden, dtype, act):
 def test_gated_large_tiles(dtype):
     """enough tiles for the largest tile form, with a ragged last tile each way"""
     cases.check_gated(2560 + 9, 1160, 2568, dtype, 'cuda', act='silu')
+
+
+NORM_8BIT_SMALL = [(1, 32, BF16), (5, 37, F32), (3, 129, F16), (70, 20, F32), (1, 2049, BF16)]
+GATED_8BIT_SMALL = [(1, 32, 32), (3, 64, 96), (33, 160, 32), (5, 96, 288)]
+
+
+@pytest.mark.parametrize('rows,dim,dtype', NORM_8BIT_SMALL)
+def test_norm_8bit_standin(emu, rows, dim, dtype):
+    cases.check_norm_8bit(rows, dim, dtype, emu)
+    cases.check_quantize(rows, dim, dtype, emu)
+
+
+@pytest.mark.parametrize('rows,dim,hidden', GATED_8BIT_SMALL)
+def test_gated_8bit_standin(emu, rows, dim, hidden):
+    cases.check_gated_8bit(rows, dim, hidden, emu, act=('silu', 'gelu', 'relu')[rows % 3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,dim,dtype', NORM_8BIT_SMALL + [(16, 5120, BF16), (2100, 1023, F32), (2049, 4097, F16), (2, 40000, F32), (513, 64, F32)])
+def test_norm_8bit(rows, dim, dtype):
+    cases.check_norm_8bit(rows, dim, dtype, 'cuda')
+    cases.check_norm_8bit(rows, dim, dtype, 'cuda', residual=False)
+    cases.check_quantize(rows, dim, dtype, 'cuda')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act,dtype', [('silu', BF16), ('gelu', F32), ('relu', F16)])
+@pytest.mark.parametrize('rows,dim,hidden', GATED_8BIT_SMALL + [(1, 4096, 1024), (16, 256, 512), (129, 1056, 544), (700, 320, 2080), (2569, 1184, 2592)])
+def test_gated_8bit(rows, dim, hidden, act, dtype):
+    cases.check_gated_8bit(rows, dim, hidden, 'cuda', act=act, dtype=dtype)
