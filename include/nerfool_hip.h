@@ -433,7 +433,7 @@ int nf_in_act_pad_bwd(const float* dy_padded, const float* d_extra, const float*
  *   whole number with max|block| <= 448 2^e; q [rows, dim] e4m3 of v / 2^e (a block with an infinity or NaN: byte 255, q NaN).
  *   rstd (nullable, [rows] float): what nf_rms_norm_bwd reads.
  * nf_rms_norm_bwd: dx = rstd (w dy - xhat mean(w dy xhat)) + dh (nullable), the gradient of x and of residual alike; dweight (nullable) =
- *   sum over rows of dy xhat, which needs a workspace of nf_rms_norm_bwd_workspace_floats(dim) floats.  Sums are in a fixed order.
+ *   sum over rows of dy xhat, xhat = (h + residual) rstd (residual nullable: h is the sum already), which needs a workspace of nf_rms_norm_bwd_workspace_floats(dim) floats.  Sums are in a fixed order.
  * nf_quantize_8bit: x itself in that 8-bit form.
  *
  * nf_gated_ff_fwd: out [rows, dim] = (act(x Wg^T) * (x Wu^T)) Wd^T; Wg, Wu [hidden, dim], Wd [dim, hidden].  g_save, u_save (nullable, together):
@@ -446,7 +446,7 @@ int nf_in_act_pad_bwd(const float* dy_padded, const float* d_extra, const float*
 int nf_rms_norm_fwd(const void* x, const void* residual, const void* weight, int64_t rows, int dim, int dtype, float eps, void* h, void* y,
                     uint8_t* q, uint8_t* scale, float* rstd, nf_stream_t stream);
 int64_t nf_rms_norm_bwd_workspace_floats(int dim);
-int nf_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, const float* rstd, int64_t rows, int dim, int dtype,
+int nf_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* residual, const void* weight, const float* rstd, int64_t rows, int dim, int dtype,
                     void* dx, void* dweight, float* workspace, nf_stream_t stream);
 int nf_quantize_8bit(const void* x, int64_t rows, int dim, int dtype, uint8_t* q, uint8_t* scale, nf_stream_t stream);
 int64_t nf_gated_ff_fwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype);

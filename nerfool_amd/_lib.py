@@ -125,7 +125,7 @@ _PROTOTYPES = {
     'nf_pgd_adam_step_dev': (c_int, [_P, _P, _P, _P, _P, c_int64, _P, c_float, c_float, c_float, c_float, c_float, c_float, c_float, _P]),
     'nf_rms_norm_fwd': (c_int, [_P, _P, _P, c_int64, c_int, c_int, c_float, _P, _P, _P, _P, _P, _P]),
     'nf_rms_norm_bwd_workspace_floats': (c_int64, [c_int]),
-    'nf_rms_norm_bwd': (c_int, [_P, _P, _P, _P, _P, c_int64, c_int, c_int, _P, _P, _P, _P]),
+    'nf_rms_norm_bwd': (c_int, [_P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, _P, _P, _P, _P]),
     'nf_quantize_8bit': (c_int, [_P, c_int64, c_int, c_int, _P, _P, _P]),
     'nf_gated_ff_fwd_workspace_bytes': (c_int64, [c_int64, c_int, c_int, c_int]),
     'nf_gated_ff_fwd': (c_int, [_P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P]),

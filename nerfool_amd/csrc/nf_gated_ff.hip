@@ -9,6 +9,7 @@
 // h, dg and du are rounded once, to the inputs' type, because they are operands of a matrix product in that type.  float32 inputs are split into
 // three bf16 parts (8 + 8 + 8 bits, exact) and multiplied as six products of order <= 2^-16: float32-grade sums at 16 / 6 of the float32 pipe's rate.
 #include "nf_ff_gemm.h"
+#include "nf_ff_rows.h"
 
 namespace {
 
@@ -291,9 +292,23 @@ struct FwdPlan {
     }
 };
 
+// Up to this many rows the weights' bytes bound the block and k_ff_rows streams them; above, the tiles of k_ff_gemm read them once for more tokens.
+constexpr int FF_ROWS_MAX = 64;
+
+template <typename T, bool GATED>
+int few_rows(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, hipStream_t st) {
+    if (M <= 16) return ff_rows_launch<T, 1, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+    if (M <= 32) return ff_rows_launch<T, 2, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+    return ff_rows_launch<T, 4, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+}
+
 template <typename T>
 int ff_fwd(const void* x, const void* wg, const void* wu, const void* wd, int M, int D, int F, int act, void* out, float* g_save, float* u_save,
            void* workspace, hipStream_t st) {
+    if (M <= FF_ROWS_MAX) {
+        FF_TRY((few_rows<T, true>(wg, wu, x, M, F, D, workspace, g_save, u_save, act, st)));
+        return few_rows<T, false>(wd, nullptr, workspace, M, D, F, out, nullptr, nullptr, 0, st);
+    }
     FwdPlan<T> f((char*)workspace, M, D, F);
     pack_run<T>(x, M, D, f.x, st);
     pack_run<T>(wg, F, D, f.wg, st);
@@ -370,6 +385,7 @@ bool ff_sizes_ok(const char* what, int64_t M, int D, int F, int dtype, int act) 
 
 extern "C" int64_t nf_gated_ff_fwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype) {
     if (!ff_sizes_ok("nf_gated_ff_fwd_workspace_bytes", rows, dim, hidden, dtype, 0)) return -1;
+    if (rows <= FF_ROWS_MAX) return rows * hidden * (dtype == FF_F32 ? 4 : 2);          // h
     if (dtype == FF_F32) return FwdPlan<float>(nullptr, rows, dim, hidden).bytes;
     return FwdPlan<ff_bf16>(nullptr, rows, dim, hidden).bytes;
 }

@@ -12,6 +12,7 @@
 // or float32 result's it is not.  For those the values are multiplied as bfloat16, which holds value and scale exactly, on
 // v_mfma_f32_32x32x16_bf16: float32 sums, at half the rate; v_cvt_scalef32_pk_bf16_fp8 makes two operands of two values and their scale.
 #include "nf_ff_gemm.h"
+#include "nf_ff_rows.h"
 
 typedef int ff_i32x8 __attribute__((ext_vector_type(8)));
 
@@ -160,6 +161,158 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
     }
 }
 
+// few rows (nf_ff_rows.h): 32 weight rows a workgroup, so that the features of an h block are one workgroup's; 128 values of k a unit, whose scales are a
+// word a row; 16 values a lane and step, as two bfloat16 operands
+template <int NT, bool GATED, typename T>
+__global__ void __launch_bounds__(1024) k_ff_rows8(const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1, FfScales sw, const uint8_t* __restrict__ x,
+                                                   const uint8_t* __restrict__ xs, int M, int N, int K, T* __restrict__ out, uint8_t* __restrict__ hq,
+                                                   uint8_t* __restrict__ hs, int act) {
+    constexpr int NW = GATED ? 2 : 1, U = 2, UNIT = 128;
+    HIP_DYNAMIC_SHARED(ff_f32x4, part)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int r = lane & 15, q = lane >> 4, n0 = blockIdx.x * 32, blocks = K / 32;
+    const uint8_t *wr[NW][2], *ws[NW][2], *xr[NT], *xsr[NT];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {          // (N is a multiple of 32)
+        const int64_t n = n0 + 16 * h + r;
+        wr[0][h] = w0 + n * K;
+        ws[0][h] = sw.a + n * sw.pitch;
+        if (GATED) {
+            wr[NW - 1][h] = w1 + n * K;
+            ws[NW - 1][h] = sw.b + n * sw.pitch;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int64_t m = 16 * t + r < M ? 16 * t + r : M - 1;
+        xr[t] = x + m * K;
+        xsr[t] = xs + m * blocks;
+    }
+    ff_f32x4 acc[NW][2][NT];
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[i][h][t] = ff_f32x4{0.f, 0.f, 0.f, 0.f};
+    ff_u32x4 a[2][U][NW][2], b[2][U][NT];
+    unsigned as[2][NW][2], bs[2][NT];
+    auto fetch = [&](int s, int k0) {
+        const ff_u32x4 none = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int k = k0 + 64 * j + 16 * q;
+            const bool in = k < K;
+#pragma unroll
+            for (int i = 0; i < NW; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) a[s][j][i][h] = in ? *reinterpret_cast<const ff_u32x4*>(wr[i][h] + k) : none;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) b[s][j][t] = in ? *reinterpret_cast<const ff_u32x4*>(xr[t] + k) : none;
+        }
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) as[s][i][h] = ff_scale_word(ws[i][h], k0 / 32, blocks);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) bs[s][t] = ff_scale_word(xsr[t], k0 / 32, blocks);
+    };
+    auto multiply = [&](int s) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int sh = 8 * (2 * j + (q >> 1));
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {          // bytes 0 .. 7 and 8 .. 15 of the lane's 16
+                ff_bf16x8 bv[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) bv[t] = ff_from_e4m3x8(b[s][j][t][2 * p], b[s][j][t][2 * p + 1], (bs[s][t] >> sh) & 255u);
+#pragma unroll
+                for (int i = 0; i < NW; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const ff_bf16x8 av = ff_from_e4m3x8(a[s][j][i][h][2 * p], a[s][j][i][h][2 * p + 1], (as[s][i][h] >> sh) & 255u);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[i][h][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv[t], acc[i][h][t], 0, 0, 0);
+                    }
+            }
+        }
+    };
+    const int stride = waves * UNIT;
+    int k0 = wave * UNIT;
+    if (k0 < K) fetch(0, k0);
+    while (k0 < K) {
+        if (k0 + stride < K) fetch(1, k0 + stride);
+        multiply(0);
+        k0 += stride;
+        if (k0 >= K) break;
+        if (k0 + stride < K) fetch(0, k0 + stride);
+        multiply(1);
+        k0 += stride;
+    }
+    constexpr int FRAGS = NW * 2 * NT;
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) part[(wave * FRAGS + (i * 2 + h) * NT + t) * 64 + lane] = acc[i][h][t];
+    __syncthreads();
+    for (int t = wave; t < NT; t += waves) {
+        const int m = 16 * t + r;
+        ff_f32x4 v[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[h] = ff_rows_total(part, waves, FRAGS, h * NT + t, lane);
+        if (GATED) {
+            float top = 0.f;
+            bool bad = false;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const ff_f32x4 u = ff_rows_total(part, waves, FRAGS, ((NW - 1) * 2 + h) * NT + t, lane);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float ac, slope;
+                    ff_act(act, v[h][c], ac, slope);
+                    v[h][c] = ac * u[c];
+                    top = fmaxf(top, fabsf(v[h][c]));
+                    bad |= !(fabsf(v[h][c]) <= 3.4028235e38f);
+                }
+            }
+            if (bad) top = INFINITY;
+            top = fmaxf(top, __shfl_xor(top, 16, NF_WAVE));          // the 32 features of a token are on 4 lanes
+            top = fmaxf(top, __shfl_xor(top, 32, NF_WAVE));
+            const unsigned byte = ff_scale_byte(top);
+            const float inv = byte == 255u ? NAN : ff_scale_inverse(byte);
+            if (m < M) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<unsigned*>(hq + (int64_t)m * N + n0 + 16 * h + 4 * q) =
+                        ff_e4m3x4(v[h][0] * inv, v[h][1] * inv, v[h][2] * inv, v[h][3] * inv);
+                if (q == 0) hs[(int64_t)m * (N / 32) + blockIdx.x] = (uint8_t)byte;
+            }
+        } else if (m < M) {
+            typedef T V4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<V4*>(out + (int64_t)m * N + n0 + 16 * h + 4 * q) = V4{(T)v[h][0], (T)v[h][1], (T)v[h][2], (T)v[h][3]};
+        }
+    }
+}
+
+template <int NT, bool GATED, typename T>
+void rows8(const void* w0, const void* w1, const FfScales& sw, const void* x, const uint8_t* xs, int M, int N, int K, T* out, uint8_t* hq, uint8_t* hs, int act,
+           hipStream_t st) {
+    const int waves = ff_rows_waves(N / 32, (K + 127) / 128, GATED && NT >= 2 ? (NT >= 4 ? 4 : 8) : 16);          // (64 KB of LDS at most)
+    hipLaunchKernelGGL((k_ff_rows8<NT, GATED, T>), dim3(N / 32), dim3(64 * waves), (size_t)waves * (GATED ? 4 : 2) * NT * 1024, st, (const uint8_t*)w0,
+                       (const uint8_t*)w1, sw, (const uint8_t*)x, xs, M, N, K, out, hq, hs, act);
+}
+template <bool GATED, typename T>
+void few_rows8(const void* w0, const void* w1, const FfScales& sw, const void* x, const uint8_t* xs, int M, int N, int K, T* out, uint8_t* hq, uint8_t* hs, int act,
+               hipStream_t st) {
+    if (M <= 16) rows8<1, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
+    else if (M <= 32) rows8<2, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
+    else rows8<4, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
+}
+
 template <typename T>
 struct Epi8Store {
     T* out;
@@ -257,6 +410,15 @@ extern "C" int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const
     const Epi8Gate gate = {hq, hs, F, activation};
     const FfOperand pg = operand8(w_gate, w_up, F, D), qx = operand8(x, x, M, D);
     const FfScales spg = {gate_scale, up_scale, D / 32, F}, sqx = {x_scale, x_scale, D / 32, M};
+    if (M <= 64) {
+        few_rows8<true, float>(w_gate, w_up, spg, x, x_scale, M, F, D, nullptr, hq, hs, activation, st);
+        const FfScales sd = {down_scale, down_scale, F / 32, D};
+        if (out_dtype == FF_F32) few_rows8<false, float>(w_down, nullptr, sd, hq, hs, M, D, F, (float*)out, nullptr, nullptr, 0, st);
+        else if (out_dtype == FF_BF16) few_rows8<false, ff_bf16>(w_down, nullptr, sd, hq, hs, M, D, F, (ff_bf16*)out, nullptr, nullptr, 0, st);
+        else few_rows8<false, ff_half>(w_down, nullptr, sd, hq, hs, M, D, F, (ff_half*)out, nullptr, nullptr, 0, st);
+        NF_LAUNCH_CHECK("nf_gated_ff_fwd_8bit");
+        return 0;
+    }
     int rc = out_dtype == FF_BF16 ? product8<true, false>(pg, qx, spg, sqx, M, F, D, gate, st) : product8<true, true>(pg, qx, spg, sqx, M, F, D, gate, st);
     if (rc) return rc;
     const FfOperand p = operand8(w_down, w_down, D, F), q = operand8(hq, hq, M, F);

@@ -22,15 +22,15 @@ struct RmsArgs {
 };
 
 // sum over the TPR threads of a row; TPR <= 64: a butterfly inside the wave, else over the waves of the workgroup (`part`: one float a wave)
-template <int TPR>
-__device__ __forceinline__ float rms_row_sum(float v, float* part) {
+template <int TPR, typename A>
+__device__ __forceinline__ A rms_row_sum(A v, A* part) {
 #pragma unroll
     for (int m = (TPR < 64 ? TPR : 64) / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, NF_WAVE);
     if (TPR > 64) {
         __syncthreads();          // the previous row's sums have been read
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = 0.f;
+        v = 0;
 #pragma unroll
         for (int i = 0; i < TPR / 64; ++i) v += part[i];
     }
@@ -69,12 +69,24 @@ __device__ __forceinline__ void rms_store_8bit(uint8_t* q, uint8_t* s, int c, in
     }
 }
 
+// y of an 8-bit row is made in double, of the float sums x + r: a value next to a border of the grid takes the neighbouring step for an error of
+// one part in 2^24, and beside the memory's time the doubles cost nothing
+template <int MODE>
+struct RmsAcc {
+    typedef float A;
+};
+template <>
+struct RmsAcc<1> {
+    typedef double A;
+};
+
 enum { RMS_SAME = 0, RMS_8BIT = 1, RMS_QUANT = 2 };          // y in the inputs' type; y in 8 bits; x itself in 8 bits
 
 template <typename T, int TPR, int NV, int MODE>
 __global__ void __launch_bounds__(TPR <= 256 ? 256 : TPR) k_rms_fwd(RmsArgs a) {
+    typedef typename RmsAcc<MODE>::A A;
     constexpr int N = FfVec<T>::N, BLOCK = TPR <= 256 ? 256 : TPR, RPB = TPR <= 64 ? BLOCK / TPR : 1;
-    __shared__ float part[16];
+    __shared__ A part[16];
     const int t = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x, sub = TPR <= 64 ? threadIdx.x / TPR : 0;
     const int dim = a.dim;
     float w[NV][N];
@@ -93,7 +105,7 @@ __global__ void __launch_bounds__(TPR <= 256 ? 256 : TPR) k_rms_fwd(RmsArgs a) {
         const bool live = row < a.rows;
         const int64_t at = (live ? row : a.rows - 1) * dim;
         float v[NV][N];
-        float sq = 0.f;
+        A sq = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             ff_load_row((const T*)a.x + at, (j * TPR + t) * N, dim, v[j]);
@@ -108,10 +120,10 @@ __global__ void __launch_bounds__(TPR <= 256 ? 256 : TPR) k_rms_fwd(RmsArgs a) {
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int i = 0; i < N; ++i) sq = fmaf(v[j][i], v[j][i], sq);
+                for (int i = 0; i < N; ++i) sq = fma((A)v[j][i], (A)v[j][i], sq);
             sq = rms_row_sum<TPR>(sq, part);
-            const float rstd = 1.f / sqrtf(sq / (float)dim + a.eps);
-            if (a.rstd && t == 0 && live) a.rstd[row] = rstd;
+            const A rstd = (A)1 / sqrt(sq / (A)dim + (A)a.eps);
+            if (a.rstd && t == 0 && live) a.rstd[row] = (float)rstd;
             if (a.h && live) {
 #pragma unroll
                 for (int j = 0; j < NV; ++j) ff_store_row((T*)a.h + at, (j * TPR + t) * N, dim, v[j]);
@@ -119,7 +131,7 @@ __global__ void __launch_bounds__(TPR <= 256 ? 256 : TPR) k_rms_fwd(RmsArgs a) {
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[j][i] = v[j][i] * rstd * w[j][i];
+                for (int i = 0; i < N; ++i) v[j][i] = (float)((A)v[j][i] * rstd * (A)w[j][i]);
         }
         if (MODE == RMS_SAME) {
             if (live) {
@@ -138,26 +150,28 @@ __global__ void __launch_bounds__(TPR <= 256 ? 256 : TPR) k_rms_fwd(RmsArgs a) {
 // rows of any length, read twice: a workgroup per row
 template <typename T, int MODE>
 __global__ void __launch_bounds__(1024) k_rms_fwd_long(RmsArgs a) {
+    typedef typename RmsAcc<MODE>::A A;
     constexpr int N = FfVec<T>::N, STEP = 1024 * N;
-    __shared__ float part[16];
+    __shared__ A part[16];
     const int dim = a.dim;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const int64_t at = row * dim;
-        float rstd = 1.f, v[N], r[N], w[N];
+        float v[N], r[N], w[N];
+        A rstd = 1;
         if (MODE != RMS_QUANT) {
-            float sq = 0.f;
+            A sq = 0;
             for (int c = threadIdx.x * N; c < dim; c += STEP) {
                 ff_load_row((const T*)a.x + at, c, dim, v);
                 if (a.r) {
                     ff_load_row((const T*)a.r + at, c, dim, r);
                     for (int i = 0; i < N; ++i) v[i] += r[i];
                 }
-                for (int i = 0; i < N; ++i) sq = fmaf(v[i], v[i], sq);
+                for (int i = 0; i < N; ++i) sq = fma((A)v[i], (A)v[i], sq);
                 if (a.h) ff_store_row((T*)a.h + at, c, dim, v);
             }
             sq = rms_row_sum<1024>(sq, part);
-            rstd = 1.f / sqrtf(sq / (float)dim + a.eps);
-            if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+            rstd = (A)1 / sqrt(sq / (A)dim + (A)a.eps);
+            if (a.rstd && threadIdx.x == 0) a.rstd[row] = (float)rstd;
         }
         for (int c0 = 0; c0 < dim; c0 += STEP) {          // every lane stays for the block maxima
             const int c = c0 + threadIdx.x * N;
@@ -169,7 +183,7 @@ __global__ void __launch_bounds__(1024) k_rms_fwd_long(RmsArgs a) {
                 }
                 for (int i = 0; i < N; ++i) w[i] = 1.f;
                 if (a.w) ff_load_row((const T*)a.w, c, dim, w);
-                for (int i = 0; i < N; ++i) v[i] = v[i] * rstd * w[i];
+                for (int i = 0; i < N; ++i) v[i] = (float)((A)v[i] * rstd * (A)w[i]);
             }
             if (MODE == RMS_SAME)
                 ff_store_row((T*)a.y + at, c, dim, v);
@@ -180,13 +194,25 @@ __global__ void __launch_bounds__(1024) k_rms_fwd_long(RmsArgs a) {
 }
 
 struct RmsBwdArgs {
-    const void *dy, *dh, *h, *w;
+    const void *dy, *dh, *h, *r, *w;          // r: nullable, added to h
     const float* rstd;
     void* dx;
     float* partial;          // [gridDim.x][dim], nullable (dw not asked for)
     int64_t rows;
     int dim;
 };
+
+// h's values, or x + r
+template <typename T>
+__device__ __forceinline__ void rms_load_h(const RmsBwdArgs& a, int64_t at, int c, float* v) {
+    ff_load_row((const T*)a.h + at, c, a.dim, v);
+    if (a.r) {
+        float r[FfVec<T>::N];
+        ff_load_row((const T*)a.r + at, c, a.dim, r);
+#pragma unroll
+        for (int i = 0; i < FfVec<T>::N; ++i) v[i] += r[i];
+    }
+}
 
 template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(TPR <= 256 ? 256 : TPR) k_rms_bwd(RmsBwdArgs a) {
@@ -214,7 +240,7 @@ __global__ void __launch_bounds__(TPR <= 256 ? 256 : TPR) k_rms_bwd(RmsBwdArgs a
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             ff_load_row((const T*)a.dy + at, (j * TPR + t) * N, dim, g[j]);
-            ff_load_row((const T*)a.h + at, (j * TPR + t) * N, dim, xh[j]);
+            rms_load_h<T>(a, at, (j * TPR + t) * N, xh[j]);
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -274,7 +300,7 @@ __global__ void __launch_bounds__(1024) k_rms_bwd_long(RmsBwdArgs a) {
             for (int i = 0; i < N; ++i) w[i] = 1.f;
             if (a.w) ff_load_row((const T*)a.w, c, dim, w);
             ff_load_row((const T*)a.dy + at, c, dim, g);
-            ff_load_row((const T*)a.h + at, c, dim, xh);
+            rms_load_h<T>(a, at, c, xh);
             for (int i = 0; i < N; ++i) dot = fmaf(g[i] * w[i], xh[i] * rstd, dot);
         }
         dot = rms_row_sum<1024>(dot, part) / (float)dim;
@@ -283,7 +309,7 @@ __global__ void __launch_bounds__(1024) k_rms_bwd_long(RmsBwdArgs a) {
             if (a.w) ff_load_row((const T*)a.w, c, dim, w);
             if (a.dh) ff_load_row((const T*)a.dh + at, c, dim, d);
             ff_load_row((const T*)a.dy + at, c, dim, g);
-            ff_load_row((const T*)a.h + at, c, dim, xh);
+            rms_load_h<T>(a, at, c, xh);
             for (int i = 0; i < N; ++i) d[i] = fmaf(rstd, g[i] * w[i] - xh[i] * rstd * dot, d[i]);
             ff_store_row((T*)a.dx + at, c, dim, d);
         }
@@ -296,7 +322,7 @@ __global__ void __launch_bounds__(256) k_rms_dw_long(RmsBwdArgs a) {
     if (c >= a.dim) return;
     float s = 0.f;
     for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y)
-        s = fmaf((float)((const T*)a.dy)[row * a.dim + c], (float)((const T*)a.h)[row * a.dim + c] * a.rstd[row], s);
+        s = fmaf((float)((const T*)a.dy)[row * a.dim + c], ((float)((const T*)a.h)[row * a.dim + c] + (a.r ? (float)((const T*)a.r)[row * a.dim + c] : 0.f)) * a.rstd[row], s);
     a.partial[(int64_t)blockIdx.y * a.dim + c] = s;
 }
 
@@ -403,12 +429,12 @@ extern "C" int nf_rms_norm_fwd(const void* x, const void* residual, const void* 
 
 extern "C" int64_t nf_rms_norm_bwd_workspace_floats(int dim) { return (int64_t)RMS_MAX_PARTIALS * dim; }
 
-extern "C" int nf_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, const float* rstd, int64_t rows, int dim,
+extern "C" int nf_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* residual, const void* weight, const float* rstd, int64_t rows, int dim,
                                int dtype, void* dx, void* dweight, float* workspace, nf_stream_t stream) {
     NF_REQUIRE(rows >= 1 && dim >= 1 && dim <= (1 << 24) && dtype >= FF_F32 && dtype <= FF_F16,
                "nf_rms_norm_bwd: need rows >= 1, 1 <= dim <= 2^24, dtype in 0 .. 2 (got rows %lld dim %d dtype %d)", (long long)rows, dim, dtype);
     NF_REQUIRE(!dweight || workspace, "nf_rms_norm_bwd: dweight needs a workspace");
-    const RmsBwdArgs a = {dy, dh, h, weight, rstd, dx, dweight ? workspace : nullptr, rows, dim};
+    const RmsBwdArgs a = {dy, dh, h, residual, weight, rstd, dx, dweight ? workspace : nullptr, rows, dim};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == FF_F32) rms_bwd<float>(a, dweight, st);
     else if (dtype == FF_BF16) rms_bwd<ff_bf16>(a, dweight, st);

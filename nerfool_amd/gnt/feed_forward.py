@@ -27,7 +27,11 @@ from .. import ops
 def _rows(t, name):
     if t.dim() < 1 or not t.shape[-1]:
         raise ValueError('%s must have a last axis of at least one value (got the shape %s)' % (name, tuple(t.shape)))
-    return t.reshape(-1, t.shape[-1])
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])          # (a view is a node of its own in the backward pass)
+
+
+def _as(t, shape):
+    return t if t.dim() == len(shape) else t.reshape(shape)
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -37,17 +41,22 @@ class _RMSNorm(torch.autograd.Function):
         h, y, rstd = ops.rms_norm_fwd(x, weight, residual, eps, want_rstd=need)
         ctx.set_materialize_grads(False)
         if need:
-            ctx.save_for_backward(x if h is None else h, weight, rstd)
+            # the gradient of the weight is a sum of dy * xhat over the rows: from h as rounded to 16 bits it would carry that rounding beside its own,
+            # so x and the residual are kept and added again; in float32, and for the gradient of x alone, h as stored is as good and half the reading
+            if h is None or (ctx.needs_input_grad[1] and x.dtype != torch.float32):
+                ctx.save_for_backward(x, residual, weight, rstd)
+            else:
+                ctx.save_for_backward(h, None, weight, rstd)
         return (y, h) if h is not None else y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
+        h, residual, weight, rstd = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if dy is None:          # only the sum was used
             return (dh if need_x else None, torch.zeros_like(weight) if need_w else None, dh if need_r else None, None)
-        dx, dw = ops.rms_norm_bwd(dy, dh, h, weight, rstd, need_w)
+        dx, dw = ops.rms_norm_bwd(dy, dh, h, residual, weight, rstd, need_w)
         return dx if need_x else None, dw, dx if need_r else None, None
 
 
@@ -57,8 +66,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
         raise ValueError('residual has the shape %s, x %s' % (tuple(residual.shape), tuple(x.shape)))
     got = _RMSNorm.apply(_rows(x, 'x'), weight, None if residual is None else _rows(residual, 'residual'), float(eps))
     if residual is None:
-        return got.reshape(x.shape)
-    return got[0].reshape(x.shape), got[1].reshape(x.shape)
+        return _as(got, x.shape)
+    return _as(got[0], x.shape), _as(got[1], x.shape)
 
 
 def _no_gradient(what, tensors):
@@ -104,7 +113,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation='silu'):
     """x [..., dim], w_gate, w_up [hidden, dim], w_down [dim, hidden] -> [..., dim]; activation: 'silu', 'gelu' (the error function), 'relu'.
     Constant weights (requires_grad False, as everywhere in an attack) cost no gradient of their own."""
     ops.ff_activation(activation)
-    return _GatedFeedForward.apply(_rows(x, 'x'), w_gate, w_up, w_down, activation).reshape(x.shape)
+    return _as(_GatedFeedForward.apply(_rows(x, 'x'), w_gate, w_up, w_down, activation), x.shape)
 
 
 def gated_feed_forward_8bit(x, w_gate, w_up, w_down, activation='silu', dtype=torch.bfloat16):

@@ -976,6 +976,14 @@ _FF_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FF_ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
 
 
+def _ff_launch(name, t, meta, *args):
+    """_launch, bracketed for a kernel timer only where one runs: the context manager costs a tenth of a one-token call"""
+    if prof._active is None:
+        return _launch(getattr(_lib.lib(), name), name, t, *args)
+    with prof.launch(name, t, **meta):
+        _launch(getattr(_lib.lib(), name), name, t, *args)
+
+
 def _ff(t, name, like=None):
     """contiguous, 16-byte aligned, of a supported type; with `like`: of its type and on its device"""
     if t.dtype not in _FF_DTYPES:
@@ -991,7 +999,7 @@ def _ff(t, name, like=None):
 
 
 def _ff_shape(t, shape, name):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError('%s has the shape %s, not %s' % (name, tuple(t.shape), tuple(shape)))
     return t
 
@@ -1019,8 +1027,7 @@ def rms_norm_fwd(x, weight, residual, eps, quantize=False, want_rstd=False):
     else:
         y = torch.empty_like(x)
     if rows:
-        with prof.launch('nf_rms_norm_fwd', x, rows=rows, dim=dim):
-            _launch(_lib.lib().nf_rms_norm_fwd, 'nf_rms_norm_fwd', x, _ptr(x), _ptr(residual), _ptr(weight), rows, dim, _FF_DTYPES[x.dtype], float(eps),
+        _ff_launch('nf_rms_norm_fwd', x, dict(rows=rows, dim=dim), _ptr(x), _ptr(residual), _ptr(weight), rows, dim, _FF_DTYPES[x.dtype], float(eps),
                     _ptr(h), _ptr(y), _ptr(q), _ptr(scale), _ptr(rstd))
     return h, (q, scale) if quantize else y, rstd
 
@@ -1030,9 +1037,11 @@ def _empty_8bit(rows, dim, device):
             torch.empty(rows, (dim + 31) // 32, dtype=torch.float8_e8m0fnu, device=device))
 
 
-def rms_norm_bwd(dy, dh, h, weight, rstd, want_dweight):
-    """-> (dx, dweight or None); dh: or None"""
+def rms_norm_bwd(dy, dh, h, residual, weight, rstd, want_dweight):
+    """h: the sum as stored, or x with its residual (else None) -> (dx, dweight or None); dh: or None"""
     h = _ff(h, 'h')
+    if residual is not None:
+        residual = _ff(residual, 'residual', h)
     dy = _ff_shape(_ff(dy, 'dy', h), h.shape, 'dy')
     if dh is not None:
         dh = _ff_shape(_ff(dh, 'dh', h), h.shape, 'dh')
@@ -1046,8 +1055,7 @@ def rms_norm_bwd(dy, dh, h, weight, rstd, want_dweight):
     if want_dweight:
         dw = torch.empty(dim, dtype=h.dtype, device=h.device)
         ws = torch.empty(_lib.lib().nf_rms_norm_bwd_workspace_floats(dim), dtype=torch.float32, device=h.device)
-    with prof.launch('nf_rms_norm_bwd', h, rows=rows, dim=dim):
-        _launch(_lib.lib().nf_rms_norm_bwd, 'nf_rms_norm_bwd', h, _ptr(dy), _ptr(dh), _ptr(h), _ptr(weight), _ptr(rstd), rows, dim, _FF_DTYPES[h.dtype],
+    _ff_launch('nf_rms_norm_bwd', h, dict(rows=rows, dim=dim), _ptr(dy), _ptr(dh), _ptr(h), _ptr(residual), _ptr(weight), _ptr(rstd), rows, dim, _FF_DTYPES[h.dtype],
                 _ptr(dx), _ptr(dw), _ptr(ws))
     return dx, dw
 
@@ -1058,8 +1066,7 @@ def quantize_8bit(x):
     rows, dim = x.shape
     q, scale = _empty_8bit(rows, dim, x.device)
     if rows:
-        with prof.launch('nf_quantize_8bit', x, rows=rows, dim=dim):
-            _launch(_lib.lib().nf_quantize_8bit, 'nf_quantize_8bit', x, _ptr(x), rows, dim, _FF_DTYPES[x.dtype], _ptr(q), _ptr(scale))
+        _ff_launch('nf_quantize_8bit', x, dict(rows=rows, dim=dim), _ptr(x), rows, dim, _FF_DTYPES[x.dtype], _ptr(q), _ptr(scale))
     return q, scale
 
 
@@ -1083,8 +1090,7 @@ def gated_ff_fwd(x, w_gate, w_up, w_down, activation, save=False):
     if rows:
         L = _lib.lib()
         ws = _workspace_bytes(L.nf_gated_ff_fwd_workspace_bytes(rows, dim, hidden, _FF_DTYPES[x.dtype]), 'nf_gated_ff_fwd', x)
-        with prof.launch('nf_gated_ff_fwd', x, rows=rows, dim=dim, hidden=hidden):
-            _launch(L.nf_gated_ff_fwd, 'nf_gated_ff_fwd', x, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), rows, dim, hidden, _FF_DTYPES[x.dtype], act,
+        _ff_launch('nf_gated_ff_fwd', x, dict(rows=rows, dim=dim, hidden=hidden), _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), rows, dim, hidden, _FF_DTYPES[x.dtype], act,
                     _ptr(out), _ptr(g), _ptr(u), _ptr(ws))
     return out, g, u
 
@@ -1108,8 +1114,7 @@ def gated_ff_bwd(x, w_gate, w_up, w_down, dy, g, u, activation, want):
         L = _lib.lib()
         ws = _workspace_bytes(L.nf_gated_ff_bwd_workspace_bytes(rows, dim, hidden, _FF_DTYPES[x.dtype], int(bool(want[0])), int(bool(want[1] or want[2])),
                                                                 int(bool(want[3]))), 'nf_gated_ff_bwd', x)
-        with prof.launch('nf_gated_ff_bwd', x, rows=rows, dim=dim, hidden=hidden):
-            _launch(L.nf_gated_ff_bwd, 'nf_gated_ff_bwd', x, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(dy), _ptr(g), _ptr(u), rows, dim, hidden,
+        _ff_launch('nf_gated_ff_bwd', x, dict(rows=rows, dim=dim, hidden=hidden), _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(dy), _ptr(g), _ptr(u), rows, dim, hidden,
                     _FF_DTYPES[x.dtype], act, *[_ptr(t) for t in grads], _ptr(ws))
     return grads
 
@@ -1147,7 +1152,6 @@ def gated_ff_fwd_8bit(x, w_gate, w_up, w_down, activation, dtype):
     if rows:
         L = _lib.lib()
         ws = _workspace_bytes(L.nf_gated_ff_fwd_8bit_workspace_bytes(rows, hidden), 'nf_gated_ff_fwd_8bit', out)
-        with prof.launch('nf_gated_ff_fwd_8bit', out, rows=rows, dim=dim, hidden=hidden):
-            _launch(L.nf_gated_ff_fwd_8bit, 'nf_gated_ff_fwd_8bit', out, *[_ptr(t) for pair in (x, w_gate, w_up, w_down) for t in pair], rows, dim, hidden,
+        _ff_launch('nf_gated_ff_fwd_8bit', out, dict(rows=rows, dim=dim, hidden=hidden), *[_ptr(t) for pair in (x, w_gate, w_up, w_down) for t in pair], rows, dim, hidden,
                     _FF_DTYPES[dtype], act, _ptr(out), _ptr(ws))
     return out

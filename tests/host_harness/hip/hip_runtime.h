@@ -279,6 +279,24 @@ static inline nf_emu_f32x16 __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(nf_e
     }
     return d;
 }
+// D = A(16x32) * B(32x16) + C, bf16 / float16: lane l (r = l & 15, q = l >> 4) holds k = 8 q + j; C/D as the 16x16x4 form
+template <typename V>
+static inline nf_emu_f32x4 nf_emu_mfma_16x16x32(V a, V b, nf_emu_f32x4 c) {
+    float A[8][64], B[8][64];
+    for (int j = 0; j < 8; ++j) nf_emu_publish_ab((float)a[j], (float)b[j], A[j], B[j]);
+    nf_emu_f32x4 d = c;
+    int l = hip_emu::lane(), col = l & 15, q = l >> 4;
+    for (int r = 0; r < 4; ++r) {
+        float acc = c[r];
+        for (int h = 0; h < 4; ++h)
+            for (int j = 0; j < 8; ++j) acc = fmaf(A[j][4 * q + r + 16 * h], B[j][col + 16 * h], acc);
+        d[r] = acc;
+    }
+    return d;
+}
+static inline nf_emu_f32x4 __builtin_amdgcn_mfma_f32_16x16x32_bf16(nf_emu_bf16x8 a, nf_emu_bf16x8 b, nf_emu_f32x4 c, int, int, int) { return nf_emu_mfma_16x16x32(a, b, c); }
+static inline nf_emu_f32x4 __builtin_amdgcn_mfma_f32_16x16x32_f16(nf_emu_f16x8 a, nf_emu_f16x8 b, nf_emu_f32x4 c, int, int, int) { return nf_emu_mfma_16x16x32(a, b, c); }
+
 // ds_read_b64_tr_b16: each lane reads 8 bytes at its own address; within 16 lanes, lane i gets element i % 4 of lanes 4 j + i / 4, j = 0 .. 3
 static inline uint64_t nf_emu_read_tr16(const char* p) {
     uint64_t raw;
