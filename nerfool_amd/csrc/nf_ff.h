@@ -120,16 +120,17 @@ __device__ __forceinline__ ff_bf16x8 ff_from_e4m3x8(unsigned lo, unsigned hi, un
 enum { FF_F32 = 0, FF_BF16 = 1, FF_F16 = 2 };
 enum { FF_SILU = 0, FF_GELU = 1, FF_RELU = 2 };
 
-// act(g) and act'(g)
+// act(g) and act'(g).  FAST (results that are rounded to 16 bits): the hardware's exponential and reciprocal, good to 2^-21
+template <bool FAST>
 __device__ __forceinline__ void ff_act(int act, float g, float& a, float& slope) {
     if (act == FF_SILU) {
-        const float s = 1.f / (1.f + expf(-g));
+        const float e = 1.f + (FAST ? __expf(-g) : expf(-g)), s = FAST ? nf_rcp(e) : 1.f / e;
         a = g * s;
         slope = s * (1.f + g * (1.f - s));
     } else if (act == FF_GELU) {
-        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f)), q = -0.5f * g * g;
         a = g * cdf;
-        slope = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
+        slope = cdf + g * (0.39894228040143268f * (FAST ? __expf(q) : expf(q)));
     } else {
         a = g > 0.f ? g : (g != g ? g : 0.f);
         slope = g > 0.f ? 1.f : 0.f;

@@ -5,12 +5,15 @@
 //   k innermost    row r at a + r * pitch, k contiguous.  A gated P has two sources: the features' gate rows in a and their up rows in b.
 //   k outermost    row k at a + k * pitch (k < seg) or b + (k - seg) * pitch, the product's n or m contiguous: the gradients' products read the
 //                  tensors as they lie, the transposition happens in the LDS read (ds_read_b64_tr_b16).
-// Tiles go global -> LDS by LDS-DMA, 16 bytes a lane, one k step ahead of their use; nothing passes through registers.  A lane whose 16 bytes lie
+// Tiles go global -> LDS by LDS-DMA, 16 bytes a lane, into a ring of STAGES buffers, STAGES - 1 k steps ahead of their use: a step waits for its own tile
+// only (the counter of outstanding loads), with one barrier.  Nothing passes through registers.  A lane whose 16 bytes lie
 // behind the end of k, n or m reads a page of zeros instead (k, and n or m where they are contiguous, are multiples of 8: the host pads what is not).
 // The 16-byte chunks of a row are placed at (chunk ^ f(row)), so that neither the plain nor the transposed reads collide in the LDS banks; the
 // DMA writes lanes in order, hence the permutation is applied to the address that a lane reads.
 //
 // P is the A operand of v_mfma_f32_32x32x16 (rows in registers), Q the B operand (columns on lanes): a lane ends with one m and 4 consecutive n.
+// The results go through LDS, 32 rows of every wave at a time, so that the output stage reads and writes whole rows: from the fragments directly a
+// wave's 16-byte accesses lie in 32 rows, and the stage of dh's product (g, u in, three tensors out) took twice the time of its 64 k steps.
 #pragma once
 
 #include "nf_ff.h"
@@ -24,23 +27,39 @@ struct FfOperand {
 
 static __device__ ff_u32x4 ff_zero_page = {0u, 0u, 0u, 0u};
 
-// one LDS-DMA: the wave's lane l moves 16 bytes from its own address to dst + 16 l
-__device__ __forceinline__ void ff_dma16(const void* src, char* dst, int lane) {
+// one LDS-DMA: the wave's lane l moves 16 bytes from its own address to lds + at + 16 l (lds: the workgroup's dynamic LDS, at: the same for the wave)
+__device__ __forceinline__ void ff_dma16(const void* src, char* lds, int at, int lane) {
 #if defined(__HIP_DEVICE_COMPILE__)
     unsigned keep;
-    const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)dst;
+    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds + at);
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep)
-                 : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
+                 : "v"(src), "s"(to)
                  : "memory");
 #else
-    __builtin_memcpy(dst + 16 * lane, src, 16);
+    __builtin_memcpy(lds + at + 16 * lane, src, 16);
 #endif
 }
-// all of this wave's LDS-DMAs have landed
-__device__ __forceinline__ void ff_dma_wait() {
+// the compiler moves nothing across this
+__device__ __forceinline__ void ff_keep_order() {
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+__device__ __forceinline__ int ff_wave_index() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#else
+    return threadIdx.x >> 6;
+#endif
+}
+// at most N of this wave's LDS-DMAs are still under way (they land in order), its LDS reads have returned, and so it is for every wave of the workgroup
+template <int N>
+__device__ __forceinline__ void ff_dma_barrier() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+#else
+    __syncthreads();
 #endif
 }
 
@@ -73,7 +92,7 @@ struct FfMfma<ff_half> {
 // where chunk c (16 bytes) of row r of an LDS tile lies; CH chunks a row
 template <int CH>
 __device__ __forceinline__ int ff_swz_inner(int r) {          // rows are n or m, read 32 rows x one chunk at a time
-    return CH == 8 ? (r & 7) : ((r >> 2) & 3);
+    return CH == 8 ? (r >> 1) & 7 : (r >> 2) & 3;          // (16 lanes of a read cover the 64 banks once)
 }
 template <int CH>
 __device__ __forceinline__ int ff_swz_outer(int k) {          // rows are k, read 4 rows x 32 bytes a quarter wave
@@ -110,7 +129,7 @@ struct FfLoader {
                 ptr[i] = o.a + plane * o.plane + (int64_t)(k0 + r) * o.pitch + col;
             } else {
                 const int chunk = slot ^ ff_swz_inner<CH>(r);
-                kc = 8 * chunk;          // (r mod 8, r / 4 mod 4 do not depend on the piece)
+                kc = 8 * (slot ^ ff_swz_inner<CH>(rr));          // (of an even piece; see k_of)
                 const uint16_t* base = o.a;
                 int row;
                 if (GATED) {          // a wave's WSPAN rows: half gate, half up, of the same features
@@ -120,25 +139,27 @@ struct FfLoader {
                 } else
                     row = row0 + r;
                 if (row >= o.rows) row = o.rows - 1;          // a row behind the end: any values, its results are not stored
-                ptr[i] = base + plane * o.plane + (int64_t)row * o.pitch + k0 + kc;
+                ptr[i] = base + plane * o.plane + (int64_t)row * o.pitch + k0 + 8 * chunk;
             }
         }
     }
-    // the tile at k0 (which the pointers stand at) -> buf
-    __device__ __forceinline__ void load(char* buf, int k0, int K, int wave, int lane) {
-        const int rr = lane / CH;
+    // this lane's k in a tile's piece: where a piece is 8 rows, the next piece's rows swap the row's halves
+    __device__ __forceinline__ int k_of(int piece) const { return CH == 8 ? kc ^ ((piece & 1) << 5) : kc; }
+    // piece i of this wave of the tile at k0 (which the pointers stand at) -> lds + at
+    __device__ __forceinline__ void issue(int i, char* lds, int at, int k0, int K, int wave, int lane) {
+        const int li = wave * PER_WAVE + i;
+        const void* src;
+        if (OUTER) {
+            const int k = k0 + (li % PIECES) * RPP + lane / CH;
+            src = k < K && (k < len || k >= seg) && ((valid >> i) & 1u) ? (const void*)(ptr[i] + (k >= seg ? jump : 0)) : (const void*)&ff_zero_page;
+        } else
+            src = k0 + k_of(li % PIECES) < K ? (const void*)ptr[i] : (const void*)&ff_zero_page;
+        ff_dma16(src, lds, at + li * 1024, lane);
+        ptr[i] += step;
+    }
+    __device__ __forceinline__ void load(char* lds, int at, int k0, int K, int wave, int lane) {
 #pragma unroll
-        for (int i = 0; i < PER_WAVE; ++i) {
-            const int li = wave * PER_WAVE + i;
-            const void* src;
-            if (OUTER) {
-                const int k = k0 + (li % PIECES) * RPP + rr;
-                src = k < K && (k < len || k >= seg) && ((valid >> i) & 1u) ? (const void*)(ptr[i] + (k >= seg ? jump : 0)) : (const void*)&ff_zero_page;
-            } else
-                src = k0 + kc < K ? (const void*)ptr[i] : (const void*)&ff_zero_page;
-            ff_dma16(src, buf + li * 1024, lane);
-            ptr[i] += step;
-        }
+        for (int i = 0; i < PER_WAVE; ++i) issue(i, lds, at, k0, K, wave, lane);
     }
 };
 
@@ -168,8 +189,7 @@ struct FfShape {
     int M, N, K;           // N: columns of the result (features for the gated form)
     int n_end;             // columns N .. n_end - 1 are stored as zeros (the padding of an operand of a later product)
     int tiles_m, tiles_n;
-    int k_split;           // k is cut into this many parts of k_part (a multiple of the k step)
-    int k_part;
+    int k_part;            // k is cut into parts of this length (a multiple of the k step)
 };
 
 // Workgroup -> tile.  Consecutive workgroups go to the 8 XCDs in turn: each XCD gets a contiguous run of the tile order, so that its L2 keeps
@@ -183,8 +203,44 @@ __device__ __forceinline__ void ff_tile_of(const FfShape& s, int id, int& tm, in
     tn = in / rows;
 }
 
+// bytes of LDS that ff_output needs
+template <int BP, int BQ, int WP, int WQ>
+constexpr int ff_output_bytes() {
+    return WQ * 32 * (BP + 4) * 4;
+}
+// The accumulators of a tile -> epi, 4 consecutive n of a row at a time: epi.plain(part, m, n, left, inside, v) or epi.gated(part, m, n, left, inside, gate, up), left = s.N - n.
+// Every thread makes every call (epi may exchange values between neighbouring lanes, which hold neighbouring n of the row); inside: the place exists.
+template <int BP, int BQ, int WP, int WQ, bool GATED, int TP, int TQ, typename Epi>
+__device__ __forceinline__ void ff_output(float* lds, const ff_f32x16 (&acc)[TP][TQ], const FfShape& s, int m0, int n0, int part, const Epi& epi) {
+    constexpr int SP = BP / WP, SQ = BQ / WQ, PITCH = BP + 4, COLS = GATED ? BP / 2 : BP, THREADS = WP * WQ * 64, ITEMS = WQ * 32 * COLS / 4;
+    static_assert(ITEMS % THREADS == 0, "every thread makes the same number of calls");
+    const int lane = threadIdx.x & 63, wave = ff_wave_index(), wp = wave % WP, wq = wave / WP;
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        if (j) __syncthreads();
+        float* row = lds + (wq * 32 + (lane & 31)) * PITCH + wp * SP + 4 * (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<ff_f32x4*>(row + 32 * i + 8 * g) = ff_f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        __syncthreads();
+#pragma unroll 2
+        for (int it = threadIdx.x; it < ITEMS; it += THREADS) {
+            const int r = it / (COLS / 4), c = 4 * (it % (COLS / 4));
+            const int m = m0 + (r >> 5) * SQ + 32 * j + (r & 31), n = n0 + c;
+            const bool inside = m < s.M && n < s.n_end;
+            if (GATED) {
+                const float* p = lds + r * PITCH + (c / (SP / 2)) * SP + c % (SP / 2);
+                epi.gated(part, m, n, s.N - n, inside, *reinterpret_cast<const ff_f32x4*>(p), *reinterpret_cast<const ff_f32x4*>(p + SP / 2));
+            } else
+                epi.plain(part, m, n, s.N - n, inside, *reinterpret_cast<const ff_f32x4*>(lds + r * PITCH + c));
+        }
+    }
+}
+
 // tile BP (rows of P) x BQ (rows of Q), WP x WQ waves
-template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, bool PO, bool QO, bool GATED, typename Epi>
+template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, int STAGES, bool PO, bool QO, bool GATED, typename Epi>
 __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand q, FfShape s, Epi epi) {
     typedef typename FfMfma<E>::V V;
     constexpr int WAVES = WP * WQ, SP = BP / WP, SQ = BQ / WQ, TP = SP / 32, TQ = SQ / 32;
@@ -192,7 +248,7 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand 
     typedef FfLoader<NP, BQ, BK, WAVES, QO, false, SQ> LQ;
     constexpr int BUF = LP::BYTES + LQ::BYTES;
     HIP_DYNAMIC_SHARED(char, lds)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = ff_wave_index();
     const int wp = wave % WP, wq = wave / WP;
     const int tiles = s.tiles_m * s.tiles_n, part = blockIdx.x / tiles;
     int tm, tn;
@@ -210,29 +266,35 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand 
         for (int j = 0; j < TQ; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    lp.load(lds, k_lo, k_hi, wave, lane);
-    lq.load(lds + LP::BYTES, k_lo, k_hi, wave, lane);
-    int cur = 0;
+    constexpr int LOADS = LP::PER_WAVE + LQ::PER_WAVE;
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) {
+        lp.load(lds, t * BUF, k_lo + t * BK, k_hi, wave, lane);
+        lq.load(lds, t * BUF + LP::BYTES, k_lo + t * BK, k_hi, wave, lane);
+    }
+    // Fragments are read one k block of 16 ahead of their products, across the step's end too: a barrier therefore says that the NEXT tile has landed.
+    // The reads and the loads are put between the products by hand, one or two behind each: left to itself the compiler gathers the
+    // reads in front of their products to save registers, and the matrix pipe waits for them.
+    V a[2][NP][TP], b[2][NP][TQ];
+    constexpr int KK = BK / 16, READS = NP * (TP + TQ), PRODUCTS = NP * (NP + 1) / 2 * TP * TQ;
+    static_assert(KK % 2 == 0 && STAGES >= 3, "two fragment sets in turn; the next tile lands before the last load starts");
+    auto read = [&](int n, int set, int at, int kk) {
+        const int e = n / (TP + TQ), f = n % (TP + TQ);
+        if (f < TQ) b[set][e][f] = ff_fragment<V, BQ, BK, QO>(lds + at + LP::BYTES + e * (LQ::BYTES / NP), wq * SQ + 32 * f, kk, lane);
+        else a[set][e][f - TQ] = ff_fragment<V, BP, BK, PO>(lds + at + e * (LP::BYTES / NP), wp * SP + 32 * (f - TQ), kk, lane);
+    };
+    ff_dma_barrier<LOADS*(STAGES - 2)>();
+#pragma unroll
+    for (int n = 0; n < READS; ++n) read(n, 0, 0, 0);
+    int cur = 0, next = 1, fill = STAGES - 1;
     for (int k0 = k_lo; k0 < k_hi; k0 += BK) {
-        ff_dma_wait();
-        __syncthreads();          // the tile has landed for every wave, and the other buffer has been read by every wave
-        if (k0 + BK < k_hi) {
-            char* nb = lds + (cur ^ 1) * BUF;
-            lp.load(nb, k0 + BK, k_hi, wave, lane);
-            lq.load(nb + LP::BYTES, k0 + BK, k_hi, wave, lane);
-        }
-        const char* bp = lds + cur * BUF;
-        const char* bq = bp + LP::BYTES;
+        ff_dma_barrier<LOADS*(STAGES - 3)>();          // the next tile has landed for every wave, and the buffer to fill has been read by every wave
+        const int load_at = fill * BUF, load_k = k0 + (STAGES - 1) * BK;
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk) {
-            V a[NP][TP], b[NP][TQ];
-#pragma unroll
-            for (int e = 0; e < NP; ++e) {
-#pragma unroll
-                for (int i = 0; i < TP; ++i) a[e][i] = ff_fragment<V, BP, BK, PO>(bp + e * (LP::BYTES / NP), wp * SP + 32 * i, kk, lane);
-#pragma unroll
-                for (int j = 0; j < TQ; ++j) b[e][j] = ff_fragment<V, BQ, BK, QO>(bq + e * (LQ::BYTES / NP), wq * SQ + 32 * j, kk, lane);
-            }
+        for (int kk = 0; kk < KK; ++kk) {
+            const int set = kk & 1, read_at = kk + 1 < KK ? cur * BUF : next * BUF, read_kk = kk + 1 < KK ? kk + 1 : 0;
+            const int ops = kk == 0 ? READS + LOADS : READS;
+            int m = 0;
             // smallest products first
 #pragma unroll
             for (int o = NP - 1; o >= 0; --o)
@@ -241,41 +303,22 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand 
 #pragma unroll
                     for (int i = 0; i < TP; ++i)
 #pragma unroll
-                        for (int j = 0; j < TQ; ++j) acc[i][j] = FfMfma<E>::mul(a[e][i], b[o - e][j], acc[i][j]);
+                        for (int j = 0; j < TQ; ++j, ++m) {
+                            acc[i][j] = FfMfma<E>::mul(a[set][e][i], b[set][o - e][j], acc[i][j]);
+#pragma unroll
+                            for (int n = m * ops / PRODUCTS; n < (m + 1) * ops / PRODUCTS; ++n) {
+                                // (loads behind the end go on, from the page of zeros: the count of those under way stays right)
+                                if (n < READS) read(n, set ^ 1, read_at, read_kk);
+                                else if (n < READS + LP::PER_WAVE) lp.issue(n - READS, lds, load_at, load_k, k_hi, wave, lane);
+                                else lq.issue(n - READS - LP::PER_WAVE, lds, load_at + LP::BYTES, load_k, k_hi, wave, lane);
+                            }
+                            ff_keep_order();
+                        }
         }
-        cur ^= 1;
+        cur = next;
+        next = next + 1 == STAGES ? 0 : next + 1;
+        fill = fill + 1 == STAGES ? 0 : fill + 1;
     }
-    // lane: m = the lane's column, n = 8 g + 4 (lane / 32) + 0 .. 3 of each 32 x 32 block
-    const int h = lane >> 5;
-#pragma unroll
-    for (int j = 0; j < TQ; ++j) {
-        const int m = m0 + wq * SQ + 32 * j + (lane & 31);
-        if (m >= s.M) continue;
-        if (GATED) {
-#pragma unroll
-            for (int i = 0; i < TP / 2; ++i)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int n = n0 + wp * (SP / 2) + 32 * i + 8 * g + 4 * h;
-                    float v[4], u[4];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        v[c] = acc[i][j][4 * g + c];
-                        u[c] = acc[(i + TP / 2) % TP][j][4 * g + c];
-                    }
-                    if (n < s.n_end) epi.gated(part, m, n, s.N - n, v, u);
-                }
-        } else {
-#pragma unroll
-            for (int i = 0; i < TP; ++i)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int n = n0 + wp * SP + 32 * i + 8 * g + 4 * h;
-                    float v[4];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) v[c] = acc[i][j][4 * g + c];
-                    if (n < s.n_end) epi.plain(part, m, n, s.N - n, v);
-                }
-        }
-    }
+    ff_dma_barrier<0>();          // no load may land in LDS that the workgroup has given back
+    ff_output<BP, BQ, WP, WQ, GATED>(reinterpret_cast<float*>(lds), acc, s, m0, n0, part, epi);
 }

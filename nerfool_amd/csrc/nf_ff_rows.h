@@ -51,6 +51,8 @@ __device__ __forceinline__ typename FfRow<T>::V ff_row_load(const T* row, int k,
 }
 
 constexpr int FF_ROWS_UNIT = 4;          // steps
+// most waves of a workgroup: 64 KB of LDS for their sums, and registers for the two units in flight
+constexpr int ff_rows_most(int nt) { return nt == 1 ? 16 : 8; }
 
 // the waves' sums of fragment f: part[wave][f][lane]
 __device__ __forceinline__ ff_f32x4 ff_rows_total(const ff_f32x4* part, int waves, int frags, int f, int lane) {
@@ -59,8 +61,27 @@ __device__ __forceinline__ ff_f32x4 ff_rows_total(const ff_f32x4* part, int wave
     return s;
 }
 
+// A wave's units along k: wave, wave + waves, ...  Each workgroup begins at another of them: rows whose length is a power of two lie in the same memory
+// channels at the same k, and workgroups that all read the same k at the same time would share a few channels.
+struct FfRounds {
+    int n, first, stride, unit, base;
+    __device__ __forceinline__ FfRounds(int K, int unit_, int waves, int wave, int block) {
+        const int units = (K + unit_ - 1) / unit_;
+        unit = unit_;
+        base = wave * unit_;
+        stride = waves * unit_;
+        n = wave < units ? (units - wave - 1) / waves + 1 : 0;
+        first = n ? block % n : 0;
+    }
+    __device__ __forceinline__ int at(int i) const {
+        int r = first + i;
+        if (r >= n) r -= n;
+        return base + r * stride;
+    }
+};
+
 template <typename T, int NT, bool GATED>
-__global__ void __launch_bounds__(1024) k_ff_rows(const T* __restrict__ w0, const T* __restrict__ w1, const T* __restrict__ x, int M, int N, int K,
+__global__ void __launch_bounds__(64 * ff_rows_most(NT)) k_ff_rows(const T* __restrict__ w0, const T* __restrict__ w1, const T* __restrict__ x, int M, int N, int K,
                                                   T* __restrict__ out, float* __restrict__ g_save, float* __restrict__ u_save, int act) {
     typedef FfRow<T> R;
     typedef typename R::V V;
@@ -110,17 +131,14 @@ __global__ void __launch_bounds__(1024) k_ff_rows(const T* __restrict__ w0, cons
 #pragma unroll
                 for (int t = 0; t < NT; ++t) acc[i][t] = R::mul(a[s][j][i], b[s][j][t], acc[i][t]);
     };
-    const int stride = waves * UNIT;
-    int k0 = wave * UNIT;
-    if (k0 < K) fetch(0, k0);
-    while (k0 < K) {
-        if (k0 + stride < K) fetch(1, k0 + stride);
+    const FfRounds o(K, UNIT, waves, wave, blockIdx.x);
+    if (o.n > 0) fetch(0, o.at(0));
+    for (int i = 0; i < o.n; i += 2) {
+        if (i + 1 < o.n) fetch(1, o.at(i + 1));
         multiply(0);
-        k0 += stride;
-        if (k0 >= K) break;
-        if (k0 + stride < K) fetch(0, k0 + stride);
+        if (i + 1 >= o.n) break;
+        if (i + 2 < o.n) fetch(0, o.at(i + 2));
         multiply(1);
-        k0 += stride;
     }
     constexpr int FRAGS = NW * NT;
 #pragma unroll
@@ -141,7 +159,7 @@ __global__ void __launch_bounds__(1024) k_ff_rows(const T* __restrict__ w0, cons
             float y = v[c];
             if (GATED) {
                 float ac, slope;
-                ff_act(act, v[c], ac, slope);
+                ff_act<sizeof(T) == 2>(act, v[c], ac, slope);
                 y = ac * u[c];
                 if (g_save) {
                     g_save[at] = v[c];
@@ -163,7 +181,7 @@ static inline int ff_rows_waves(int groups, int units, int most) {
 template <typename T, int NT, bool GATED>
 int ff_rows_launch(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, hipStream_t st) {
     const int groups = (N + 15) / 16, unit = FF_ROWS_UNIT * 4 * FfRow<T>::KV;
-    const int waves = ff_rows_waves(groups, (K + unit - 1) / unit, NT >= 4 ? 8 : 16);          // (64 KB of LDS at most)
+    const int waves = ff_rows_waves(groups, (K + unit - 1) / unit, ff_rows_most(NT));
     hipLaunchKernelGGL((k_ff_rows<T, NT, GATED>), dim3(groups), dim3(64 * waves), (size_t)waves * (GATED ? 2 : 1) * NT * 1024, st, (const T*)w0, (const T*)w1,
                        (const T*)x, M, N, K, (T*)out, g_save, u_save, act);
     return 0;

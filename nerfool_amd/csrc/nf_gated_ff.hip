@@ -15,7 +15,7 @@ namespace {
 
 // ---- stores of 4 consecutive values of a row (`left`: how many the row still has); pitch and address allow one store where `wide`
 template <typename T>
-__device__ __forceinline__ void ff_put(T* p, int left, const float* v) {
+__device__ __forceinline__ void ff_put(T* p, int left, const ff_f32x4& v) {
     if (left >= 4) {
         typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
         *reinterpret_cast<V4*>(p) = V4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
@@ -37,7 +37,7 @@ __device__ __forceinline__ void ff_split3(float v, ff_bf16* part) {
     part[1] = (ff_bf16)mid;
     part[2] = (ff_bf16)(rest - mid);
 }
-__device__ __forceinline__ void ff_put3(ff_bf16* p, int64_t plane, int left, const float* v) {
+__device__ __forceinline__ void ff_put3(ff_bf16* p, int64_t plane, int left, const ff_f32x4& v) {
     ff_bf16 t[4][3];
 #pragma unroll
     for (int c = 0; c < 4; ++c) ff_split3(v[c], t[c]);
@@ -56,7 +56,7 @@ template <typename T>
 struct FfMid {
     T* p;
     int64_t pitch;
-    __device__ __forceinline__ void put(int64_t m, int n, int left, const float* v) const {
+    __device__ __forceinline__ void put(int64_t m, int n, int left, const ff_f32x4& v) const {
         T* d = p + m * pitch + n;
         if (left >= 4) {
             typedef T V4 __attribute__((ext_vector_type(4)));
@@ -69,7 +69,7 @@ template <>
 struct FfMid<float> {
     ff_bf16* p;
     int64_t pitch, plane;
-    __device__ __forceinline__ void put(int64_t m, int n, int left, const float* v) const { ff_put3(p + m * pitch + n, plane, left, v); }
+    __device__ __forceinline__ void put(int64_t m, int n, int left, const ff_f32x4& v) const { ff_put3(p + m * pitch + n, plane, left, v); }
 };
 
 template <typename T>
@@ -77,13 +77,22 @@ struct EpiStore {
     T *out, *out2;          // nullable
     int64_t pitch;
     int len, split_m;          // rows m < len go to out, rows m >= split_m to out2, at most len of them
-    __device__ __forceinline__ void plain(int, int m, int n, int left, const float* v) const {
+    __device__ __forceinline__ void plain(int, int m, int n, int left, bool inside, const ff_f32x4& v) const {
         const bool second = m >= split_m;
         const int r = second ? m - split_m : m;
         T* o = second ? out2 : out;
-        if (o && r < len) ff_put(o + r * pitch + n, left, v);
+        if (inside && o && r < len) ff_put(o + r * pitch + n, left, v);
     }
-    __device__ __forceinline__ void gated(int, int, int, int, const float*, const float*) const {}
+    __device__ __forceinline__ void gated(int, int, int, int, bool, const ff_f32x4&, const ff_f32x4&) const {}
+};
+// a part of the sum over k: [part][M][pitch]
+struct EpiPart {
+    float* out;
+    int64_t pitch, stride;
+    __device__ __forceinline__ void plain(int part, int m, int n, int left, bool inside, const ff_f32x4& v) const {
+        if (inside) *reinterpret_cast<ff_f32x4*>(out + part * stride + m * pitch + n) = v;          // (pitch is a multiple of 4)
+    }
+    __device__ __forceinline__ void gated(int, int, int, int, bool, const ff_f32x4&, const ff_f32x4&) const {}
 };
 template <typename T>
 struct EpiGate {
@@ -91,11 +100,13 @@ struct EpiGate {
     float *g_save, *u_save;          // [M, F], nullable
     int64_t F;
     int act;
-    __device__ __forceinline__ void gated(int, int m, int n, int left, const float* g, const float* u) const {
-        float v[4], a, slope;
+    __device__ __forceinline__ void gated(int, int m, int n, int left, bool inside, const ff_f32x4& g, const ff_f32x4& u) const {
+        if (!inside) return;
+        ff_f32x4 v;
+        float a, slope;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            ff_act(act, g[c], a, slope);
+            ff_act<sizeof(T) == 2>(act, g[c], a, slope);
             v[c] = a * u[c];
         }
         h.put(m, n, left, v);
@@ -104,7 +115,7 @@ struct EpiGate {
             ff_put(u_save + m * F + n, left, u);
         }
     }
-    __device__ __forceinline__ void plain(int, int, int, int, const float*) const {}
+    __device__ __forceinline__ void plain(int, int, int, int, bool, const ff_f32x4&) const {}
 };
 template <typename T>
 struct EpiGateBwd {
@@ -112,20 +123,20 @@ struct EpiGateBwd {
     const float *g, *u;
     int64_t F, Fp;
     int act, want_h;
-    __device__ __forceinline__ void plain(int, int m, int n, int left, const float* dh) const {
-        float gv[4], uv[4], dg[4], du[4], hv[4];
+    __device__ __forceinline__ void plain(int, int m, int n, int left, bool inside, const ff_f32x4& dh) const {
+        if (!inside) return;
+        ff_f32x4 gv = {0.f, 0.f, 0.f, 0.f}, uv = gv, dg, du, hv;
         const float *gp = g + m * F + n, *up = u + m * F + n;
         if (left >= 4) {
             typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
-            const F4 a = *reinterpret_cast<const F4*>(gp), b = *reinterpret_cast<const F4*>(up);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) gv[c] = a[c], uv[c] = b[c];
+            gv = *reinterpret_cast<const F4*>(gp);
+            uv = *reinterpret_cast<const F4*>(up);
         } else
-            for (int c = 0; c < 4; ++c) gv[c] = c < left ? gp[c] : 0.f, uv[c] = c < left ? up[c] : 0.f;
+            for (int c = 0; c < left; ++c) gv[c] = gp[c], uv[c] = up[c];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             float a, slope;
-            ff_act(act, gv[c], a, slope);
+            ff_act<sizeof(T) == 2>(act, gv[c], a, slope);
             hv[c] = a * uv[c];
             dg[c] = dh[c] * uv[c] * slope;
             du[c] = dh[c] * a;
@@ -134,8 +145,23 @@ struct EpiGateBwd {
         dgu.put(m, (int)Fp + n, left, du);
         if (want_h) h.put(m, n, left, hv);
     }
-    __device__ __forceinline__ void gated(int, int, int, int, const float*, const float*) const {}
+    __device__ __forceinline__ void gated(int, int, int, int, bool, const ff_f32x4&, const ff_f32x4&) const {}
 };
+
+// the parts of a sum over k, added in their order, -> epi
+template <typename Epi>
+__global__ void __launch_bounds__(256) k_ff_join(EpiPart parts, int n_parts, int64_t M, int N, Epi epi) {
+    const int per_row = (int)(parts.pitch / 4);
+    const int64_t items = M * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / per_row;
+        const int n = (int)(i - m * per_row) * 4;
+        const float* p = parts.out + m * parts.pitch + n;
+        ff_f32x4 v = *reinterpret_cast<const ff_f32x4*>(p);
+        for (int k = 1; k < n_parts; ++k) v += *reinterpret_cast<const ff_f32x4*>(p + k * parts.stride);
+        epi.plain(0, (int)m, n, N - n, n < N, v);
+    }
+}
 
 // rows [R, C] -> rows padded with zeros to `pitch` (a multiple of 8); float -> three planes of bf16 parts
 template <typename T>
@@ -145,7 +171,7 @@ __global__ void __launch_bounds__(256) k_ff_pack(const T* __restrict__ src, int6
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / per_row;
         const int c = (int)(i - r * per_row) * 4, left = cols - c;
-        float v[4];
+        ff_f32x4 v;
         const T* s = src + r * cols + c;
         if (left >= 4) {
             typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -235,12 +261,12 @@ void pack_run(const void* src, int64_t rows, int cols, FfPacked<T>& p, hipStream
     hipLaunchKernelGGL((k_ff_pack<T>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)src, rows, cols, p.mid);
 }
 
-template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, bool PO, bool QO, bool GATED, typename Epi>
-int launch(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
-    constexpr int LDS = 2 * NP * (BP + BQ) * BK * 2, COLS = GATED ? BP / 2 : BP;
+template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, int STAGES, bool PO, bool QO, bool GATED, typename Epi>
+int launch(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, int parts, const Epi& epi, hipStream_t st) {
+    constexpr int RING = STAGES * NP * (BP + BQ) * BK * 2, OUT = ff_output_bytes<BP, BQ, WP, WQ>(), LDS = RING > OUT ? RING : OUT, COLS = GATED ? BP / 2 : BP;
     static bool set[NF_MAX_DEVICES];
     const int dev = nf_current_device();
-    const auto kernel = k_ff_gemm<E, NP, BP, BQ, WP, WQ, BK, PO, QO, GATED, Epi>;
+    const auto kernel = k_ff_gemm<E, NP, BP, BQ, WP, WQ, BK, STAGES, PO, QO, GATED, Epi>;
     if (!set[dev]) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) {
@@ -252,22 +278,72 @@ int launch(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int 
     FfShape s;
     s.M = M, s.N = N, s.K = K, s.n_end = n_end;
     s.tiles_m = (M + BQ - 1) / BQ, s.tiles_n = (N + COLS - 1) / COLS;
-    s.k_split = 1, s.k_part = (K + BK - 1) / BK * BK;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.tiles_m * s.tiles_n)), dim3(WP * WQ * 64), LDS, st, p, q, s, epi);
+    const int steps = (K + BK - 1) / BK;
+    s.k_part = (steps + parts - 1) / parts * BK;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(s.tiles_m * s.tiles_n * parts)), dim3(WP * WQ * 64), LDS, st, p, q, s, epi);
     return 0;
 }
 
-// tile: 256 x 256 where that gives most of the 256 CUs a tile, else 128 x 128 (float32 parts: 128 x 128, whose three planes fill the LDS)
+// ---- which tile, and in how many parts k is cut.  The time of a product, in microseconds, as measured on its pieces: a 256 x 256 tile takes 0.95 a k step of 32 and
+//      has a CU for itself; two 128 x 128 tiles share one and take 0.7 a step together; of a float32 operand's three planes a 128 x 128 tile takes 1.4 a step.  A tile
+//      costs about 8 steps beside its k loop (first loads, output stage).  Parts cost their writing and reading, and a launch.
+struct FfChoice {
+    bool big;
+    int parts;
+};
+FfChoice ff_choose(bool three, int64_t M, int64_t N, int64_t K, bool may_split) {
+    FfChoice best = {false, 1};
+    double least = 1e30;
+    for (int big = three ? 0 : 1; big >= 0; --big) {
+        const int64_t b = big ? 256 : 128, tiles = ((M + b - 1) / b) * ((N + b - 1) / b), steps = (K + 31) / 32, slots = big || three ? 256 : 512;
+        const double step = three ? 1.4 : big ? 0.95 : 0.7;
+        for (int parts = 1; parts <= 8; ++parts) {
+            if (parts > 1 && (!may_split || steps < 8 * parts)) break;
+            const int64_t per = (steps + parts - 1) / parts, n = tiles * parts;
+            if (per * (parts - 1) >= steps) continue;          // the last part would be empty
+            // (a last round that fills less than half of a 128 x 128 tile's slots has the CUs' whole rate for one tile each)
+            const int64_t rounds = n / slots, rest = n % slots;
+            double t = rounds * (per + 8) * step + (rest ? (per + 8) * step * (!big && !three && rest <= 256 ? 0.6 : 1.0) : 0.0);
+            if (parts > 1) t += 4.0 + (double)M * N * 4 * (parts + 1) / 4.5e6;
+            if (t < least) least = t, best = {big != 0, parts};
+        }
+    }
+    return best;
+}
+int64_t pad4(int64_t n) { return (n + 3) / 4 * 4; }
+// bytes of the parts of a product that may be split
+int64_t ff_part_bytes(bool three, int64_t M, int64_t N, int64_t K) {
+    const FfChoice c = ff_choose(three, M, N, K, true);
+    return c.parts > 1 ? c.parts * M * pad4(N) * 4 : 0;
+}
+
 template <typename T, bool PO, bool QO, bool GATED, typename Epi>
-int product(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
+int product_as(const FfChoice& c, const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
     typedef typename FfElem<T>::E E;
     if constexpr (FfElem<T>::NP == 3) {
-        return launch<E, 3, 128, 128, 2, 4, 32, PO, QO, GATED>(p, q, M, N, n_end, K, epi, st);
+        return launch<E, 3, 128, 128, 2, 4, 32, 3, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
     } else {
-        const int64_t big = (int64_t)((M + 255) / 256) * ((N * (GATED ? 2 : 1) + 255) / 256);
-        if (big >= 160) return launch<E, 1, 256, 256, 2, 4, 64, PO, QO, GATED>(p, q, M, N, n_end, K, epi, st);
-        return launch<E, 1, 128, 128, 2, 2, 64, PO, QO, GATED>(p, q, M, N, n_end, K, epi, st);
+        if (c.big) return launch<E, 1, 256, 256, 2, 4, 32, 4, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
+        return launch<E, 1, 128, 128, 2, 2, 32, 4, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
     }
+}
+// the whole sum over k in one tile
+template <typename T, bool PO, bool QO, bool GATED, typename Epi>
+int product(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
+    return product_as<T, PO, QO, GATED>(ff_choose(FfElem<T>::NP == 3, M, GATED ? 2 * (int64_t)N : N, K, false), p, q, M, N, n_end, K, epi, st);
+}
+// ... or in parts: `parts` has room for ff_part_bytes
+template <typename T, bool PO, bool QO>
+int product_split(const FfOperand& p, const FfOperand& q, int M, int N, int K, const EpiStore<T>& epi, float* parts, hipStream_t st) {
+    const FfChoice c = ff_choose(FfElem<T>::NP == 3, M, N, K, true);
+    if (c.parts == 1) return product_as<T, PO, QO, false>(c, p, q, M, N, N, K, epi, st);
+    const EpiPart part = {parts, pad4(N), M * pad4(N)};
+    const int rc = product_as<T, PO, QO, false>(c, p, q, M, N, N, K, part, st);
+    if (rc) return rc;
+    int64_t blocks = (M * (part.pitch / 4) + 255) / 256;
+    if (blocks > 256 * 16) blocks = 256 * 16;
+    hipLaunchKernelGGL((k_ff_join<EpiStore<T>>), dim3((unsigned)blocks), dim3(256), 0, st, part, c.parts, (int64_t)M, N, epi);
+    return 0;
 }
 
 #define FF_TRY(call)            \
@@ -280,6 +356,7 @@ template <typename T>
 struct FwdPlan {
     FfPacked<T> x, wg, wu, wd;
     FfMid<T> h;
+    float* parts;
     int64_t bytes;
     FwdPlan(char* base, int64_t M, int D, int F) {
         Carve ws{base};
@@ -288,6 +365,7 @@ struct FwdPlan {
         wu = pack_at<T>(ws, F, D);
         wd = pack_at<T>(ws, D, F);
         h = mid_at<T>(ws, M, pad8(F));
+        parts = (float*)ws.take(ff_part_bytes(FfElem<T>::NP == 3, M, D, pad8(F)));
         bytes = ws.used;
     }
 };
@@ -299,6 +377,7 @@ template <typename T, bool GATED>
 int few_rows(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, hipStream_t st) {
     if (M <= 16) return ff_rows_launch<T, 1, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
     if (M <= 32) return ff_rows_launch<T, 2, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+    if (M <= 48) return ff_rows_launch<T, 3, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
     return ff_rows_launch<T, 4, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
 }
 
@@ -319,7 +398,7 @@ int ff_fwd(const void* x, const void* wg, const void* wu, const void* wd, int M,
     const EpiGate<T> gate = {f.h, g_save, u_save, F, act};
     FF_TRY((product<T, false, false, true>(p, as_operand(f.x.mid, M), M, F, (int)f.h.pitch, (int)f.x.mid.pitch, gate, st)));
     const EpiStore<T> store = {(T*)out, nullptr, D, M, 0x7fffffff};
-    FF_TRY((product<T, false, false, false>(as_operand(f.wd.mid, D), as_operand(f.h, M), M, D, D, (int)f.h.pitch, store, st)));
+    FF_TRY((product_split<T, false, false>(as_operand(f.wd.mid, D), as_operand(f.h, M), M, D, (int)f.h.pitch, store, f.parts, st)));
     return 0;
 }
 
@@ -327,6 +406,7 @@ template <typename T>
 struct BwdPlan {
     FfPacked<T> x, wg, wu, wd, dy;
     FfMid<T> dgu, h;
+    float* parts;          // of one product at a time
     int64_t bytes;
     BwdPlan(char* base, int64_t M, int D, int F, bool dx, bool dwgu, bool dwd) {
         Carve ws{base};
@@ -336,6 +416,18 @@ struct BwdPlan {
         if (dx) wg = pack_at<T>(ws, F, D), wu = pack_at<T>(ws, F, D);
         dgu = mid_at<T>(ws, M, 2 * pad8(F));
         if (dwd) h = mid_at<T>(ws, M, pad8(F));
+        const bool three = FfElem<T>::NP == 3;
+        int64_t most = 0;
+        if (dx) most = ff_part_bytes(three, M, D, pad8(F) + F);
+        if (dwgu) {
+            const int64_t n = ff_part_bytes(three, 2 * pad8(F), D, M);
+            most = n > most ? n : most;
+        }
+        if (dwd) {
+            const int64_t n = ff_part_bytes(three, D, F, M);
+            most = n > most ? n : most;
+        }
+        parts = (float*)ws.take(most);
         bytes = ws.used;
     }
 };
@@ -359,16 +451,16 @@ int ff_bwd(const void* x, const void* wg, const void* wu, const void* wd, const 
         p.b = (const uint16_t*)f.wu.mid.p;
         p.len = F, p.seg = Fp;
         const EpiStore<T> store = {(T*)dx, nullptr, D, M, 0x7fffffff};
-        FF_TRY((product<T, true, false, false>(p, as_operand(f.dgu, M), M, D, D, Fp + F, store, st)));
+        FF_TRY((product_split<T, true, false>(p, as_operand(f.dgu, M), M, D, Fp + F, store, f.parts, st)));
     }
     if (dwgu) {          // [dWg; dWu][f][d] = sum over m of dgu[m][f] x[m][d]
         pack_run<T>(x, M, D, f.x, st);
         const EpiStore<T> store = {(T*)dwg, (T*)dwu, D, F, Fp};
-        FF_TRY((product<T, true, true, false>(as_operand(f.x.mid, (int)f.x.mid.pitch), as_operand(f.dgu, 2 * Fp), 2 * Fp, D, D, M, store, st)));
+        FF_TRY((product_split<T, true, true>(as_operand(f.x.mid, (int)f.x.mid.pitch), as_operand(f.dgu, 2 * Fp), 2 * Fp, D, M, store, f.parts, st)));
     }
     if (dwd) {          // dWd[d][f] = sum over m of dy[m][d] h[m][f]
         const EpiStore<T> store = {(T*)dwd, nullptr, F, D, 0x7fffffff};
-        FF_TRY((product<T, true, true, false>(as_operand(f.h, Fp), as_operand(f.dy.mid, (int)f.dy.mid.pitch), D, F, F, M, store, st)));
+        FF_TRY((product_split<T, true, true>(as_operand(f.h, Fp), as_operand(f.dy.mid, (int)f.dy.mid.pitch), D, F, M, store, f.parts, st)));
     }
     return 0;
 }

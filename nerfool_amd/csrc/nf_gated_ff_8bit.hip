@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
     typedef FfLoader<1, BQ, BK, WAVES, false, false, SQ> LQ;
     constexpr int BUF = LP::BYTES + LQ::BYTES;
     HIP_DYNAMIC_SHARED(char, lds)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = ff_wave_index(), r32 = lane & 31, half = lane >> 5;
     const int wp = wave % WP, wq = wave / WP;
     int tm, tn;
     ff_tile_of(s, blockIdx.x, tm, tn);
@@ -81,12 +81,11 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
     for (int i = 0; i < TP; ++i) pn[i] = ff_scale_word(prow[i], 0, blocks);
 #pragma unroll
     for (int j = 0; j < TQ; ++j) qn[j] = ff_scale_word(qrow[j], 0, blocks);
-    lp.load(lds, 0, K, wave, lane);
-    lq.load(lds + LP::BYTES, 0, K, wave, lane);
+    lp.load(lds, 0, 0, K, wave, lane);
+    lq.load(lds, LP::BYTES, 0, K, wave, lane);
     int cur = 0;
     for (int k0 = 0; k0 < K; k0 += BK) {
-        ff_dma_wait();
-        __syncthreads();
+        ff_dma_barrier<0>();
         unsigned pc[TP], qc[TQ];          // the lane's scales of this step: byte 0 for its first 64 values, byte 2 for the others
 #pragma unroll
         for (int i = 0; i < TP; ++i) pc[i] = EXACT ? pn[i] : pn[i] >> (8 * half);
@@ -98,9 +97,8 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
             for (int i = 0; i < TP; ++i) pn[i] = ff_scale_word(prow[i], blk, blocks);
 #pragma unroll
             for (int j = 0; j < TQ; ++j) qn[j] = ff_scale_word(qrow[j], blk, blocks);
-            char* nb = lds + (cur ^ 1) * BUF;
-            lp.load(nb, k0 + BK, K, wave, lane);
-            lq.load(nb + LP::BYTES, k0 + BK, K, wave, lane);
+            lp.load(lds, (cur ^ 1) * BUF, k0 + BK, K, wave, lane);
+            lq.load(lds, (cur ^ 1) * BUF + LP::BYTES, k0 + BK, K, wave, lane);
         }
         const char* bp = lds + cur * BUF;
         const char* bq = bp + LP::BYTES;
@@ -148,23 +146,15 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
         }
         cur ^= 1;
     }
-#pragma unroll
-    for (int j = 0; j < TQ; ++j) {
-        const int m = m0 + wq * SQ + 32 * j + r32;
-        if (GATED) {
-#pragma unroll
-            for (int i = 0; i < TP / 2; ++i) epi.gated(m, n0 + wp * (SP / 2) + 32 * i, half, s, acc[i][j], acc[(i + TP / 2) % TP][j]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < TP; ++i) epi.plain(m, n0 + wp * SP + 32 * i, half, s, acc[i][j]);
-        }
-    }
+    ff_dma_barrier<0>();
+    ff_output<BP, BQ, WP, WQ, GATED>(reinterpret_cast<float*>(lds), acc, s, m0, n0, 0, epi);
 }
 
 // few rows (nf_ff_rows.h): 32 weight rows a workgroup, so that the features of an h block are one workgroup's; 128 values of k a unit, whose scales are a
 // word a row; 16 values a lane and step, as two bfloat16 operands
+constexpr int ff_rows8_most(int nt, bool gated) { return gated ? (nt >= 3 ? 4 : 8) : (nt >= 3 ? 8 : 16); }          // 64 KB of LDS at most
 template <int NT, bool GATED, typename T>
-__global__ void __launch_bounds__(1024) k_ff_rows8(const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1, FfScales sw, const uint8_t* __restrict__ x,
+__global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1, FfScales sw, const uint8_t* __restrict__ x,
                                                    const uint8_t* __restrict__ xs, int M, int N, int K, T* __restrict__ out, uint8_t* __restrict__ hq,
                                                    uint8_t* __restrict__ hs, int act) {
     constexpr int NW = GATED ? 2 : 1, U = 2, UNIT = 128;
@@ -237,17 +227,14 @@ __global__ void __launch_bounds__(1024) k_ff_rows8(const uint8_t* __restrict__ w
             }
         }
     };
-    const int stride = waves * UNIT;
-    int k0 = wave * UNIT;
-    if (k0 < K) fetch(0, k0);
-    while (k0 < K) {
-        if (k0 + stride < K) fetch(1, k0 + stride);
+    const FfRounds o(K, UNIT, waves, wave, blockIdx.x);
+    if (o.n > 0) fetch(0, o.at(0));
+    for (int i = 0; i < o.n; i += 2) {
+        if (i + 1 < o.n) fetch(1, o.at(i + 1));
         multiply(0);
-        k0 += stride;
-        if (k0 >= K) break;
-        if (k0 + stride < K) fetch(0, k0 + stride);
+        if (i + 1 >= o.n) break;
+        if (i + 2 < o.n) fetch(0, o.at(i + 2));
         multiply(1);
-        k0 += stride;
     }
     constexpr int FRAGS = NW * 2 * NT;
 #pragma unroll
@@ -271,7 +258,7 @@ __global__ void __launch_bounds__(1024) k_ff_rows8(const uint8_t* __restrict__ w
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float ac, slope;
-                    ff_act(act, v[h][c], ac, slope);
+                    ff_act<false>(act, v[h][c], ac, slope);
                     v[h][c] = ac * u[c];
                     top = fmaxf(top, fabsf(v[h][c]));
                     bad |= !(fabsf(v[h][c]) <= 3.4028235e38f);
@@ -301,7 +288,7 @@ __global__ void __launch_bounds__(1024) k_ff_rows8(const uint8_t* __restrict__ w
 template <int NT, bool GATED, typename T>
 void rows8(const void* w0, const void* w1, const FfScales& sw, const void* x, const uint8_t* xs, int M, int N, int K, T* out, uint8_t* hq, uint8_t* hs, int act,
            hipStream_t st) {
-    const int waves = ff_rows_waves(N / 32, (K + 127) / 128, GATED && NT >= 2 ? (NT >= 4 ? 4 : 8) : 16);          // (64 KB of LDS at most)
+    const int waves = ff_rows_waves(N / 32, (K + 127) / 128, ff_rows8_most(NT, GATED));
     hipLaunchKernelGGL((k_ff_rows8<NT, GATED, T>), dim3(N / 32), dim3(64 * waves), (size_t)waves * (GATED ? 4 : 2) * NT * 1024, st, (const uint8_t*)w0,
                        (const uint8_t*)w1, sw, (const uint8_t*)x, xs, M, N, K, out, hq, hs, act);
 }
@@ -310,6 +297,7 @@ void few_rows8(const void* w0, const void* w1, const FfScales& sw, const void* x
                hipStream_t st) {
     if (M <= 16) rows8<1, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
     else if (M <= 32) rows8<2, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
+    else if (M <= 48) rows8<3, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
     else rows8<4, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
 }
 
@@ -317,50 +305,43 @@ template <typename T>
 struct Epi8Store {
     T* out;
     int64_t pitch;
-    __device__ __forceinline__ void plain(int m, int n0, int half, const FfShape& s, const ff_f32x16& v) const {
-        if (m >= s.M) return;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int n = n0 + 8 * g + 4 * half;          // N is a multiple of 32
-            typedef T V4 __attribute__((ext_vector_type(4)));
-            if (n < s.N) *reinterpret_cast<V4*>(out + m * pitch + n) = V4{(T)v[4 * g], (T)v[4 * g + 1], (T)v[4 * g + 2], (T)v[4 * g + 3]};
-        }
+    __device__ __forceinline__ void plain(int, int m, int n, int, bool inside, const ff_f32x4& v) const {          // N is a multiple of 32
+        typedef T V4 __attribute__((ext_vector_type(4)));
+        if (inside) *reinterpret_cast<V4*>(out + m * pitch + n) = V4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
     }
-    __device__ __forceinline__ void gated(int, int, int, const FfShape&, const ff_f32x16&, const ff_f32x16&) const {}
+    __device__ __forceinline__ void gated(int, int, int, int, bool, const ff_f32x4&, const ff_f32x4&) const {}
 };
 
 struct Epi8Gate {
     uint8_t *q, *scale;
     int64_t F;
     int act;
-    __device__ __forceinline__ void gated(int m, int n0, int half, const FfShape& s, const ff_f32x16& g, const ff_f32x16& u) const {
-        float v[16], top = 0.f;
+    // 8 neighbouring lanes hold the 32 features of a block
+    __device__ __forceinline__ void gated(int, int m, int n, int, bool inside, const ff_f32x4& g, const ff_f32x4& u) const {
+        float v[4], top = 0.f;
         bool bad = false;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
+        for (int c = 0; c < 4; ++c) {
             float a, slope;
-            ff_act(act, g[r], a, slope);
-            v[r] = a * u[r];
-            top = fmaxf(top, fabsf(v[r]));
-            bad |= !(fabsf(v[r]) <= 3.4028235e38f);
+            ff_act<false>(act, g[c], a, slope);
+            v[c] = a * u[c];
+            top = fmaxf(top, fabsf(v[c]));
+            bad |= !(fabsf(v[c]) <= 3.4028235e38f);
         }
-        if (bad) top = INFINITY;
-        top = nf_half_max(top);
-        if (m >= s.M || n0 >= s.N) return;
+        if (bad) top = INFINITY;          // (fmaxf drops a NaN)
+        top = nf_grp_reduce<8>(top, NfMax());
+        if (!inside) return;
         const unsigned byte = ff_scale_byte(top);
         const float inv = byte == 255u ? NAN : ff_scale_inverse(byte);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<unsigned*>(q + m * F + n0 + 8 * c + 4 * half) =
-                ff_e4m3x4(v[4 * c] * inv, v[4 * c + 1] * inv, v[4 * c + 2] * inv, v[4 * c + 3] * inv);
-        if (half == 0) scale[m * (F / 32) + n0 / 32] = (uint8_t)byte;
+        *reinterpret_cast<unsigned*>(q + m * F + n) = ff_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+        if (n % 32 == 0) scale[m * (F / 32) + n / 32] = (uint8_t)byte;
     }
-    __device__ __forceinline__ void plain(int, int, int, const FfShape&, const ff_f32x16&) const {}
+    __device__ __forceinline__ void plain(int, int, int, int, bool, const ff_f32x4&) const {}
 };
 
 template <int BP, int BQ, int WP, int WQ, bool GATED, bool EXACT, typename Epi>
 int launch8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const FfScales& sq, int M, int N, int K, const Epi& epi, hipStream_t st) {
-    constexpr int LDS = 2 * (BP + BQ) * 128, COLS = GATED ? BP / 2 : BP;
+    constexpr int RING = 2 * (BP + BQ) * 128, OUT = ff_output_bytes<BP, BQ, WP, WQ>(), LDS = RING > OUT ? RING : OUT, COLS = GATED ? BP / 2 : BP;
     static bool set[NF_MAX_DEVICES];
     const int dev = nf_current_device();
     const auto kernel = k_ff_gemm8<BP, BQ, WP, WQ, GATED, EXACT, Epi>;
@@ -375,7 +356,7 @@ int launch8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const Ff
     FfShape s;
     s.M = M, s.N = N, s.K = K / 2, s.n_end = N;
     s.tiles_m = (M + BQ - 1) / BQ, s.tiles_n = (N + COLS - 1) / COLS;
-    s.k_split = 1, s.k_part = K / 2;
+    s.k_part = K / 2;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(s.tiles_m * s.tiles_n)), dim3(WP * WQ * 64), LDS, st, p, q, sp, sq, s, epi);
     return 0;
 }

@@ -364,8 +364,6 @@ int64_t rms_grid(int64_t rows, int rows_per_block, int64_t most) {
         else if (nv_ <= 32) { GO(32, 1); }          \
         else if (nv_ <= 64) { GO(64, 1); }          \
         else if (many_ && nv_ <= 128) { GO(64, 2); }\
-        else if (many_ && nv_ <= 256) { GO(64, 4); }\
-        else if (many_ && nv_ <= 512) { GO(64, 8); }\
         else if (nv_ <= 256) { GO(256, 1); }        \
         else if (nv_ <= 512) { GO(256, 2); }        \
         else if (nv_ <= 1024) { GO(256, 4); }       \
