@@ -456,7 +456,7 @@ int64_t nf_gated_ff_bwd_workspace_bytes(int64_t rows, int dim, int hidden, int d
 int nf_gated_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* dy, const float* g, const float* u,
                     int64_t rows, int dim, int hidden, int dtype, int activation, void* dx, void* dw_gate, void* dw_up, void* dw_down,
                     void* workspace, nf_stream_t stream);
-int64_t nf_gated_ff_fwd_8bit_workspace_bytes(int64_t rows, int hidden);
+int64_t nf_gated_ff_fwd_8bit_workspace_bytes(int64_t rows, int dim, int hidden);
 int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const void* w_gate, const uint8_t* gate_scale, const void* w_up,
                          const uint8_t* up_scale, const void* w_down, const uint8_t* down_scale, int64_t rows, int dim, int hidden, int out_dtype,
                          int activation, void* out, void* workspace, nf_stream_t stream);

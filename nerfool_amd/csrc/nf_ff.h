@@ -128,9 +128,17 @@ __device__ __forceinline__ void ff_act(int act, float g, float& a, float& slope)
         a = g * s;
         slope = s * (1.f + g * (1.f - s));
     } else if (act == FF_GELU) {
-        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f)), q = -0.5f * g * g;
+        const float e = FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g);
+        float cdf;
+        if (FAST) {          // Abramowitz and Stegun 7.1.26 for erf(|g| / sqrt 2): off by at most 1.5e-7
+            const float x = fabsf(g) * 0.70710678118654752f, t = nf_rcp(1.f + 0.3275911f * x);
+            const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+            const float tail = 0.5f * p * e;          // half of erfc(x)
+            cdf = g < 0.f ? tail : 1.f - tail;
+        } else
+            cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
         a = g * cdf;
-        slope = cdf + g * (0.39894228040143268f * (FAST ? __expf(q) : expf(q)));
+        slope = cdf + g * (0.39894228040143268f * e);
     } else {
         a = g > 0.f ? g : (g != g ? g : 0.f);
         slope = g > 0.f ? 1.f : 0.f;

@@ -40,6 +40,19 @@ __device__ __forceinline__ void ff_dma16(const void* src, char* lds, int at, int
     __builtin_memcpy(lds + at + 16 * lane, src, 16);
 #endif
 }
+// ... 4 bytes a lane
+__device__ __forceinline__ void ff_dma4(const void* src, char* lds, int at, int lane) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    unsigned keep;
+    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds + at);
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(src), "s"(to)
+                 : "memory");
+#else
+    __builtin_memcpy(lds + at + 4 * lane, src, 4);
+#endif
+}
 // the compiler moves nothing across this
 __device__ __forceinline__ void ff_keep_order() {
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -36,39 +36,50 @@ __device__ __forceinline__ unsigned ff_scale_word(const uint8_t* row, int blk, i
     return w;
 }
 
+static __device__ unsigned ff_unit_scales = 0x7f7f7f7fu;          // four scales of 1
+
+// Steps go in pairs: 64 values of k a step, 128 a pair, whose four scales of a row are one word; the words come with a 4-byte LDS-DMA a wave and pair, two
+// pairs ahead, into a ring of their own (rows of words need a pitch of 4 bytes: the host pads other lengths with scales of 1).  A step past the
+// end multiplies zeros by scales of 1.
 // EXACT: the products in bfloat16
 template <int BP, int BQ, int WP, int WQ, bool GATED, bool EXACT, typename Epi>
 __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand q, FfScales sp, FfScales sq, FfShape s, Epi epi) {
-    constexpr int BK = 64;          // in pairs of values
+    constexpr int BK = 32, STAGES = 4;          // BK in pairs of values
     constexpr int WAVES = WP * WQ, SP = BP / WP, SQ = BQ / WQ, TP = SP / 32, TQ = SQ / 32;
     typedef FfLoader<1, BP, BK, WAVES, false, GATED, SP> LP;
     typedef FfLoader<1, BQ, BK, WAVES, false, false, SQ> LQ;
-    constexpr int BUF = LP::BYTES + LQ::BYTES;
+    constexpr int BUF = LP::BYTES + LQ::BYTES, LOADS = LP::PER_WAVE + LQ::PER_WAVE, SCALES = STAGES * BUF, WORDS = (BP + BQ) * 4;
+    static_assert(BP + BQ == WAVES * 64, "a wave moves the words of 64 rows");
     HIP_DYNAMIC_SHARED(char, lds)
     const int lane = threadIdx.x & 63, wave = ff_wave_index(), r32 = lane & 31, half = lane >> 5;
     const int wp = wave % WP, wq = wave / WP;
     int tm, tn;
     ff_tile_of(s, blockIdx.x, tm, tn);
     const int m0 = tm * BQ, n0 = tn * (GATED ? BP / 2 : BP);
-    const int K = s.K;          // pairs
-    const int blocks = K / 16;
+    const int K = s.K;          // pairs of values
+    const int words = (K + 63) / 64;
     LP lp;
     LQ lq;
     lp.init(p, n0, 0, wave, lane);
     lq.init(q, m0, 0, wave, lane);
-    const uint8_t *prow[TP], *qrow[TQ];
-#pragma unroll
-    for (int i = 0; i < TP; ++i) {
-        int row = GATED ? n0 + wp * (SP / 2) + 32 * (i % (TP > 1 ? TP / 2 : 1)) + r32 : n0 + wp * SP + 32 * i + r32;
-        if (row >= sp.rows) row = sp.rows - 1;
-        prow[i] = (GATED && i >= TP / 2 ? sp.b : sp.a) + row * sp.pitch;
+    const uint8_t* srow;          // the row whose words this lane moves
+    {
+        const int v = wave * 64 + lane;
+        if (v < BP) {
+            const int in = v % SP;
+            int row = GATED ? n0 + (v / SP) * (SP / 2) + in % (SP / 2) : n0 + v;
+            if (row >= sp.rows) row = sp.rows - 1;
+            srow = (GATED && in >= SP / 2 ? sp.b : sp.a) + row * sp.pitch;
+        } else {
+            int row = m0 + v - BP;
+            if (row >= sq.rows) row = sq.rows - 1;
+            srow = sq.a + row * sq.pitch;
+        }
     }
-#pragma unroll
-    for (int j = 0; j < TQ; ++j) {
-        int row = m0 + wq * SQ + 32 * j + r32;
-        if (row >= sq.rows) row = sq.rows - 1;
-        qrow[j] = sq.a + row * sq.pitch;
-    }
+    auto load_scales = [&](int pair) {
+        const void* src = pair < words ? (const void*)(srow + 4 * pair) : (const void*)&ff_unit_scales;
+        ff_dma4(src, lds, SCALES + (pair & 3) * WORDS + wave * 256, lane);
+    };
     ff_f32x16 acc[TP][TQ];
 #pragma unroll
     for (int i = 0; i < TP; ++i)
@@ -76,83 +87,107 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
         for (int j = 0; j < TQ; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    unsigned pn[TP], qn[TQ];
+    load_scales(0);
+    load_scales(1);
 #pragma unroll
-    for (int i = 0; i < TP; ++i) pn[i] = ff_scale_word(prow[i], 0, blocks);
+    for (int t = 0; t < STAGES - 1; ++t) {
+        lp.load(lds, t * BUF, t * BK, K, wave, lane);
+        lq.load(lds, t * BUF + LP::BYTES, t * BK, K, wave, lane);
+    }
+    ff_u32x4 a[2][TP][2], b[2][TQ][2];
+    unsigned pw[2][TP], qw[2][TQ];          // words of the pair at hand and of the next
+    constexpr int READS = 2 * (TP + TQ);
+    auto read = [&](int n, int set, int at) {          // half n % 2 of a fragment: k 16 (lane / 32) .. + 15 of its 32
+        const int f = n / 2, c = n % 2;
+        const int row32 = f < TQ ? wq * SQ + 32 * f : wp * SP + 32 * (f - TQ), r = row32 + r32;
+        const char* tile = lds + at + (f < TQ ? LP::BYTES : 0);
+        const ff_u32x4 v = *reinterpret_cast<const ff_u32x4*>(tile + r * (BK * 2) + (((2 * c + half) ^ ff_swz_inner<4>(r)) << 4));
+        if (f < TQ) b[set][f][c] = v;
+        else a[set][f - TQ][c] = v;
+    };
+    auto read_words = [&](int set, int pair) {
+        const char* w = lds + SCALES + (pair & 3) * WORDS;
 #pragma unroll
-    for (int j = 0; j < TQ; ++j) qn[j] = ff_scale_word(qrow[j], 0, blocks);
-    lp.load(lds, 0, 0, K, wave, lane);
-    lq.load(lds, LP::BYTES, 0, K, wave, lane);
-    int cur = 0;
-    for (int k0 = 0; k0 < K; k0 += BK) {
-        ff_dma_barrier<0>();
-        unsigned pc[TP], qc[TQ];          // the lane's scales of this step: byte 0 for its first 64 values, byte 2 for the others
+        for (int i = 0; i < TP; ++i) pw[set][i] = *reinterpret_cast<const unsigned*>(w + 4 * (wp * SP + 32 * i + r32));
 #pragma unroll
-        for (int i = 0; i < TP; ++i) pc[i] = EXACT ? pn[i] : pn[i] >> (8 * half);
+        for (int j = 0; j < TQ; ++j) qw[set][j] = *reinterpret_cast<const unsigned*>(w + 4 * (BP + wq * SQ + 32 * j + r32));
+        if (!EXACT) {          // the instruction takes byte 0 (first step) or 2 (second) of the lane's word: its own half's block
 #pragma unroll
-        for (int j = 0; j < TQ; ++j) qc[j] = EXACT ? qn[j] : qn[j] >> (8 * half);
-        if (k0 + BK < K) {
-            const int blk = (k0 + BK) / 16;
+            for (int i = 0; i < TP; ++i) pw[set][i] >>= 8 * half;
 #pragma unroll
-            for (int i = 0; i < TP; ++i) pn[i] = ff_scale_word(prow[i], blk, blocks);
-#pragma unroll
-            for (int j = 0; j < TQ; ++j) qn[j] = ff_scale_word(qrow[j], blk, blocks);
-            lp.load(lds, (cur ^ 1) * BUF, k0 + BK, K, wave, lane);
-            lq.load(lds, (cur ^ 1) * BUF + LP::BYTES, k0 + BK, K, wave, lane);
+            for (int j = 0; j < TQ; ++j) qw[set][j] >>= 8 * half;
         }
-        const char* bp = lds + cur * BUF;
-        const char* bq = bp + LP::BYTES;
+    };
+    ff_dma_barrier<LOADS*(STAGES - 2)>();
+#pragma unroll
+    for (int n = 0; n < READS; ++n) read(n, 0, 0);
+    read_words(0, 0);
+    int cur = 0, next = 1, fill = STAGES - 1;
+    auto multiply = [&](int set, int i, int j) {          // (set: also the step of the pair)
         if constexpr (EXACT) {
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {
-                ff_bf16x8 a[TP], b[TQ];
-                auto fragment = [&](const char* tile, int row32, unsigned scales) {
-                    const int r = row32 + r32;
-                    const ff_u32x2 v = *reinterpret_cast<const ff_u32x2*>(tile + r * (BK * 2) + ((kk ^ ff_swz_inner<8>(r)) << 4) + 8 * half);
-                    return ff_from_e4m3x8(v.x, v.y, (scales >> (8 * (kk / 2))) & 255u);
-                };
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int i = 0; i < TP; ++i) a[i] = fragment(bp, wp * SP + 32 * i, pc[i]);
-#pragma unroll
-                for (int j = 0; j < TQ; ++j) b[j] = fragment(bq, wq * SQ + 32 * j, qc[j]);
-#pragma unroll
-                for (int i = 0; i < TP; ++i)
-#pragma unroll
-                    for (int j = 0; j < TQ; ++j) acc[i][j] = FfMfma<ff_bf16>::mul(a[i], b[j], acc[i][j]);
-            }
+                for (int h = 0; h < 2; ++h)
+                    acc[i][j] = FfMfma<ff_bf16>::mul(ff_from_e4m3x8(a[set][i][c][2 * h], a[set][i][c][2 * h + 1], (pw[0][i] >> (8 * (2 * set + c))) & 255u),
+                                                     ff_from_e4m3x8(b[set][j][c][2 * h], b[set][j][c][2 * h + 1], (qw[0][j] >> (8 * (2 * set + c))) & 255u), acc[i][j]);
         } else {
+            const ff_i32x8 av = __builtin_bit_cast(ff_i32x8, a[set][i]), bv = __builtin_bit_cast(ff_i32x8, b[set][j]);
+            acc[i][j] = set == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 0, 0, 0, (int)pw[0][i], 0, (int)qw[0][j])
+                                 : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 0, 0, 2, (int)pw[0][i], 2, (int)qw[0][j]);
+        }
+    };
+    for (int k0 = 0, pair = 0; k0 < K; k0 += 2 * BK, ++pair) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            ff_i32x8 a[TP], b[TQ];
-            auto fragment = [&](const char* tile, int row32) {
-                const int r = row32 + r32;
-                ff_u32x4 v[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    v[c] = *reinterpret_cast<const ff_u32x4*>(tile + r * (BK * 2) + (((4 * t + 2 * c + half) ^ ff_swz_inner<8>(r)) << 4));
-                return __builtin_bit_cast(ff_i32x8, v);
-            };
-#pragma unroll
-            for (int i = 0; i < TP; ++i) a[i] = fragment(bp, wp * SP + 32 * i);
-#pragma unroll
-            for (int j = 0; j < TQ; ++j) b[j] = fragment(bq, wq * SQ + 32 * j);
+        for (int set = 0; set < 2; ++set) {
+            // the next tile has landed, and the buffer to fill has been read; under way may be what the step before began
+            if (set == 0) ff_dma_barrier<LOADS*(STAGES - 3)>();
+            else ff_dma_barrier<LOADS*(STAGES - 3) + 1>();
+            if (set == 0) load_scales(pair + 2);
+            else read_words(1, pair + 1);
+            const int load_at = fill * BUF, load_k = k0 + (set + STAGES - 1) * BK, read_at = next * BUF;
+            constexpr int PRODUCTS = TP * TQ, OPS = READS + LOADS;
 #pragma unroll
             for (int i = 0; i < TP; ++i)
 #pragma unroll
-                for (int j = 0; j < TQ; ++j)
-                    acc[i][j] = t == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 0, 0, 0, (int)pc[i], 0, (int)qc[j])
-                                       : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 0, 0, 2, (int)pc[i], 2, (int)qc[j]);
+                for (int j = 0; j < TQ; ++j) {
+                    const int m = i * TQ + j;
+                    multiply(set, i, j);
+#pragma unroll
+                    for (int n = m * OPS / PRODUCTS; n < (m + 1) * OPS / PRODUCTS; ++n) {
+                        if (n < READS) read(n, set ^ 1, read_at);
+                        else if (n < READS + LP::PER_WAVE) lp.issue(n - READS, lds, load_at, load_k, K, wave, lane);
+                        else lq.issue(n - READS - LP::PER_WAVE, lds, load_at + LP::BYTES, load_k, K, wave, lane);
+                    }
+                    ff_keep_order();
+                }
+            cur = next;
+            next = next + 1 == STAGES ? 0 : next + 1;
+            fill = fill + 1 == STAGES ? 0 : fill + 1;
         }
-        }
-        cur ^= 1;
+#pragma unroll
+        for (int i = 0; i < TP; ++i) pw[0][i] = pw[1][i];
+#pragma unroll
+        for (int j = 0; j < TQ; ++j) qw[0][j] = qw[1][j];
     }
-    ff_dma_barrier<0>();
+    (void)cur;
+    ff_dma_barrier<0>();          // no load may land in LDS that the workgroup has given back
     ff_output<BP, BQ, WP, WQ, GATED>(reinterpret_cast<float*>(lds), acc, s, m0, n0, 0, epi);
+}
+
+// rows of scales -> rows of `pitch` bytes (a multiple of 4), scales of 1 behind the end
+__global__ void __launch_bounds__(256) k_ff_pad_scales(const uint8_t* __restrict__ src, int64_t rows, int blocks, int pitch, uint8_t* __restrict__ dst) {
+    const int64_t n = rows * pitch;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / pitch;
+        const int c = (int)(i - r * pitch);
+        dst[i] = c < blocks ? src[r * blocks + c] : (uint8_t)127;
+    }
 }
 
 // few rows (nf_ff_rows.h): 32 weight rows a workgroup, so that the features of an h block are one workgroup's; 128 values of k a unit, whose scales are a
 // word a row; 16 values a lane and step, as two bfloat16 operands
-constexpr int ff_rows8_most(int nt, bool gated) { return gated ? (nt >= 3 ? 4 : 8) : (nt >= 3 ? 8 : 16); }          // 64 KB of LDS at most
+constexpr int ff_rows8_most(int nt, bool gated) { return gated && nt >= 3 ? 4 : 8; }          // 64 KB of LDS at most
 template <int NT, bool GATED, typename T>
 __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1, FfScales sw, const uint8_t* __restrict__ x,
                                                    const uint8_t* __restrict__ xs, int M, int N, int K, T* __restrict__ out, uint8_t* __restrict__ hq,
@@ -312,9 +347,10 @@ struct Epi8Store {
     __device__ __forceinline__ void gated(int, int, int, int, bool, const ff_f32x4&, const ff_f32x4&) const {}
 };
 
+template <bool FAST>
 struct Epi8Gate {
     uint8_t *q, *scale;
-    int64_t F;
+    int64_t F, scale_pitch;
     int act;
     // 8 neighbouring lanes hold the 32 features of a block
     __device__ __forceinline__ void gated(int, int m, int n, int, bool inside, const ff_f32x4& g, const ff_f32x4& u) const {
@@ -323,7 +359,7 @@ struct Epi8Gate {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             float a, slope;
-            ff_act<false>(act, g[c], a, slope);
+            ff_act<FAST>(act, g[c], a, slope);
             v[c] = a * u[c];
             top = fmaxf(top, fabsf(v[c]));
             bad |= !(fabsf(v[c]) <= 3.4028235e38f);
@@ -334,14 +370,16 @@ struct Epi8Gate {
         const unsigned byte = ff_scale_byte(top);
         const float inv = byte == 255u ? NAN : ff_scale_inverse(byte);
         *reinterpret_cast<unsigned*>(q + m * F + n) = ff_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-        if (n % 32 == 0) scale[m * (F / 32) + n / 32] = (uint8_t)byte;
+        if (n % 32 == 0) scale[m * scale_pitch + n / 32] = (uint8_t)byte;
+        if (n + 4 == F)
+            for (int64_t c = F / 32; c < scale_pitch; ++c) scale[m * scale_pitch + c] = 127;
     }
     __device__ __forceinline__ void plain(int, int, int, int, bool, const ff_f32x4&) const {}
 };
 
 template <int BP, int BQ, int WP, int WQ, bool GATED, bool EXACT, typename Epi>
 int launch8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const FfScales& sq, int M, int N, int K, const Epi& epi, hipStream_t st) {
-    constexpr int RING = 2 * (BP + BQ) * 128, OUT = ff_output_bytes<BP, BQ, WP, WQ>(), LDS = RING > OUT ? RING : OUT, COLS = GATED ? BP / 2 : BP;
+    constexpr int RING = 4 * (BP + BQ) * 64 + 4 * (BP + BQ) * 4, OUT = ff_output_bytes<BP, BQ, WP, WQ>(), LDS = RING > OUT ? RING : OUT, COLS = GATED ? BP / 2 : BP;
     static bool set[NF_MAX_DEVICES];
     const int dev = nf_current_device();
     const auto kernel = k_ff_gemm8<BP, BQ, WP, WQ, GATED, EXACT, Epi>;
@@ -373,9 +411,36 @@ FfOperand operand8(const void* a, const void* b, int rows, int K) {
     return FfOperand{(const uint16_t*)a, (const uint16_t*)b, 0, K / 2, rows, 0x7fffffff, 0x7fffffff};
 }
 
+// the workspace of the tiled form: h in 8 bits, and the scales whose rows are no multiple of 4 bytes
+struct Plan8 {
+    uint8_t *hq, *hs, *xs = nullptr, *gs = nullptr, *us = nullptr, *ds = nullptr;
+    int64_t dp, fp;          // pitches of the scales of rows of D and F values
+    int64_t bytes = 0;
+    Plan8(uint8_t* base, int64_t M, int64_t D, int64_t F) {
+        dp = (D / 32 + 3) / 4 * 4;
+        fp = (F / 32 + 3) / 4 * 4;
+        auto take = [&](int64_t n) {
+            uint8_t* p = base ? base + bytes : nullptr;
+            bytes += (n + 255) / 256 * 256;
+            return p;
+        };
+        hq = take(M * F);
+        hs = take(M * fp);
+        if (dp != D / 32) xs = take(M * dp), gs = take(F * dp), us = take(F * dp);
+        if (fp != F / 32) ds = take(D * fp);
+    }
+};
+const uint8_t* padded_scales(const uint8_t* src, int64_t rows, int blocks, int64_t pitch, uint8_t* to, hipStream_t st) {
+    if (pitch == blocks) return src;
+    int64_t grid = (rows * pitch + 255) / 256;
+    if (grid > 4096) grid = 4096;
+    hipLaunchKernelGGL(k_ff_pad_scales, dim3((unsigned)grid), dim3(256), 0, st, src, rows, blocks, (int)pitch, to);
+    return to;
+}
+
 }  // namespace
 
-extern "C" int64_t nf_gated_ff_fwd_8bit_workspace_bytes(int64_t rows, int hidden) { return rows * hidden + rows * (hidden / 32) + 512; }
+extern "C" int64_t nf_gated_ff_fwd_8bit_workspace_bytes(int64_t rows, int dim, int hidden) { return Plan8(nullptr, rows, dim, hidden).bytes; }
 
 extern "C" int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const void* w_gate, const uint8_t* gate_scale, const void* w_up,
                                     const uint8_t* up_scale, const void* w_down, const uint8_t* down_scale, int64_t rows, int dim, int hidden,
@@ -386,24 +451,25 @@ extern "C" int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const
                "hidden %d dtype %d activation %d)", (long long)rows, dim, hidden, out_dtype, activation);
     hipStream_t st = (hipStream_t)stream;
     const int M = (int)rows, D = dim, F = hidden;
-    uint8_t* hq = (uint8_t*)workspace;
-    uint8_t* hs = hq + (rows * hidden + 255) / 256 * 256;
-    const Epi8Gate gate = {hq, hs, F, activation};
-    const FfOperand pg = operand8(w_gate, w_up, F, D), qx = operand8(x, x, M, D);
-    const FfScales spg = {gate_scale, up_scale, D / 32, F}, sqx = {x_scale, x_scale, D / 32, M};
+    const Plan8 f((uint8_t*)workspace, rows, dim, hidden);
     if (M <= 64) {
-        few_rows8<true, float>(w_gate, w_up, spg, x, x_scale, M, F, D, nullptr, hq, hs, activation, st);
+        const FfScales spg = {gate_scale, up_scale, D / 32, F};
+        few_rows8<true, float>(w_gate, w_up, spg, x, x_scale, M, F, D, nullptr, f.hq, f.hs, activation, st);
         const FfScales sd = {down_scale, down_scale, F / 32, D};
-        if (out_dtype == FF_F32) few_rows8<false, float>(w_down, nullptr, sd, hq, hs, M, D, F, (float*)out, nullptr, nullptr, 0, st);
-        else if (out_dtype == FF_BF16) few_rows8<false, ff_bf16>(w_down, nullptr, sd, hq, hs, M, D, F, (ff_bf16*)out, nullptr, nullptr, 0, st);
-        else few_rows8<false, ff_half>(w_down, nullptr, sd, hq, hs, M, D, F, (ff_half*)out, nullptr, nullptr, 0, st);
+        if (out_dtype == FF_F32) few_rows8<false, float>(w_down, nullptr, sd, f.hq, f.hs, M, D, F, (float*)out, nullptr, nullptr, 0, st);
+        else if (out_dtype == FF_BF16) few_rows8<false, ff_bf16>(w_down, nullptr, sd, f.hq, f.hs, M, D, F, (ff_bf16*)out, nullptr, nullptr, 0, st);
+        else few_rows8<false, ff_half>(w_down, nullptr, sd, f.hq, f.hs, M, D, F, (ff_half*)out, nullptr, nullptr, 0, st);
         NF_LAUNCH_CHECK("nf_gated_ff_fwd_8bit");
         return 0;
     }
-    int rc = out_dtype == FF_BF16 ? product8<true, false>(pg, qx, spg, sqx, M, F, D, gate, st) : product8<true, true>(pg, qx, spg, sqx, M, F, D, gate, st);
+    const FfOperand pg = operand8(w_gate, w_up, F, D), qx = operand8(x, x, M, D);
+    const FfScales sqx = {padded_scales(x_scale, M, D / 32, f.dp, f.xs, st), nullptr, f.dp, M};
+    const FfScales spg = {padded_scales(gate_scale, F, D / 32, f.dp, f.gs, st), padded_scales(up_scale, F, D / 32, f.dp, f.us, st), f.dp, F};
+    int rc = out_dtype == FF_BF16 ? product8<true, false>(pg, qx, spg, sqx, M, F, D, Epi8Gate<true>{f.hq, f.hs, F, f.fp, activation}, st)
+                                  : product8<true, true>(pg, qx, spg, sqx, M, F, D, Epi8Gate<false>{f.hq, f.hs, F, f.fp, activation}, st);
     if (rc) return rc;
-    const FfOperand p = operand8(w_down, w_down, D, F), q = operand8(hq, hq, M, F);
-    const FfScales sp = {down_scale, down_scale, F / 32, D}, sq = {hs, hs, F / 32, M};
+    const FfOperand p = operand8(w_down, w_down, D, F), q = operand8(f.hq, f.hq, M, F);
+    const FfScales sp = {padded_scales(down_scale, D, F / 32, f.fp, f.ds, st), nullptr, f.fp, D}, sq = {f.hs, f.hs, f.fp, M};
     if (out_dtype == FF_F32) rc = product8<false, true>(p, q, sp, sq, M, D, F, Epi8Store<float>{(float*)out, D}, st);
     else if (out_dtype == FF_BF16) rc = product8<false, false>(p, q, sp, sq, M, D, F, Epi8Store<ff_bf16>{(ff_bf16*)out, D}, st);
     else rc = product8<false, true>(p, q, sp, sq, M, D, F, Epi8Store<ff_half>{(ff_half*)out, D}, st);

@@ -1120,7 +1120,7 @@ def gated_ff_bwd(x, w_gate, w_up, w_down, dy, g, u, activation, want):
 
 
 def _pair_8bit(pair, rows, dim, name, like=None):
-    """(q, scale) checked against [rows, dim] (rows or dim None: any) -> contiguous, q 16-byte aligned"""
+    """(q, scale) checked against [rows, dim] (rows or dim None: any) -> contiguous, q 16-byte and scale 4-byte aligned"""
     q, scale = pair
     if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.float8_e8m0fnu:
         raise TypeError('%s must be a pair of float8_e4m3fn values and float8_e8m0fnu scales (got %s, %s)' % (name, q.dtype, scale.dtype))
@@ -1133,7 +1133,7 @@ def _pair_8bit(pair, rows, dim, name, like=None):
     _ff_shape(q, (q.shape[0] if rows is None else rows, q.shape[1] if dim is None else dim), name)
     _ff_shape(scale, (q.shape[0], q.shape[1] // 32), name + "'s scales")
     q, scale = q.contiguous(), scale.contiguous()
-    return (q if q.data_ptr() % 16 == 0 else q.clone()), scale
+    return (q if q.data_ptr() % 16 == 0 else q.clone()), (scale if scale.data_ptr() % 4 == 0 else scale.clone())
 
 
 def gated_ff_fwd_8bit(x, w_gate, w_up, w_down, activation, dtype):
@@ -1151,7 +1151,7 @@ def gated_ff_fwd_8bit(x, w_gate, w_up, w_down, activation, dtype):
     out = torch.empty(rows, dim, dtype=dtype, device=x[0].device)
     if rows:
         L = _lib.lib()
-        ws = _workspace_bytes(L.nf_gated_ff_fwd_8bit_workspace_bytes(rows, hidden), 'nf_gated_ff_fwd_8bit', out)
+        ws = _workspace_bytes(L.nf_gated_ff_fwd_8bit_workspace_bytes(rows, dim, hidden), 'nf_gated_ff_fwd_8bit', out)
         _ff_launch('nf_gated_ff_fwd_8bit', out, dict(rows=rows, dim=dim, hidden=hidden), *[_ptr(t) for pair in (x, w_gate, w_up, w_down) for t in pair], rows, dim, hidden,
                     _FF_DTYPES[dtype], act, _ptr(out), _ptr(ws))
     return out
