@@ -16,6 +16,8 @@
 
 typedef int ff_i32x8 __attribute__((ext_vector_type(8)));
 
+static __device__ unsigned ff_unit_scales = 0x7f7f7f7fu;          // four scales of 1
+
 namespace {
 
 struct FfScales {
@@ -35,8 +37,6 @@ __device__ __forceinline__ unsigned ff_scale_word(const uint8_t* row, int blk, i
     for (int i = 0; i < 4; ++i) w |= (blk + i < blocks ? (unsigned)row[blk + i] : 127u) << (8 * i);
     return w;
 }
-
-static __device__ unsigned ff_unit_scales = 0x7f7f7f7fu;          // four scales of 1
 
 // Steps go in pairs: 64 values of k a step, 128 a pair, whose four scales of a row are one word; the words come with a 4-byte LDS-DMA a wave and pair, two
 // pairs ahead, into a ring of their own (rows of words need a pitch of 4 bytes: the host pads other lengths with scales of 1).  A step past the
@@ -94,16 +94,17 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
         lp.load(lds, t * BUF, t * BK, K, wave, lane);
         lq.load(lds, t * BUF + LP::BYTES, t * BK, K, wave, lane);
     }
-    ff_u32x4 a[2][TP][2], b[2][TQ][2];
+    // (one set of fragments: each is read again, for the next step, behind its last product -- two sets do not fit the registers)
+    ff_u32x4 a[TP][2], b[TQ][2];
     unsigned pw[2][TP], qw[2][TQ];          // words of the pair at hand and of the next
     constexpr int READS = 2 * (TP + TQ);
-    auto read = [&](int n, int set, int at) {          // half n % 2 of a fragment: k 16 (lane / 32) .. + 15 of its 32
+    auto read = [&](int n, int at) {          // half n % 2 of a fragment: k 16 (lane / 32) .. + 15 of its 32
         const int f = n / 2, c = n % 2;
         const int row32 = f < TQ ? wq * SQ + 32 * f : wp * SP + 32 * (f - TQ), r = row32 + r32;
         const char* tile = lds + at + (f < TQ ? LP::BYTES : 0);
         const ff_u32x4 v = *reinterpret_cast<const ff_u32x4*>(tile + r * (BK * 2) + (((2 * c + half) ^ ff_swz_inner<4>(r)) << 4));
-        if (f < TQ) b[set][f][c] = v;
-        else a[set][f - TQ][c] = v;
+        if (f < TQ) b[f][c] = v;
+        else a[f - TQ][c] = v;
     };
     auto read_words = [&](int set, int pair) {
         const char* w = lds + SCALES + (pair & 3) * WORDS;
@@ -119,8 +120,6 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
         }
     };
     ff_dma_barrier<LOADS*(STAGES - 2)>();
-#pragma unroll
-    for (int n = 0; n < READS; ++n) read(n, 0, 0);
     read_words(0, 0);
     int cur = 0, next = 1, fill = STAGES - 1;
     auto multiply = [&](int set, int i, int j) {          // (set: also the step of the pair)
@@ -129,10 +128,10 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    acc[i][j] = FfMfma<ff_bf16>::mul(ff_from_e4m3x8(a[set][i][c][2 * h], a[set][i][c][2 * h + 1], (pw[0][i] >> (8 * (2 * set + c))) & 255u),
-                                                     ff_from_e4m3x8(b[set][j][c][2 * h], b[set][j][c][2 * h + 1], (qw[0][j] >> (8 * (2 * set + c))) & 255u), acc[i][j]);
+                    acc[i][j] = FfMfma<ff_bf16>::mul(ff_from_e4m3x8(a[i][c][2 * h], a[i][c][2 * h + 1], (pw[0][i] >> (8 * (2 * set + c))) & 255u),
+                                                     ff_from_e4m3x8(b[j][c][2 * h], b[j][c][2 * h + 1], (qw[0][j] >> (8 * (2 * set + c))) & 255u), acc[i][j]);
         } else {
-            const ff_i32x8 av = __builtin_bit_cast(ff_i32x8, a[set][i]), bv = __builtin_bit_cast(ff_i32x8, b[set][j]);
+            const ff_i32x8 av = __builtin_bit_cast(ff_i32x8, a[i]), bv = __builtin_bit_cast(ff_i32x8, b[j]);
             acc[i][j] = set == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 0, 0, 0, (int)pw[0][i], 0, (int)qw[0][j])
                                  : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 0, 0, 2, (int)pw[0][i], 2, (int)qw[0][j]);
         }
@@ -145,22 +144,15 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
             else ff_dma_barrier<LOADS*(STAGES - 3) + 1>();
             if (set == 0) load_scales(pair + 2);
             else read_words(1, pair + 1);
-            const int load_at = fill * BUF, load_k = k0 + (set + STAGES - 1) * BK, read_at = next * BUF;
-            constexpr int PRODUCTS = TP * TQ, OPS = READS + LOADS;
+            const int load_at = fill * BUF, load_k = k0 + (set + STAGES - 1) * BK;
+            lp.load(lds, load_at, load_k, K, wave, lane);
+            lq.load(lds, load_at + LP::BYTES, load_k, K, wave, lane);
+#pragma unroll
+            for (int n = 0; n < READS; ++n) read(n, cur * BUF);
 #pragma unroll
             for (int i = 0; i < TP; ++i)
 #pragma unroll
-                for (int j = 0; j < TQ; ++j) {
-                    const int m = i * TQ + j;
-                    multiply(set, i, j);
-#pragma unroll
-                    for (int n = m * OPS / PRODUCTS; n < (m + 1) * OPS / PRODUCTS; ++n) {
-                        if (n < READS) read(n, set ^ 1, read_at);
-                        else if (n < READS + LP::PER_WAVE) lp.issue(n - READS, lds, load_at, load_k, K, wave, lane);
-                        else lq.issue(n - READS - LP::PER_WAVE, lds, load_at + LP::BYTES, load_k, K, wave, lane);
-                    }
-                    ff_keep_order();
-                }
+                for (int j = 0; j < TQ; ++j) multiply(set, i, j);
             cur = next;
             next = next + 1 == STAGES ? 0 : next + 1;
             fill = fill + 1 == STAGES ? 0 : fill + 1;
