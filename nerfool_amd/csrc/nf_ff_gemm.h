@@ -11,9 +11,9 @@
 // The 16-byte chunks of a row are placed at (chunk ^ f(row)), so that neither the plain nor the transposed reads collide in the LDS banks; the
 // DMA writes lanes in order, hence the permutation is applied to the address that a lane reads.
 //
-// P is the A operand of v_mfma_f32_32x32x16 (rows in registers), Q the B operand (columns on lanes): a lane ends with one m and 4 consecutive n.
+// P is the A operand of v_mfma_f32_16x16x32 (rows in registers), Q the B operand (columns on lanes): a lane ends with one m and 4 consecutive n.
 // The results go through LDS, 32 rows of every wave at a time, so that the output stage reads and writes whole rows: from the fragments directly a
-// wave's 16-byte accesses lie in 32 rows, and the stage of dh's product (g, u in, three tensors out) took twice the time of its 64 k steps.
+// wave's 16-byte accesses lie in 16 or 32 rows, and the stage of dh's product (g, u in, three tensors out) took twice the time of its 64 k steps.
 #pragma once
 
 #include "nf_ff.h"
@@ -94,12 +94,12 @@ struct FfMfma;
 template <>
 struct FfMfma<ff_bf16> {
     typedef ff_bf16x8 V;
-    static __device__ __forceinline__ ff_f32x16 mul(V a, V b, ff_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ ff_f32x4 mul(V a, V b, ff_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct FfMfma<ff_half> {
     typedef ff_half8 V;
-    static __device__ __forceinline__ ff_f32x16 mul(V a, V b, ff_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ ff_f32x4 mul(V a, V b, ff_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
 // where chunk c (16 bytes) of row r of an LDS tile lies; CH chunks a row
@@ -108,8 +108,8 @@ __device__ __forceinline__ int ff_swz_inner(int r) {          // rows are n or m
     return CH == 8 ? (r >> 1) & 7 : (r >> 2) & 3;          // (16 lanes of a read cover the 64 banks once)
 }
 template <int CH>
-__device__ __forceinline__ int ff_swz_outer(int k) {          // rows are k, read 4 rows x 32 bytes a quarter wave
-    return CH >= 16 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
+__device__ __forceinline__ int ff_swz_outer(int k) {          // rows are k, read 4 rows x 32 bytes a quarter wave, quarters 8 rows apart
+    return (CH >= 16 ? (k & 3) << 2 : (k & 2) << 1) ^ (((k >> 3) & 1) << 1);
 }
 
 // one operand's share of the tile loads of a wave
@@ -176,16 +176,17 @@ struct FfLoader {
     }
 };
 
-// the 8 k of a fragment: row `row` (of this lane) of the tile plane at `tile`, k block kk of 16
+// a 16 x 32 fragment of the tile plane at `tile`: lane l holds row row16 + l mod 16, k = 8 (l / 16) .. + 7
 template <typename V, int ROWS, int BK, bool OUTER>
-__device__ __forceinline__ V ff_fragment(const char* tile, int row32, int kk, int lane) {
+__device__ __forceinline__ V ff_fragment(const char* tile, int row16, int lane) {
+    static_assert(BK == 32, "a k step is one fragment");
     constexpr int CH = OUTER ? ROWS / 8 : BK / 8;
     if (!OUTER) {
-        const int r = row32 + (lane & 31), chunk = 2 * kk + (lane >> 5);
-        return *reinterpret_cast<const V*>(tile + r * (BK * 2) + ((chunk ^ ff_swz_inner<CH>(r)) << 4));
+        const int r = row16 + (lane & 15);
+        return *reinterpret_cast<const V*>(tile + r * (BK * 2) + (((lane >> 4) ^ ff_swz_inner<CH>(r)) << 4));
     } else {
-        // quarter wave g: rows 16 (g & 1) .., k 8 (g >> 1) ..; two transposed reads of 4 k
-        const int i = lane & 15, col = row32 + ((lane >> 4) & 1) * 16 + (i & 3) * 4, k = 16 * kk + (lane >> 5) * 8 + (i >> 2);
+        // a quarter wave reads rows k = 8 (l / 16) + 4 s + i / 4, columns row16 + 4 (i % 4) .. + 3, and gets its transpose
+        const int i = lane & 15, col = row16 + (i & 3) * 4, k = (lane >> 4) * 8 + (i >> 2);
         uint64_t t[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -223,20 +224,30 @@ constexpr int ff_output_bytes() {
 }
 // The accumulators of a tile -> epi, 4 consecutive n of a row at a time: epi.plain(part, m, n, left, inside, v) or epi.gated(part, m, n, left, inside, gate, up), left = s.N - n.
 // Every thread makes every call (epi may exchange values between neighbouring lanes, which hold neighbouring n of the row); inside: the place exists.
-template <int BP, int BQ, int WP, int WQ, bool GATED, int TP, int TQ, typename Epi>
-__device__ __forceinline__ void ff_output(float* lds, const ff_f32x16 (&acc)[TP][TQ], const FfShape& s, int m0, int n0, int part, const Epi& epi) {
+template <int BP, int BQ, int WP, int WQ, bool GATED, typename Acc, int TP, int TQ, typename Epi>
+__device__ __forceinline__ void ff_output(float* lds, const Acc (&acc)[TP][TQ], const FfShape& s, int m0, int n0, int part, const Epi& epi) {
+    constexpr bool SMALL = sizeof(Acc) == 16;          // 16 x 16 blocks, else 32 x 32
     constexpr int SP = BP / WP, SQ = BQ / WQ, PITCH = BP + 4, COLS = GATED ? BP / 2 : BP, THREADS = WP * WQ * 64, ITEMS = WQ * 32 * COLS / 4;
     static_assert(ITEMS % THREADS == 0, "every thread makes the same number of calls");
     const int lane = threadIdx.x & 63, wave = ff_wave_index(), wp = wave % WP, wq = wave / WP;
 #pragma unroll
-    for (int j = 0; j < TQ; ++j) {
+    for (int j = 0; j < SQ / 32; ++j) {
         if (j) __syncthreads();
-        float* row = lds + (wq * 32 + (lane & 31)) * PITCH + wp * SP + 4 * (lane >> 5);
+        if constexpr (SMALL) {
 #pragma unroll
-        for (int i = 0; i < TP; ++i)
+            for (int h = 0; h < 2; ++h) {
+                float* row = lds + (wq * 32 + 16 * h + (lane & 15)) * PITCH + wp * SP + 4 * (lane >> 4);
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<ff_f32x4*>(row + 32 * i + 8 * g) = ff_f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                for (int i = 0; i < TP; ++i) *reinterpret_cast<ff_f32x4*>(row + 16 * i) = acc[i][2 * j + h];
+            }
+        } else {
+            float* row = lds + (wq * 32 + (lane & 31)) * PITCH + wp * SP + 4 * (lane >> 5);
+#pragma unroll
+            for (int i = 0; i < TP; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<ff_f32x4*>(row + 32 * i + 8 * g) = ff_f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        }
         __syncthreads();
 #pragma unroll 2
         for (int it = threadIdx.x; it < ITEMS; it += THREADS) {
@@ -256,7 +267,7 @@ __device__ __forceinline__ void ff_output(float* lds, const ff_f32x16 (&acc)[TP]
 template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, int STAGES, bool PO, bool QO, bool GATED, typename Epi>
 __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand q, FfShape s, Epi epi) {
     typedef typename FfMfma<E>::V V;
-    constexpr int WAVES = WP * WQ, SP = BP / WP, SQ = BQ / WQ, TP = SP / 32, TQ = SQ / 32;
+    constexpr int WAVES = WP * WQ, SP = BP / WP, SQ = BQ / WQ, TP = SP / 16, TQ = SQ / 16;
     typedef FfLoader<NP, BP, BK, WAVES, PO, GATED, SP> LP;
     typedef FfLoader<NP, BQ, BK, WAVES, QO, false, SQ> LQ;
     constexpr int BUF = LP::BYTES + LQ::BYTES;
@@ -272,42 +283,40 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand 
     LQ lq;
     lp.init(p, n0, k_lo, wave, lane);
     lq.init(q, m0, k_lo, wave, lane);
-    ff_f32x16 acc[TP][TQ];
+    ff_f32x4 acc[TP][TQ];
 #pragma unroll
     for (int i = 0; i < TP; ++i)
 #pragma unroll
-        for (int j = 0; j < TQ; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        for (int j = 0; j < TQ; ++j) acc[i][j] = ff_f32x4{0.f, 0.f, 0.f, 0.f};
     constexpr int LOADS = LP::PER_WAVE + LQ::PER_WAVE;
 #pragma unroll
     for (int t = 0; t < STAGES - 1; ++t) {
         lp.load(lds, t * BUF, k_lo + t * BK, k_hi, wave, lane);
         lq.load(lds, t * BUF + LP::BYTES, k_lo + t * BK, k_hi, wave, lane);
     }
-    // Fragments are read one k block of 16 ahead of their products, across the step's end too: a barrier therefore says that the NEXT tile has landed.
-    // The reads and the loads are put between the products by hand, one or two behind each: left to itself the compiler gathers the
-    // reads in front of their products to save registers, and the matrix pipe waits for them.
-    V a[2][NP][TP], b[2][NP][TQ];
-    constexpr int KK = BK / 16, READS = NP * (TP + TQ), PRODUCTS = NP * (NP + 1) / 2 * TP * TQ;
-    static_assert(KK % 2 == 0 && STAGES >= 3, "two fragment sets in turn; the next tile lands before the last load starts");
-    auto read = [&](int n, int set, int at, int kk) {
-        const int e = n / (TP + TQ), f = n % (TP + TQ);
-        if (f < TQ) b[set][e][f] = ff_fragment<V, BQ, BK, QO>(lds + at + LP::BYTES + e * (LQ::BYTES / NP), wq * SQ + 32 * f, kk, lane);
-        else a[set][e][f - TQ] = ff_fragment<V, BP, BK, PO>(lds + at + e * (LP::BYTES / NP), wp * SP + 32 * (f - TQ), kk, lane);
+    V a[NP][TP], b[2][NP][TQ];
+    auto read_p = [&](int at, int i) {
+#pragma unroll
+        for (int e = 0; e < NP; ++e) a[e][i] = ff_fragment<V, BP, BK, PO>(lds + at + e * (LP::BYTES / NP), wp * SP + 16 * i, lane);
     };
-    ff_dma_barrier<LOADS*(STAGES - 2)>();
+    auto read_q = [&](int at, int set, int n) {
+        const int e = n / TQ, j = n % TQ;
+        b[set][e][j] = ff_fragment<V, BQ, BK, QO>(lds + at + LP::BYTES + e * (LQ::BYTES / NP), wq * SQ + 16 * j, lane);
+    };
+    int next = 1, fill = STAGES - 1;
+    if constexpr (NP == 3) {
+        // Three stages of three planes fill the LDS: a step waits for its own tile only, with the next one under way, and reads its fragments at its head.  (Waiting
+        // for the next tile as below leaves one step for a load to arrive: 39 us instead of 33 for 1500 x 2666 x 500.)
+        static_assert(STAGES == 3, "");
+        int cur = 0;
+        for (int k0 = k_lo; k0 < k_hi; k0 += BK) {
+            ff_dma_barrier<LOADS*(STAGES - 2)>();          // the tile has landed for every wave, and the buffer to fill has been read by every wave
+            lp.load(lds, fill * BUF, k0 + (STAGES - 1) * BK, k_hi, wave, lane);
+            lq.load(lds, fill * BUF + LP::BYTES, k0 + (STAGES - 1) * BK, k_hi, wave, lane);
 #pragma unroll
-    for (int n = 0; n < READS; ++n) read(n, 0, 0, 0);
-    int cur = 0, next = 1, fill = STAGES - 1;
-    for (int k0 = k_lo; k0 < k_hi; k0 += BK) {
-        ff_dma_barrier<LOADS*(STAGES - 3)>();          // the next tile has landed for every wave, and the buffer to fill has been read by every wave
-        const int load_at = fill * BUF, load_k = k0 + (STAGES - 1) * BK;
+            for (int n = 0; n < NP * TQ; ++n) read_q(cur * BUF, 0, n);
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const int set = kk & 1, read_at = kk + 1 < KK ? cur * BUF : next * BUF, read_kk = kk + 1 < KK ? kk + 1 : 0;
-            const int ops = kk == 0 ? READS + LOADS : READS;
-            int m = 0;
+            for (int i = 0; i < TP; ++i) read_p(cur * BUF, i);
             // smallest products first
 #pragma unroll
             for (int o = NP - 1; o >= 0; --o)
@@ -316,21 +325,52 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand 
 #pragma unroll
                     for (int i = 0; i < TP; ++i)
 #pragma unroll
-                        for (int j = 0; j < TQ; ++j, ++m) {
-                            acc[i][j] = FfMfma<E>::mul(a[set][e][i], b[set][o - e][j], acc[i][j]);
+                        for (int j = 0; j < TQ; ++j) acc[i][j] = FfMfma<E>::mul(a[e][i], b[0][o - e][j], acc[i][j]);
+            cur = cur + 1 == STAGES ? 0 : cur + 1;
+            fill = fill + 1 == STAGES ? 0 : fill + 1;
+        }
+    } else {
+    // A step's fragments are read during the step before (a barrier therefore says that the NEXT tile has landed): each of P's behind its own last
+    // product, Q's into a second set.  The reads and the loads are put between the products by hand: left to itself the compiler gathers the
+    // reads in front of their products to save registers, and the matrix pipe waits for them.
+    constexpr int PRODUCTS = NP * (NP + 1) / 2 * TP * TQ, OPS = NP * TQ + LOADS;
+    static_assert(STAGES >= 4, "the next tile lands before the last load starts");
+    ff_dma_barrier<LOADS*(STAGES - 2)>();
 #pragma unroll
-                            for (int n = m * ops / PRODUCTS; n < (m + 1) * ops / PRODUCTS; ++n) {
+    for (int n = 0; n < NP * TQ; ++n) read_q(0, 0, n);
+#pragma unroll
+    for (int i = 0; i < TP; ++i) read_p(0, i);
+    for (int k0 = k_lo; k0 < k_hi; k0 += 2 * BK) {
+#pragma unroll
+        for (int set = 0; set < 2; ++set) {          // (the second step may lie behind the end: it multiplies zeros)
+            ff_dma_barrier<LOADS*(STAGES - 3)>();          // the next tile has landed for every wave, and the buffer to fill has been read by every wave
+            const int load_at = fill * BUF, load_k = k0 + (set + STAGES - 1) * BK, read_at = next * BUF;
+            int m = 0;
+#pragma unroll
+            for (int i = 0; i < TP; ++i) {
+                // smallest products first
+#pragma unroll
+                for (int o = NP - 1; o >= 0; --o)
+#pragma unroll
+                    for (int e = 0; e <= o; ++e)
+#pragma unroll
+                        for (int j = 0; j < TQ; ++j, ++m) {
+                            acc[i][j] = FfMfma<E>::mul(a[e][i], b[set][o - e][j], acc[i][j]);
+#pragma unroll
+                            for (int n = m * OPS / PRODUCTS; n < (m + 1) * OPS / PRODUCTS; ++n) {
                                 // (loads behind the end go on, from the page of zeros: the count of those under way stays right)
-                                if (n < READS) read(n, set ^ 1, read_at, read_kk);
-                                else if (n < READS + LP::PER_WAVE) lp.issue(n - READS, lds, load_at, load_k, k_hi, wave, lane);
-                                else lq.issue(n - READS - LP::PER_WAVE, lds, load_at + LP::BYTES, load_k, k_hi, wave, lane);
+                                if (n < NP * TQ) read_q(read_at, set ^ 1, n);
+                                else if (n < NP * TQ + LP::PER_WAVE) lp.issue(n - NP * TQ, lds, load_at, load_k, k_hi, wave, lane);
+                                else lq.issue(n - NP * TQ - LP::PER_WAVE, lds, load_at + LP::BYTES, load_k, k_hi, wave, lane);
                             }
+                            if (o == 0 && j == TQ - 1) read_p(read_at, i);
                             ff_keep_order();
                         }
+            }
+            next = next + 1 == STAGES ? 0 : next + 1;
+            fill = fill + 1 == STAGES ? 0 : fill + 1;
         }
-        cur = next;
-        next = next + 1 == STAGES ? 0 : next + 1;
-        fill = fill + 1 == STAGES ? 0 : fill + 1;
+    }
     }
     ff_dma_barrier<0>();          // no load may land in LDS that the workgroup has given back
     ff_output<BP, BQ, WP, WQ, GATED>(reinterpret_cast<float*>(lds), acc, s, m0, n0, part, epi);

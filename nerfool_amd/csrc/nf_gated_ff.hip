@@ -163,16 +163,26 @@ __global__ void __launch_bounds__(256) k_ff_join(EpiPart parts, int n_parts, int
     }
 }
 
-// rows [R, C] -> rows padded with zeros to `pitch` (a multiple of 8); float -> three planes of bf16 parts
+// rows [R, C] -> rows padded with zeros to `pitch` (a multiple of 8); float -> three planes of bf16 parts.  Up to 5 tensors a launch: blockIdx.y
 template <typename T>
-__global__ void __launch_bounds__(256) k_ff_pack(const T* __restrict__ src, int64_t rows, int cols, FfMid<T> dst) {
-    const int per_row = (int)(dst.pitch / 4);
-    const int64_t n = rows * per_row;
+struct FfPackJobs {
+    struct Job {
+        const T* src;
+        int64_t rows;
+        int cols;
+        FfMid<T> dst;
+    } job[5];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) k_ff_pack(FfPackJobs<T> jobs) {
+    const auto& job = jobs.job[blockIdx.y];
+    const int per_row = (int)(job.dst.pitch / 4);
+    const int64_t n = job.rows * per_row;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / per_row;
-        const int c = (int)(i - r * per_row) * 4, left = cols - c;
+        const int c = (int)(i - r * per_row) * 4, left = job.cols - c;
         ff_f32x4 v;
-        const T* s = src + r * cols + c;
+        const T* s = job.src + r * job.cols + c;
         if (left >= 4) {
             typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
             const V4 t = *reinterpret_cast<const V4*>(s);
@@ -180,7 +190,7 @@ __global__ void __launch_bounds__(256) k_ff_pack(const T* __restrict__ src, int6
             for (int j = 0; j < 4; ++j) v[j] = (float)t[j];
         } else
             for (int j = 0; j < 4; ++j) v[j] = j < left ? (float)s[j] : 0.f;
-        dst.put(r, c, left > 0 ? left : 0, v);
+        job.dst.put(r, c, left > 0 ? left : 0, v);
     }
 }
 
@@ -250,16 +260,31 @@ FfPacked<T> pack_at(Carve& ws, int64_t rows, int cols) {
     }
     return p;
 }
+// collects the tensors to copy; those that need no copy are operands as they are
 template <typename T>
-void pack_run(const void* src, int64_t rows, int cols, FfPacked<T>& p, hipStream_t st) {
-    if (!p.copy) {
-        p.mid.p = (decltype(p.mid.p))const_cast<void*>(src);
-        return;
+struct Packing {
+    FfPackJobs<T> jobs;
+    int n = 0;
+    int64_t most = 0;
+    void add(const void* src, int64_t rows, int cols, FfPacked<T>& p) {
+        if (!p.copy) {
+            p.mid.p = (decltype(p.mid.p))const_cast<void*>(src);
+            return;
+        }
+        jobs.job[n++] = {(const T*)src, rows, cols, p.mid};
+        const int64_t items = rows * (p.mid.pitch / 4);
+        most = items > most ? items : most;
     }
-    int64_t blocks = (rows * (p.mid.pitch / 4) + 255) / 256;
-    if (blocks > 256 * 16) blocks = 256 * 16;
-    hipLaunchKernelGGL((k_ff_pack<T>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)src, rows, cols, p.mid);
-}
+    void run(hipStream_t st) {
+        if (!n) return;
+        int64_t blocks = (most + 255) / 256;
+        if (blocks > 256 * 8) blocks = 256 * 8;
+        hipLaunchKernelGGL((k_ff_pack<T>), dim3((unsigned)blocks, n), dim3(256), 0, st, jobs);
+    }
+};
+
+// steps of a part of k: even, as the kernel takes them in pairs
+int64_t ff_part_steps(int64_t steps, int parts) { return ((steps + parts - 1) / parts + 1) / 2 * 2; }
 
 template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, int STAGES, bool PO, bool QO, bool GATED, typename Epi>
 int launch(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, int parts, const Epi& epi, hipStream_t st) {
@@ -279,33 +304,38 @@ int launch(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int 
     s.M = M, s.N = N, s.K = K, s.n_end = n_end;
     s.tiles_m = (M + BQ - 1) / BQ, s.tiles_n = (N + COLS - 1) / COLS;
     const int steps = (K + BK - 1) / BK;
-    s.k_part = (steps + parts - 1) / parts * BK;
+    s.k_part = ff_part_steps(steps, parts) * BK;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(s.tiles_m * s.tiles_n * parts)), dim3(WP * WQ * 64), LDS, st, p, q, s, epi);
     return 0;
 }
 
-// ---- which tile, and in how many parts k is cut.  The time of a product, in microseconds, as measured on its pieces: a 256 x 256 tile takes 0.95 a k step of 32 and
-//      has a CU for itself; two 128 x 128 tiles share one and take 0.7 a step together; of a float32 operand's three planes a 128 x 128 tile takes 1.4 a step.  A tile
-//      costs about 8 steps beside its k loop (first loads, output stage).  Parts cost their writing and reading, and a launch.
+// ---- which tile, and in how many parts k is cut.  The time of a product, in microseconds, as measured on its pieces: a 256 x 256 tile takes 0.85 a k step of 32 and
+//      has a CU for itself; two 128 x 128 tiles share one and take 0.7 a step together.  Of a float32 operand's three planes a 128 x 128 tile takes 1.2 a step.  (Tiles of
+//      128 x 64 take 0.85 a step: no gain.)  A tile costs about 8 steps beside its k loop (first loads, output stage).  Parts cost their writing and reading, and a launch.
+enum { TILE_256, TILE_128, TILE_128_THREE };
 struct FfChoice {
-    bool big;
-    int parts;
+    int tile, parts;
 };
 FfChoice ff_choose(bool three, int64_t M, int64_t N, int64_t K, bool may_split) {
-    FfChoice best = {false, 1};
+    static const struct {
+        int bm, bn, slots;
+        double step;
+    } tiles[3] = {{256, 256, 256, 0.85}, {128, 128, 512, 0.7}, {128, 128, 256, 1.2}};
+    FfChoice best = {three ? TILE_128_THREE : TILE_128, 1};
     double least = 1e30;
-    for (int big = three ? 0 : 1; big >= 0; --big) {
-        const int64_t b = big ? 256 : 128, tiles = ((M + b - 1) / b) * ((N + b - 1) / b), steps = (K + 31) / 32, slots = big || three ? 256 : 512;
-        const double step = three ? 1.4 : big ? 0.95 : 0.7;
+    const int64_t steps = (K + 31) / 32;
+    for (int tile = three ? TILE_128_THREE : TILE_256; tile <= (three ? TILE_128_THREE : TILE_128); ++tile) {
+        const auto& c = tiles[tile];
+        const int64_t count = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
         for (int parts = 1; parts <= 8; ++parts) {
             if (parts > 1 && (!may_split || steps < 8 * parts)) break;
-            const int64_t per = (steps + parts - 1) / parts, n = tiles * parts;
+            const int64_t per = ff_part_steps(steps, parts), n = count * parts;
             if (per * (parts - 1) >= steps) continue;          // the last part would be empty
             // (a last round that fills less than half of a 128 x 128 tile's slots has the CUs' whole rate for one tile each)
-            const int64_t rounds = n / slots, rest = n % slots;
-            double t = rounds * (per + 8) * step + (rest ? (per + 8) * step * (!big && !three && rest <= 256 ? 0.6 : 1.0) : 0.0);
+            const int64_t rounds = n / c.slots, rest = n % c.slots;
+            double t = rounds * (per + 8) * c.step + (rest ? (per + 8) * c.step * (tile == TILE_128 && rest <= 256 ? 0.6 : 1.0) : 0.0);
             if (parts > 1) t += 4.0 + (double)M * N * 4 * (parts + 1) / 4.5e6;
-            if (t < least) least = t, best = {big != 0, parts};
+            if (t < least) least = t, best = {tile, parts};
         }
     }
     return best;
@@ -323,7 +353,7 @@ int product_as(const FfChoice& c, const FfOperand& p, const FfOperand& q, int M,
     if constexpr (FfElem<T>::NP == 3) {
         return launch<E, 3, 128, 128, 2, 4, 32, 3, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
     } else {
-        if (c.big) return launch<E, 1, 256, 256, 2, 4, 32, 4, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
+        if (c.tile == TILE_256) return launch<E, 1, 256, 256, 2, 4, 32, 4, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
         return launch<E, 1, 128, 128, 2, 2, 32, 4, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
     }
 }
@@ -389,10 +419,12 @@ int ff_fwd(const void* x, const void* wg, const void* wu, const void* wd, int M,
         return few_rows<T, false>(wd, nullptr, workspace, M, D, F, out, nullptr, nullptr, 0, st);
     }
     FwdPlan<T> f((char*)workspace, M, D, F);
-    pack_run<T>(x, M, D, f.x, st);
-    pack_run<T>(wg, F, D, f.wg, st);
-    pack_run<T>(wu, F, D, f.wu, st);
-    pack_run<T>(wd, D, F, f.wd, st);
+    Packing<T> pack;
+    pack.add(x, M, D, f.x);
+    pack.add(wg, F, D, f.wg);
+    pack.add(wu, F, D, f.wu);
+    pack.add(wd, D, F, f.wd);
+    pack.run(st);
     FfOperand p = as_operand(f.wg.mid, F);
     p.b = (const uint16_t*)f.wu.mid.p;
     const EpiGate<T> gate = {f.h, g_save, u_save, F, act};
@@ -438,15 +470,20 @@ int ff_bwd(const void* x, const void* wg, const void* wu, const void* wd, const 
     const bool dwgu = dwg || dwu;
     BwdPlan<T> f((char*)workspace, M, D, F, dx != nullptr, dwgu, dwd != nullptr);
     const int Fp = (int)pad8(F);
-    pack_run<T>(dy, M, D, f.dy, st);
-    pack_run<T>(wd, D, F, f.wd, st);
+    Packing<T> pack;
+    pack.add(dy, M, D, f.dy);
+    pack.add(wd, D, F, f.wd);
+    if (dx) {
+        pack.add(wg, F, D, f.wg);
+        pack.add(wu, F, D, f.wu);
+    }
+    if (dwgu) pack.add(x, M, D, f.x);
+    pack.run(st);
     // dh[m][f] = sum over d of dy[m][d] Wd[d][f]
     const EpiGateBwd<T> gate = {f.dgu, f.h, g, u, F, Fp, act, dwd != nullptr};
     FfOperand p = as_operand(f.wd.mid, (int)f.wd.mid.pitch);
     FF_TRY((product<T, true, false, false>(p, as_operand(f.dy.mid, M), M, F, Fp, D, gate, st)));
     if (dx) {          // dx[m][d] = sum over k of dgu[m][k] [Wg; zeros up to Fp; Wu][k][d]
-        pack_run<T>(wg, F, D, f.wg, st);
-        pack_run<T>(wu, F, D, f.wu, st);
         p = as_operand(f.wg.mid, (int)f.wg.mid.pitch);
         p.b = (const uint16_t*)f.wu.mid.p;
         p.len = F, p.seg = Fp;
@@ -454,7 +491,6 @@ int ff_bwd(const void* x, const void* wg, const void* wu, const void* wd, const 
         FF_TRY((product_split<T, true, false>(p, as_operand(f.dgu, M), M, D, Fp + F, store, f.parts, st)));
     }
     if (dwgu) {          // [dWg; dWu][f][d] = sum over m of dgu[m][f] x[m][d]
-        pack_run<T>(x, M, D, f.x, st);
         const EpiStore<T> store = {(T*)dwg, (T*)dwu, D, F, Fp};
         FF_TRY((product_split<T, true, true>(as_operand(f.x.mid, (int)f.x.mid.pitch), as_operand(f.dgu, 2 * Fp), 2 * Fp, D, M, store, f.parts, st)));
     }

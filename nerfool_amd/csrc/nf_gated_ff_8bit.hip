@@ -128,8 +128,8 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    acc[i][j] = FfMfma<ff_bf16>::mul(ff_from_e4m3x8(a[i][c][2 * h], a[i][c][2 * h + 1], (pw[0][i] >> (8 * (2 * set + c))) & 255u),
-                                                     ff_from_e4m3x8(b[j][c][2 * h], b[j][c][2 * h + 1], (qw[0][j] >> (8 * (2 * set + c))) & 255u), acc[i][j]);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ff_from_e4m3x8(a[i][c][2 * h], a[i][c][2 * h + 1], (pw[0][i] >> (8 * (2 * set + c))) & 255u),
+                                                     ff_from_e4m3x8(b[j][c][2 * h], b[j][c][2 * h + 1], (qw[0][j] >> (8 * (2 * set + c))) & 255u), acc[i][j], 0, 0, 0);
         } else {
             const ff_i32x8 av = __builtin_bit_cast(ff_i32x8, a[i]), bv = __builtin_bit_cast(ff_i32x8, b[j]);
             acc[i][j] = set == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 0, 0, 0, (int)pw[0][i], 0, (int)qw[0][j])
