@@ -5,9 +5,9 @@
 //   k innermost    row r at a + r * pitch, k contiguous.  A gated P has two sources: the features' gate rows in a and their up rows in b.
 //   k outermost    row k at a + k * pitch (k < seg) or b + (k - seg) * pitch, the product's n or m contiguous: the gradients' products read the
 //                  tensors as they lie, the transposition happens in the LDS read (ds_read_b64_tr_b16).
-// Tiles go global -> LDS by LDS-DMA, 16 bytes a lane, into a ring of STAGES buffers, STAGES - 1 k steps ahead of their use: a step waits for its own tile
-// only (the counter of outstanding loads), with one barrier.  Nothing passes through registers.  A lane whose 16 bytes lie
-// behind the end of k, n or m reads a page of zeros instead (k, and n or m where they are contiguous, are multiples of 8: the host pads what is not).
+// Tiles go global -> LDS by LDS-DMA, 16 bytes a lane, one or two k steps ahead of their use; nothing passes through registers.  A lane whose 16 bytes lie
+// behind the end of k reads a page of zeros instead, one behind the end of n or m the last rows or columns again (k, and n or m where they are contiguous, are
+// multiples of 8: the host pads what is not).
 // The 16-byte chunks of a row are placed at (chunk ^ f(row)), so that neither the plain nor the transposed reads collide in the LDS banks; the
 // DMA writes lanes in order, hence the permutation is applied to the address that a lane reads.
 //
@@ -15,6 +15,8 @@
 // The results go through LDS, 32 rows of every wave at a time, so that the output stage reads and writes whole rows: from the fragments directly a
 // wave's 16-byte accesses lie in 16 or 32 rows, and the stage of dh's product (g, u in, three tensors out) took twice the time of its 64 k steps.
 #pragma once
+
+#include <type_traits>
 
 #include "nf_ff.h"
 
@@ -38,6 +40,19 @@ __device__ __forceinline__ void ff_dma16(const void* src, char* lds, int at, int
                  : "memory");
 #else
     __builtin_memcpy(lds + at + 16 * lane, src, 16);
+#endif
+}
+// ... from base + off, off the lane's own, base the same for the wave
+__device__ __forceinline__ void ff_dma16(const char* base, unsigned off, char* lds, int at, int lane) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    unsigned keep;
+    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds + at);
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(off), "s"(to), "s"(base)
+                 : "memory");
+#else
+    __builtin_memcpy(lds + at + 16 * lane, base + off, 16);
 #endif
 }
 // ... 4 bytes a lane
@@ -112,7 +127,8 @@ __device__ __forceinline__ int ff_swz_outer(int k) {          // rows are k, rea
     return (CH >= 16 ? (k & 3) << 2 : (k & 2) << 1) ^ (((k >> 3) & 1) << 1);
 }
 
-// one operand's share of the tile loads of a wave
+// One operand's share of the tile loads of a wave.  A lane keeps a 32-bit offset a load; what changes from tile to tile is the same for the wave.  A tile whose 16-byte
+// pieces all exist (whole()) is loaded by these alone; another one, at the end of k or where a's rows end and b's begin, goes lane by lane, with zeros where nothing is.
 template <int NP, int ROWS, int BK, int WAVES, bool OUTER, bool GATED, int WSPAN>
 struct FfLoader {
     static constexpr int CH = OUTER ? ROWS / 8 : BK / 8;                     // chunks of an LDS row
@@ -121,72 +137,83 @@ struct FfLoader {
     static constexpr int RPP = 64 / CH;                                       // LDS rows a piece
     static constexpr int BYTES = NP * PIECES * 1024;
     static_assert(NP * PIECES % WAVES == 0, "every wave moves the same number of pieces");
-    const uint16_t* ptr[PER_WAVE];
-    int64_t step, jump;
-    int kc, len, seg;     // kc: this lane's k inside the tile (k innermost)
-    unsigned valid;       // outer: whether the column exists
+    static_assert(!GATED || (WSPAN / 2) % RPP == 0, "a piece's rows are of one source");
+    unsigned off[PER_WAVE];
+    const char *a, *b;
+    int64_t plane, pitch;          // bytes
+    int len, seg;
 
-    __device__ __forceinline__ void init(const FfOperand& o, int row0, int k0, int wave, int lane) {
+    __device__ __forceinline__ void init(const FfOperand& o, int row0, int wave, int lane) {
         const int slot = lane % CH, rr = lane / CH;
+        a = (const char*)o.a;
+        b = (const char*)o.b;
+        plane = o.plane * 2;
+        pitch = o.pitch * 2;
         len = o.len;
         seg = o.seg;
-        jump = OUTER ? (o.b - o.a) - (int64_t)o.seg * o.pitch : 0;
-        step = OUTER ? (int64_t)BK * o.pitch : BK;
-        valid = 0;
+        if (!OUTER) {
+            a += row0 * pitch;
+            b += row0 * pitch;
+        }
 #pragma unroll
         for (int i = 0; i < PER_WAVE; ++i) {
-            const int li = wave * PER_WAVE + i, plane = li / PIECES, r = (li % PIECES) * RPP + rr;
+            const int r = (wave * PER_WAVE + i) % PIECES * RPP + rr;
+            // a row, or columns, behind the end: the last ones, whose results are not stored
             if (OUTER) {
-                const int col = row0 + 8 * (slot ^ ff_swz_outer<CH>(r));
-                if (col < o.rows) valid |= 1u << i;
-                ptr[i] = o.a + plane * o.plane + (int64_t)(k0 + r) * o.pitch + col;
+                int col = row0 + 8 * (slot ^ ff_swz_outer<CH>(r));
+                if (col >= o.rows) col = o.rows - 8;
+                off[i] = (unsigned)(r * pitch + 2 * col);
             } else {
-                const int chunk = slot ^ ff_swz_inner<CH>(r);
-                kc = 8 * (slot ^ ff_swz_inner<CH>(rr));          // (of an even piece; see k_of)
-                const uint16_t* base = o.a;
-                int row;
-                if (GATED) {          // a wave's WSPAN rows: half gate, half up, of the same features
-                    const int in = r % WSPAN;
-                    row = row0 + (r / WSPAN) * (WSPAN / 2) + in % (WSPAN / 2);
-                    if (in >= WSPAN / 2) base = o.b;
-                } else
-                    row = row0 + r;
-                if (row >= o.rows) row = o.rows - 1;          // a row behind the end: any values, its results are not stored
-                ptr[i] = base + plane * o.plane + (int64_t)row * o.pitch + k0 + 8 * chunk;
+                int row = GATED ? (r / WSPAN) * (WSPAN / 2) + r % (WSPAN / 2) : r;          // a wave's WSPAN rows: half gate, half up, of the same features
+                if (row0 + row >= o.rows) row = o.rows - 1 - row0;
+                off[i] = (unsigned)(row * pitch + 16 * (slot ^ ff_swz_inner<CH>(r)));
             }
         }
     }
-    // this lane's k in a tile's piece: where a piece is 8 rows, the next piece's rows swap the row's halves
-    __device__ __forceinline__ int k_of(int piece) const { return CH == 8 ? kc ^ ((piece & 1) << 5) : kc; }
-    // piece i of this wave of the tile at k0 (which the pointers stand at) -> lds + at
+    __device__ __forceinline__ bool whole(int k0, int K) const { return k0 + BK <= K && (!OUTER || k0 >= seg || k0 + BK <= len); }
+    // piece i of this wave of the tile at k0 -> lds + at
+    template <bool WHOLE>
     __device__ __forceinline__ void issue(int i, char* lds, int at, int k0, int K, int wave, int lane) {
         const int li = wave * PER_WAVE + i;
-        const void* src;
-        if (OUTER) {
-            const int k = k0 + (li % PIECES) * RPP + lane / CH;
-            src = k < K && (k < len || k >= seg) && ((valid >> i) & 1u) ? (const void*)(ptr[i] + (k >= seg ? jump : 0)) : (const void*)&ff_zero_page;
-        } else
-            src = k0 + k_of(li % PIECES) < K ? (const void*)ptr[i] : (const void*)&ff_zero_page;
-        ff_dma16(src, lds, at + li * 1024, lane);
-        ptr[i] += step;
+        const char* base = GATED && li % PIECES * RPP % WSPAN >= WSPAN / 2 ? b : a;
+        if (OUTER) base = k0 >= seg ? b + (k0 - seg) * pitch : a + k0 * pitch;
+        else base += 2 * (int64_t)k0;
+        if (NP > 1) base += li / PIECES * plane;
+        if (WHOLE) {
+            ff_dma16(base, off[i], lds, at + li * 1024, lane);
+        } else {
+            const void* src = base + off[i];
+            bool in;
+            if (OUTER) {
+                const int k = k0 + li % PIECES * RPP + lane / CH;
+                in = k < K && (k < len || k >= seg);
+                if (k0 < seg && k >= seg) src = (const char*)src + ((b - a) - seg * pitch);
+            } else
+                in = k0 + 8 * ((lane % CH) ^ ff_swz_inner<CH>(li % PIECES * RPP + lane / CH)) < K;
+            ff_dma16(in ? src : (const void*)&ff_zero_page, lds, at + li * 1024, lane);
+        }
     }
     __device__ __forceinline__ void load(char* lds, int at, int k0, int K, int wave, int lane) {
+        if (whole(k0, K)) {
 #pragma unroll
-        for (int i = 0; i < PER_WAVE; ++i) issue(i, lds, at, k0, K, wave, lane);
+            for (int i = 0; i < PER_WAVE; ++i) issue<true>(i, lds, at, k0, K, wave, lane);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER_WAVE; ++i) issue<false>(i, lds, at, k0, K, wave, lane);
+        }
     }
 };
 
-// a 16 x 32 fragment of the tile plane at `tile`: lane l holds row row16 + l mod 16, k = 8 (l / 16) .. + 7
+// a 16 x 32 fragment of the tile plane at `tile`, k block kk of 32: lane l holds row row16 + l mod 16, k = 8 (l / 16) .. + 7
 template <typename V, int ROWS, int BK, bool OUTER>
-__device__ __forceinline__ V ff_fragment(const char* tile, int row16, int lane) {
-    static_assert(BK == 32, "a k step is one fragment");
+__device__ __forceinline__ V ff_fragment(const char* tile, int row16, int kk, int lane) {
     constexpr int CH = OUTER ? ROWS / 8 : BK / 8;
     if (!OUTER) {
         const int r = row16 + (lane & 15);
-        return *reinterpret_cast<const V*>(tile + r * (BK * 2) + (((lane >> 4) ^ ff_swz_inner<CH>(r)) << 4));
+        return *reinterpret_cast<const V*>(tile + r * (BK * 2) + (((4 * kk + (lane >> 4)) ^ ff_swz_inner<CH>(r)) << 4));
     } else {
         // a quarter wave reads rows k = 8 (l / 16) + 4 s + i / 4, columns row16 + 4 (i % 4) .. + 3, and gets its transpose
-        const int i = lane & 15, col = row16 + (i & 3) * 4, k = (lane >> 4) * 8 + (i >> 2);
+        const int i = lane & 15, col = row16 + (i & 3) * 4, k = 32 * kk + (lane >> 4) * 8 + (i >> 2);
         uint64_t t[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -264,7 +291,7 @@ __device__ __forceinline__ void ff_output(float* lds, const Acc (&acc)[TP][TQ], 
 }
 
 // tile BP (rows of P) x BQ (rows of Q), WP x WQ waves
-template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, int STAGES, bool PO, bool QO, bool GATED, typename Epi>
+template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, bool PO, bool QO, bool GATED, typename Epi>
 __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand q, FfShape s, Epi epi) {
     typedef typename FfMfma<E>::V V;
     constexpr int WAVES = WP * WQ, SP = BP / WP, SQ = BQ / WQ, TP = SP / 16, TQ = SQ / 16;
@@ -281,42 +308,42 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand 
     const int k_lo = part * s.k_part, k_hi = k_lo + s.k_part < s.K ? k_lo + s.k_part : s.K;
     LP lp;
     LQ lq;
-    lp.init(p, n0, k_lo, wave, lane);
-    lq.init(q, m0, k_lo, wave, lane);
+    lp.init(p, n0, wave, lane);
+    lq.init(q, m0, wave, lane);
     ff_f32x4 acc[TP][TQ];
 #pragma unroll
     for (int i = 0; i < TP; ++i)
 #pragma unroll
         for (int j = 0; j < TQ; ++j) acc[i][j] = ff_f32x4{0.f, 0.f, 0.f, 0.f};
     constexpr int LOADS = LP::PER_WAVE + LQ::PER_WAVE;
-#pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t) {
-        lp.load(lds, t * BUF, k_lo + t * BK, k_hi, wave, lane);
-        lq.load(lds, t * BUF + LP::BYTES, k_lo + t * BK, k_hi, wave, lane);
-    }
+    auto load_tile = [&](int stage, int k0) {
+        lp.load(lds, stage * BUF, k0, k_hi, wave, lane);
+        lq.load(lds, stage * BUF + LP::BYTES, k0, k_hi, wave, lane);
+    };
     V a[NP][TP], b[2][NP][TQ];
-    auto read_p = [&](int at, int i) {
+    auto read_p = [&](int at, int i, int kk) {
 #pragma unroll
-        for (int e = 0; e < NP; ++e) a[e][i] = ff_fragment<V, BP, BK, PO>(lds + at + e * (LP::BYTES / NP), wp * SP + 16 * i, lane);
+        for (int e = 0; e < NP; ++e) a[e][i] = ff_fragment<V, BP, BK, PO>(lds + at + e * (LP::BYTES / NP), wp * SP + 16 * i, kk, lane);
     };
-    auto read_q = [&](int at, int set, int n) {
+    auto read_q = [&](int at, int set, int n, int kk) {
         const int e = n / TQ, j = n % TQ;
-        b[set][e][j] = ff_fragment<V, BQ, BK, QO>(lds + at + LP::BYTES + e * (LQ::BYTES / NP), wq * SQ + 16 * j, lane);
+        b[set][e][j] = ff_fragment<V, BQ, BK, QO>(lds + at + LP::BYTES + e * (LQ::BYTES / NP), wq * SQ + 16 * j, kk, lane);
     };
-    int next = 1, fill = STAGES - 1;
     if constexpr (NP == 3) {
-        // Three stages of three planes fill the LDS: a step waits for its own tile only, with the next one under way, and reads its fragments at its head.  (Waiting
-        // for the next tile as below leaves one step for a load to arrive: 39 us instead of 33 for 1500 x 2666 x 500.)
-        static_assert(STAGES == 3, "");
-        int cur = 0;
+        // Three planes of a step of 32: three stages of them fill the LDS.  A step waits for its own tile only, with the next one under way, and reads its fragments at
+        // its head.
+        static_assert(BK == 32, "");
+        constexpr int STAGES = 3;
+        load_tile(0, k_lo);
+        load_tile(1, k_lo + BK);
+        int cur = 0, fill = STAGES - 1;
         for (int k0 = k_lo; k0 < k_hi; k0 += BK) {
-            ff_dma_barrier<LOADS*(STAGES - 2)>();          // the tile has landed for every wave, and the buffer to fill has been read by every wave
-            lp.load(lds, fill * BUF, k0 + (STAGES - 1) * BK, k_hi, wave, lane);
-            lq.load(lds, fill * BUF + LP::BYTES, k0 + (STAGES - 1) * BK, k_hi, wave, lane);
+            ff_dma_barrier<LOADS>();          // the tile has landed for every wave, and the buffer to fill has been read by every wave
+            load_tile(fill, k0 + (STAGES - 1) * BK);          // (behind the end the loads go on, from the page of zeros: the count of those under way stays right)
 #pragma unroll
-            for (int n = 0; n < NP * TQ; ++n) read_q(cur * BUF, 0, n);
+            for (int n = 0; n < NP * TQ; ++n) read_q(cur * BUF, 0, n, 0);
 #pragma unroll
-            for (int i = 0; i < TP; ++i) read_p(cur * BUF, i);
+            for (int i = 0; i < TP; ++i) read_p(cur * BUF, i, 0);
             // smallest products first
 #pragma unroll
             for (int o = NP - 1; o >= 0; --o)
@@ -330,47 +357,49 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand 
             fill = fill + 1 == STAGES ? 0 : fill + 1;
         }
     } else {
-    // A step's fragments are read during the step before (a barrier therefore says that the NEXT tile has landed): each of P's behind its own last
-    // product, Q's into a second set.  The reads and the loads are put between the products by hand: left to itself the compiler gathers the
-    // reads in front of their products to save registers, and the matrix pipe waits for them.
-    constexpr int PRODUCTS = NP * (NP + 1) / 2 * TP * TQ, OPS = NP * TQ + LOADS;
-    static_assert(STAGES >= 4, "the next tile lands before the last load starts");
-    ff_dma_barrier<LOADS*(STAGES - 2)>();
+        // A step is 64 k (128-byte rows: whole cache lines; with steps of 32 the L2 gave half its rate) in two halves, two stages.  The fragments of a half are read during
+        // the half before, each of P's behind its own last product, Q's into a second set: with the first half's products the tile has been read, and one barrier there says
+        // both that the next tile has landed and that this one's buffer may be filled again.  The reads and the loads are put between the products by hand:
+        // left to itself the compiler gathers the reads in front of their products to save registers, and the matrix pipe waits for them.
+        static_assert(BK == 64, "");
+        constexpr int PRODUCTS = TP * TQ;
+        load_tile(0, k_lo);
+        load_tile(1, k_lo + BK);
+        ff_dma_barrier<LOADS>();
 #pragma unroll
-    for (int n = 0; n < NP * TQ; ++n) read_q(0, 0, n);
+        for (int j = 0; j < TQ; ++j) read_q(0, 0, j, 0);
 #pragma unroll
-    for (int i = 0; i < TP; ++i) read_p(0, i);
-    for (int k0 = k_lo; k0 < k_hi; k0 += 2 * BK) {
+        for (int i = 0; i < TP; ++i) read_p(0, i, 0);
+        int cur = 0;
+        auto products = [&](auto which, auto whole, int read_at, int load_at, int load_k) {
+            constexpr int half = decltype(which)::value, OPS = half == 0 ? TQ : TQ + LOADS;
 #pragma unroll
-        for (int set = 0; set < 2; ++set) {          // (the second step may lie behind the end: it multiplies zeros)
-            ff_dma_barrier<LOADS*(STAGES - 3)>();          // the next tile has landed for every wave, and the buffer to fill has been read by every wave
-            const int load_at = fill * BUF, load_k = k0 + (set + STAGES - 1) * BK, read_at = next * BUF;
-            int m = 0;
+            for (int i = 0; i < TP; ++i)
 #pragma unroll
-            for (int i = 0; i < TP; ++i) {
-                // smallest products first
+                for (int j = 0; j < TQ; ++j) {
+                    const int m = i * TQ + j;
+                    acc[i][j] = FfMfma<E>::mul(a[0][i], b[half][0][j], acc[i][j]);
 #pragma unroll
-                for (int o = NP - 1; o >= 0; --o)
-#pragma unroll
-                    for (int e = 0; e <= o; ++e)
-#pragma unroll
-                        for (int j = 0; j < TQ; ++j, ++m) {
-                            acc[i][j] = FfMfma<E>::mul(a[e][i], b[set][o - e][j], acc[i][j]);
-#pragma unroll
-                            for (int n = m * OPS / PRODUCTS; n < (m + 1) * OPS / PRODUCTS; ++n) {
-                                // (loads behind the end go on, from the page of zeros: the count of those under way stays right)
-                                if (n < NP * TQ) read_q(read_at, set ^ 1, n);
-                                else if (n < NP * TQ + LP::PER_WAVE) lp.issue(n - NP * TQ, lds, load_at, load_k, k_hi, wave, lane);
-                                else lq.issue(n - NP * TQ - LP::PER_WAVE, lds, load_at + LP::BYTES, load_k, k_hi, wave, lane);
-                            }
-                            if (o == 0 && j == TQ - 1) read_p(read_at, i);
-                            ff_keep_order();
-                        }
-            }
-            next = next + 1 == STAGES ? 0 : next + 1;
-            fill = fill + 1 == STAGES ? 0 : fill + 1;
-        }
-    }
+                    for (int n = m * OPS / PRODUCTS; n < (m + 1) * OPS / PRODUCTS; ++n) {
+                        if (n < TQ) read_q(read_at, half ^ 1, n, half ^ 1);
+                        else if (n < TQ + LP::PER_WAVE) lp.template issue<decltype(whole)::value>(n - TQ, lds, load_at, load_k, k_hi, wave, lane);
+                        else lq.template issue<decltype(whole)::value>(n - TQ - LP::PER_WAVE, lds, load_at + LP::BYTES, load_k, k_hi, wave, lane);
+                    }
+                    if (j == TQ - 1) read_p(read_at, i, half ^ 1);
+                    ff_keep_order();
+                }
+        };
+        auto step = [&](auto whole, int k0) {
+            products(std::integral_constant<int, 0>(), whole, cur * BUF, 0, 0);
+            ff_dma_barrier<0>();
+            products(std::integral_constant<int, 1>(), whole, (cur ^ 1) * BUF, cur * BUF, k0 + 2 * BK);
+            cur ^= 1;
+        };
+        // two loops, not a choice inside one: the sums of two branches would meet in other registers
+        int k0 = k_lo;
+        const int k_whole = PO && p.len < k_hi && !(p.len == p.seg && p.len % BK == 0) ? p.len : k_hi;
+        for (; k0 + 3 * BK <= k_whole; k0 += BK) step(std::true_type(), k0);
+        for (; k0 < k_hi; k0 += BK) step(std::false_type(), k0);
     }
     ff_dma_barrier<0>();          // no load may land in LDS that the workgroup has given back
     ff_output<BP, BQ, WP, WQ, GATED>(reinterpret_cast<float*>(lds), acc, s, m0, n0, part, epi);

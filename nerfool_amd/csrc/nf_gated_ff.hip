@@ -283,15 +283,15 @@ struct Packing {
     }
 };
 
-// steps of a part of k: even, as the kernel takes them in pairs
+// steps (of 32) of a part of k: even, as a step of the 16-bit kernel is two of them
 int64_t ff_part_steps(int64_t steps, int parts) { return ((steps + parts - 1) / parts + 1) / 2 * 2; }
 
-template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, int STAGES, bool PO, bool QO, bool GATED, typename Epi>
+template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, bool PO, bool QO, bool GATED, typename Epi>
 int launch(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, int parts, const Epi& epi, hipStream_t st) {
-    constexpr int RING = STAGES * NP * (BP + BQ) * BK * 2, OUT = ff_output_bytes<BP, BQ, WP, WQ>(), LDS = RING > OUT ? RING : OUT, COLS = GATED ? BP / 2 : BP;
+    constexpr int RING = (NP == 3 ? 3 : 2) * NP * (BP + BQ) * BK * 2, OUT = ff_output_bytes<BP, BQ, WP, WQ>(), LDS = RING > OUT ? RING : OUT, COLS = GATED ? BP / 2 : BP;
     static bool set[NF_MAX_DEVICES];
     const int dev = nf_current_device();
-    const auto kernel = k_ff_gemm<E, NP, BP, BQ, WP, WQ, BK, STAGES, PO, QO, GATED, Epi>;
+    const auto kernel = k_ff_gemm<E, NP, BP, BQ, WP, WQ, BK, PO, QO, GATED, Epi>;
     if (!set[dev]) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) {
@@ -304,7 +304,7 @@ int launch(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int 
     s.M = M, s.N = N, s.K = K, s.n_end = n_end;
     s.tiles_m = (M + BQ - 1) / BQ, s.tiles_n = (N + COLS - 1) / COLS;
     const int steps = (K + BK - 1) / BK;
-    s.k_part = ff_part_steps(steps, parts) * BK;
+    s.k_part = ff_part_steps(steps * (BK / 32), parts) * 32;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(s.tiles_m * s.tiles_n * parts)), dim3(WP * WQ * 64), LDS, st, p, q, s, epi);
     return 0;
 }
@@ -351,10 +351,10 @@ template <typename T, bool PO, bool QO, bool GATED, typename Epi>
 int product_as(const FfChoice& c, const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
     typedef typename FfElem<T>::E E;
     if constexpr (FfElem<T>::NP == 3) {
-        return launch<E, 3, 128, 128, 2, 4, 32, 3, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
+        return launch<E, 3, 128, 128, 2, 4, 32, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
     } else {
-        if (c.tile == TILE_256) return launch<E, 1, 256, 256, 2, 4, 32, 4, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
-        return launch<E, 1, 128, 128, 2, 2, 32, 4, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
+        if (c.tile == TILE_256) return launch<E, 1, 256, 256, 2, 4, 64, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
+        return launch<E, 1, 128, 128, 2, 2, 64, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
     }
 }
 // the whole sum over k in one tile

@@ -60,8 +60,8 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
     const int words = (K + 63) / 64;
     LP lp;
     LQ lq;
-    lp.init(p, n0, 0, wave, lane);
-    lq.init(q, m0, 0, wave, lane);
+    lp.init(p, n0, wave, lane);
+    lq.init(q, m0, wave, lane);
     const uint8_t* srow;          // the row whose words this lane moves
     {
         const int v = wave * 64 + lane;
