@@ -405,10 +405,12 @@ constexpr int FF_ROWS_MAX = 64;
 
 template <typename T, bool GATED>
 int few_rows(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, hipStream_t st) {
-    if (M <= 16) return ff_rows_launch<T, 1, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
-    if (M <= 32) return ff_rows_launch<T, 2, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
-    if (M <= 48) return ff_rows_launch<T, 3, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
-    return ff_rows_launch<T, 4, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+    switch (ff_rows_tokens(M, (N + 15) / 16)) {
+        case 1: return ff_rows_launch<T, 1, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+        case 2: return ff_rows_launch<T, 2, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+        case 3: return ff_rows_launch<T, 3, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+        default: return ff_rows_launch<T, 4, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+    }
 }
 
 template <typename T>

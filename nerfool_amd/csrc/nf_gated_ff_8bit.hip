@@ -38,17 +38,16 @@ __device__ __forceinline__ unsigned ff_scale_word(const uint8_t* row, int blk, i
     return w;
 }
 
-// Steps go in pairs: 64 values of k a step, 128 a pair, whose four scales of a row are one word; the words come with a 4-byte LDS-DMA a wave and pair, two
-// pairs ahead, into a ring of their own (rows of words need a pitch of 4 bytes: the host pads other lengths with scales of 1).  A step past the
-// end multiplies zeros by scales of 1.
+// A step is 128 values of k (128-byte rows) in two halves of one instruction's 64, two stages, as in k_ff_gemm; a row's four scales of a step are one word, which comes by a 4-byte
+// LDS-DMA a row, into a ring of its own (rows of words need a pitch of 4 bytes: the host pads other lengths with scales of 1).
 // EXACT: the products in bfloat16
 template <int BP, int BQ, int WP, int WQ, bool GATED, bool EXACT, typename Epi>
 __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand q, FfScales sp, FfScales sq, FfShape s, Epi epi) {
-    constexpr int BK = 32, STAGES = 4;          // BK in pairs of values
+    constexpr int BK = 64;          // in pairs of values
     constexpr int WAVES = WP * WQ, SP = BP / WP, SQ = BQ / WQ, TP = SP / 32, TQ = SQ / 32;
     typedef FfLoader<1, BP, BK, WAVES, false, GATED, SP> LP;
     typedef FfLoader<1, BQ, BK, WAVES, false, false, SQ> LQ;
-    constexpr int BUF = LP::BYTES + LQ::BYTES, LOADS = LP::PER_WAVE + LQ::PER_WAVE, SCALES = STAGES * BUF, WORDS = (BP + BQ) * 4;
+    constexpr int BUF = LP::BYTES + LQ::BYTES, LOADS = LP::PER_WAVE + LQ::PER_WAVE, SCALES = 2 * BUF, WORDS = (BP + BQ) * 4;
     static_assert(BP + BQ == WAVES * 64, "a wave moves the words of 64 rows");
     HIP_DYNAMIC_SHARED(char, lds)
     const int lane = threadIdx.x & 63, wave = ff_wave_index(), r32 = lane & 31, half = lane >> 5;
@@ -76,9 +75,9 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
             srow = sq.a + row * sq.pitch;
         }
     }
-    auto load_scales = [&](int pair) {
-        const void* src = pair < words ? (const void*)(srow + 4 * pair) : (const void*)&ff_unit_scales;
-        ff_dma4(src, lds, SCALES + (pair & 3) * WORDS + wave * 256, lane);
+    auto load_scales = [&](int word) {          // (a word behind the end is not used: its values are zeros, and the scales must be no NaN)
+        const void* src = word < words ? (const void*)(srow + 4 * word) : (const void*)&ff_unit_scales;
+        ff_dma4(src, lds, SCALES + (word & 1) * WORDS + wave * 256, lane);
     };
     ff_f32x16 acc[TP][TQ];
 #pragma unroll
@@ -87,82 +86,88 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm8(FfOperand p, FfOperand
         for (int j = 0; j < TQ; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    load_scales(0);
-    load_scales(1);
 #pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t) {
+    for (int t = 0; t < 2; ++t) {
+        load_scales(t);
         lp.load(lds, t * BUF, t * BK, K, wave, lane);
         lq.load(lds, t * BUF + LP::BYTES, t * BK, K, wave, lane);
     }
-    // (one set of fragments: each is read again, for the next step, behind its last product -- two sets do not fit the registers)
+    // one set of fragments: each is read again, for the next half, behind its last product
     ff_u32x4 a[TP][2], b[TQ][2];
-    unsigned pw[2][TP], qw[2][TQ];          // words of the pair at hand and of the next
-    constexpr int READS = 2 * (TP + TQ);
-    auto read = [&](int n, int at) {          // half n % 2 of a fragment: k 16 (lane / 32) .. + 15 of its 32
-        const int f = n / 2, c = n % 2;
-        const int row32 = f < TQ ? wq * SQ + 32 * f : wp * SP + 32 * (f - TQ), r = row32 + r32;
-        const char* tile = lds + at + (f < TQ ? LP::BYTES : 0);
-        const ff_u32x4 v = *reinterpret_cast<const ff_u32x4*>(tile + r * (BK * 2) + (((2 * c + half) ^ ff_swz_inner<4>(r)) << 4));
-        if (f < TQ) b[f][c] = v;
-        else a[f - TQ][c] = v;
+    unsigned pw[TP], qw[TQ];
+    auto fragment = [&](int row32, int at, int h, int c) {          // part c of half h of a row: k 64 h + 32 c + 16 (lane / 32) .. + 15
+        const int r = row32 + r32;
+        return *reinterpret_cast<const ff_u32x4*>(lds + at + r * (BK * 2) + (((4 * h + 2 * c + half) ^ ff_swz_inner<8>(r)) << 4));
     };
-    auto read_words = [&](int set, int pair) {
-        const char* w = lds + SCALES + (pair & 3) * WORDS;
+    auto read_p = [&](int i, int at, int h) {
 #pragma unroll
-        for (int i = 0; i < TP; ++i) pw[set][i] = *reinterpret_cast<const unsigned*>(w + 4 * (wp * SP + 32 * i + r32));
-#pragma unroll
-        for (int j = 0; j < TQ; ++j) qw[set][j] = *reinterpret_cast<const unsigned*>(w + 4 * (BP + wq * SQ + 32 * j + r32));
-        if (!EXACT) {          // the instruction takes byte 0 (first step) or 2 (second) of the lane's word: its own half's block
-#pragma unroll
-            for (int i = 0; i < TP; ++i) pw[set][i] >>= 8 * half;
-#pragma unroll
-            for (int j = 0; j < TQ; ++j) qw[set][j] >>= 8 * half;
-        }
+        for (int c = 0; c < 2; ++c) a[i][c] = fragment(wp * SP + 32 * i, at, h, c);
     };
-    ff_dma_barrier<LOADS*(STAGES - 2)>();
-    read_words(0, 0);
-    int cur = 0, next = 1, fill = STAGES - 1;
-    auto multiply = [&](int set, int i, int j) {          // (set: also the step of the pair)
+    auto read_q = [&](int j, int at, int h) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) b[j][c] = fragment(wq * SQ + 32 * j, at + LP::BYTES, h, c);
+    };
+    auto word = [&](int row, int slot) {
+        const unsigned w = *reinterpret_cast<const unsigned*>(lds + SCALES + slot * WORDS + 4 * row);
+        return EXACT ? w : w >> (8 * half);          // the instruction takes byte 0 (first half) or 2 (second) of the lane's word: its own block's
+    };
+    auto multiply = [&](auto which, int i, int j) {
+        constexpr int h = decltype(which)::value;
         if constexpr (EXACT) {
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ff_from_e4m3x8(a[i][c][2 * h], a[i][c][2 * h + 1], (pw[0][i] >> (8 * (2 * set + c))) & 255u),
-                                                     ff_from_e4m3x8(b[j][c][2 * h], b[j][c][2 * h + 1], (qw[0][j] >> (8 * (2 * set + c))) & 255u), acc[i][j], 0, 0, 0);
+                for (int e = 0; e < 2; ++e)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ff_from_e4m3x8(a[i][c][2 * e], a[i][c][2 * e + 1], (pw[i] >> (8 * (2 * h + c))) & 255u),
+                                                                        ff_from_e4m3x8(b[j][c][2 * e], b[j][c][2 * e + 1], (qw[j] >> (8 * (2 * h + c))) & 255u),
+                                                                        acc[i][j], 0, 0, 0);
         } else {
             const ff_i32x8 av = __builtin_bit_cast(ff_i32x8, a[i]), bv = __builtin_bit_cast(ff_i32x8, b[j]);
-            acc[i][j] = set == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 0, 0, 0, (int)pw[0][i], 0, (int)qw[0][j])
-                                 : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 0, 0, 2, (int)pw[0][i], 2, (int)qw[0][j]);
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 0, 0, 2 * h, (int)pw[i], 2 * h, (int)qw[j]);
         }
     };
-    for (int k0 = 0, pair = 0; k0 < K; k0 += 2 * BK, ++pair) {
+    ff_dma_barrier<LOADS + 1>();
 #pragma unroll
-        for (int set = 0; set < 2; ++set) {
-            // the next tile has landed, and the buffer to fill has been read; under way may be what the step before began
-            if (set == 0) ff_dma_barrier<LOADS*(STAGES - 3)>();
-            else ff_dma_barrier<LOADS*(STAGES - 3) + 1>();
-            if (set == 0) load_scales(pair + 2);
-            else read_words(1, pair + 1);
-            const int load_at = fill * BUF, load_k = k0 + (set + STAGES - 1) * BK;
-            lp.load(lds, load_at, load_k, K, wave, lane);
-            lq.load(lds, load_at + LP::BYTES, load_k, K, wave, lane);
+    for (int j = 0; j < TQ; ++j) read_q(j, 0, 0);
 #pragma unroll
-            for (int n = 0; n < READS; ++n) read(n, cur * BUF);
+    for (int i = 0; i < TP; ++i) read_p(i, 0, 0);
+    int cur = 0;
+    auto products = [&](auto which, auto whole, int read_at, int load_k) {
+        constexpr int h = decltype(which)::value, PRODUCTS = TP * TQ;
 #pragma unroll
-            for (int i = 0; i < TP; ++i)
+        for (int j = 0; j < TQ; ++j)
 #pragma unroll
-                for (int j = 0; j < TQ; ++j) multiply(set, i, j);
-            cur = next;
-            next = next + 1 == STAGES ? 0 : next + 1;
-            fill = fill + 1 == STAGES ? 0 : fill + 1;
-        }
+            for (int i = 0; i < TP; ++i) {
+                const int m = j * TP + i;
+                multiply(which, i, j);
+                if (h == 1) {
 #pragma unroll
-        for (int i = 0; i < TP; ++i) pw[0][i] = pw[1][i];
+                    for (int n = m * LOADS / PRODUCTS; n < (m + 1) * LOADS / PRODUCTS; ++n) {
+                        if (n < LP::PER_WAVE) lp.template issue<decltype(whole)::value>(n, lds, cur * BUF, load_k, K, wave, lane);
+                        else lq.template issue<decltype(whole)::value>(n - LP::PER_WAVE, lds, cur * BUF + LP::BYTES, load_k, K, wave, lane);
+                    }
+                }
+                if (j == TQ - 1) read_p(i, read_at, h ^ 1);
+                if (i == TP - 1) {
+                    read_q(j, read_at, h ^ 1);
+                    if (!EXACT) ff_keep_order();          // (behind each product the fixed order costs registers that are not there)
+                }
+            }
+    };
+    auto step = [&](auto whole, int k0) {
 #pragma unroll
-        for (int j = 0; j < TQ; ++j) qw[0][j] = qw[1][j];
-    }
-    (void)cur;
+        for (int i = 0; i < TP; ++i) pw[i] = word(wp * SP + 32 * i + r32, cur);
+#pragma unroll
+        for (int j = 0; j < TQ; ++j) qw[j] = word(BP + wq * SQ + 32 * j + r32, cur);
+        products(std::integral_constant<int, 0>(), whole, cur * BUF, 0);
+        ff_dma_barrier<0>();          // the tile has been read, the next one has landed
+        load_scales(k0 / BK + 2);
+        products(std::integral_constant<int, 1>(), whole, (cur ^ 1) * BUF, k0 + 2 * BK);
+        cur ^= 1;
+    };
+    int k0 = 0;
+    for (; k0 + 3 * BK <= K; k0 += BK) step(std::true_type(), k0);
+    for (; k0 < K; k0 += BK) step(std::false_type(), k0);
     ff_dma_barrier<0>();          // no load may land in LDS that the workgroup has given back
     ff_output<BP, BQ, WP, WQ, GATED>(reinterpret_cast<float*>(lds), acc, s, m0, n0, 0, epi);
 }
@@ -177,20 +182,21 @@ __global__ void __launch_bounds__(256) k_ff_pad_scales(const uint8_t* __restrict
     }
 }
 
-// few rows (nf_ff_rows.h): 32 weight rows a workgroup, so that the features of an h block are one workgroup's; 128 values of k a unit, whose scales are a
-// word a row; 16 values a lane and step, as two bfloat16 operands
+// few rows (nf_ff_rows.h): 128 values of k a unit, whose scales are a word a row; 16 values a lane and step, as two bfloat16 operands.  The gated form has 32 weight rows
+// a workgroup, so that the features of an h block are one workgroup's
 constexpr int ff_rows8_most(int nt, bool gated) { return gated && nt >= 3 ? 4 : 8; }          // 64 KB of LDS at most
 template <int NT, bool GATED, typename T>
 __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1, FfScales sw, const uint8_t* __restrict__ x,
                                                    const uint8_t* __restrict__ xs, int M, int N, int K, T* __restrict__ out, uint8_t* __restrict__ hq,
                                                    uint8_t* __restrict__ hs, int act) {
-    constexpr int NW = GATED ? 2 : 1, U = 2, UNIT = 128;
+    constexpr int NW = GATED ? 2 : 1, HG = GATED ? 2 : 1, U = 2, UNIT = 128;
     HIP_DYNAMIC_SHARED(ff_f32x4, part)
+    const int t0 = blockIdx.y * 16 * NT;          // this workgroup's first token
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int r = lane & 15, q = lane >> 4, n0 = blockIdx.x * 32, blocks = K / 32;
-    const uint8_t *wr[NW][2], *ws[NW][2], *xr[NT], *xsr[NT];
+    const int r = lane & 15, q = lane >> 4, n0 = blockIdx.x * 16 * HG, blocks = K / 32;
+    const uint8_t *wr[NW][HG], *ws[NW][HG], *xr[NT], *xsr[NT];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {          // (N is a multiple of 32)
+    for (int h = 0; h < HG; ++h) {          // (N is a multiple of 32)
         const int64_t n = n0 + 16 * h + r;
         wr[0][h] = w0 + n * K;
         ws[0][h] = sw.a + n * sw.pitch;
@@ -201,19 +207,19 @@ __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(cons
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int64_t m = 16 * t + r < M ? 16 * t + r : M - 1;
+        const int64_t m = t0 + 16 * t + r < M ? t0 + 16 * t + r : M - 1;
         xr[t] = x + m * K;
         xsr[t] = xs + m * blocks;
     }
-    ff_f32x4 acc[NW][2][NT];
+    ff_f32x4 acc[NW][HG][NT];
 #pragma unroll
     for (int i = 0; i < NW; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < HG; ++h)
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[i][h][t] = ff_f32x4{0.f, 0.f, 0.f, 0.f};
-    ff_u32x4 a[2][U][NW][2], b[2][U][NT];
-    unsigned as[2][NW][2], bs[2][NT];
+    ff_u32x4 a[2][U][NW][HG], b[2][U][NT];
+    unsigned as[2][NW][HG], bs[2][NT];
     auto fetch = [&](int s, int k0) {
         const ff_u32x4 none = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -223,14 +229,14 @@ __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(cons
 #pragma unroll
             for (int i = 0; i < NW; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) a[s][j][i][h] = in ? *reinterpret_cast<const ff_u32x4*>(wr[i][h] + k) : none;
+                for (int h = 0; h < HG; ++h) a[s][j][i][h] = in ? *reinterpret_cast<const ff_u32x4*>(wr[i][h] + k) : none;
 #pragma unroll
             for (int t = 0; t < NT; ++t) b[s][j][t] = in ? *reinterpret_cast<const ff_u32x4*>(xr[t] + k) : none;
         }
 #pragma unroll
         for (int i = 0; i < NW; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) as[s][i][h] = ff_scale_word(ws[i][h], k0 / 32, blocks);
+            for (int h = 0; h < HG; ++h) as[s][i][h] = ff_scale_word(ws[i][h], k0 / 32, blocks);
 #pragma unroll
         for (int t = 0; t < NT; ++t) bs[s][t] = ff_scale_word(xsr[t], k0 / 32, blocks);
     };
@@ -246,7 +252,7 @@ __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(cons
 #pragma unroll
                 for (int i = 0; i < NW; ++i)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < HG; ++h) {
                         const ff_bf16x8 av = ff_from_e4m3x8(a[s][j][i][h][2 * p], a[s][j][i][h][2 * p + 1], (as[s][i][h] >> sh) & 255u);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) acc[i][h][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv[t], acc[i][h][t], 0, 0, 0);
@@ -263,25 +269,25 @@ __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(cons
         if (i + 2 < o.n) fetch(0, o.at(i + 2));
         multiply(1);
     }
-    constexpr int FRAGS = NW * 2 * NT;
+    constexpr int FRAGS = NW * HG * NT;
 #pragma unroll
     for (int i = 0; i < NW; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < HG; ++h)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) part[(wave * FRAGS + (i * 2 + h) * NT + t) * 64 + lane] = acc[i][h][t];
+            for (int t = 0; t < NT; ++t) part[(wave * FRAGS + (i * HG + h) * NT + t) * 64 + lane] = acc[i][h][t];
     __syncthreads();
     for (int t = wave; t < NT; t += waves) {
-        const int m = 16 * t + r;
-        ff_f32x4 v[2];
+        const int m = t0 + 16 * t + r;
+        ff_f32x4 v[HG];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) v[h] = ff_rows_total(part, waves, FRAGS, h * NT + t, lane);
+        for (int h = 0; h < HG; ++h) v[h] = ff_rows_total(part, waves, FRAGS, h * NT + t, lane);
         if (GATED) {
             float top = 0.f;
             bool bad = false;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const ff_f32x4 u = ff_rows_total(part, waves, FRAGS, ((NW - 1) * 2 + h) * NT + t, lane);
+            for (int h = 0; h < HG; ++h) {
+                const ff_f32x4 u = ff_rows_total(part, waves, FRAGS, ((NW - 1) * HG + h) * NT + t, lane);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float ac, slope;
@@ -298,7 +304,7 @@ __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(cons
             const float inv = byte == 255u ? NAN : ff_scale_inverse(byte);
             if (m < M) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < HG; ++h)
                     *reinterpret_cast<unsigned*>(hq + (int64_t)m * N + n0 + 16 * h + 4 * q) =
                         ff_e4m3x4(v[h][0] * inv, v[h][1] * inv, v[h][2] * inv, v[h][3] * inv);
                 if (q == 0) hs[(int64_t)m * (N / 32) + blockIdx.x] = (uint8_t)byte;
@@ -306,7 +312,7 @@ __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(cons
         } else if (m < M) {
             typedef T V4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < HG; ++h)
                 *reinterpret_cast<V4*>(out + (int64_t)m * N + n0 + 16 * h + 4 * q) = V4{(T)v[h][0], (T)v[h][1], (T)v[h][2], (T)v[h][3]};
         }
     }
@@ -315,17 +321,20 @@ __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(cons
 template <int NT, bool GATED, typename T>
 void rows8(const void* w0, const void* w1, const FfScales& sw, const void* x, const uint8_t* xs, int M, int N, int K, T* out, uint8_t* hq, uint8_t* hs, int act,
            hipStream_t st) {
-    const int waves = ff_rows_waves(N / 32, (K + 127) / 128, ff_rows8_most(NT, GATED));
-    hipLaunchKernelGGL((k_ff_rows8<NT, GATED, T>), dim3(N / 32), dim3(64 * waves), (size_t)waves * (GATED ? 4 : 2) * NT * 1024, st, (const uint8_t*)w0,
-                       (const uint8_t*)w1, sw, (const uint8_t*)x, xs, M, N, K, out, hq, hs, act);
+    constexpr int ROWS = GATED ? 32 : 16;
+    const int waves = ff_rows_waves(N / ROWS, (K + 127) / 128, ff_rows8_most(NT, GATED));
+    hipLaunchKernelGGL((k_ff_rows8<NT, GATED, T>), dim3(N / ROWS, (M + 16 * NT - 1) / (16 * NT)), dim3(64 * waves), (size_t)waves * (GATED ? 4 : 1) * NT * 1024, st,
+                       (const uint8_t*)w0, (const uint8_t*)w1, sw, (const uint8_t*)x, xs, M, N, K, out, hq, hs, act);
 }
 template <bool GATED, typename T>
 void few_rows8(const void* w0, const void* w1, const FfScales& sw, const void* x, const uint8_t* xs, int M, int N, int K, T* out, uint8_t* hq, uint8_t* hs, int act,
                hipStream_t st) {
-    if (M <= 16) rows8<1, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
-    else if (M <= 32) rows8<2, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
-    else if (M <= 48) rows8<3, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
-    else rows8<4, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
+    switch (ff_rows_tokens(M, N / (GATED ? 32 : 16))) {
+        case 1: rows8<1, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st); break;
+        case 2: rows8<2, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st); break;
+        case 3: rows8<3, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st); break;
+        default: rows8<4, GATED, T>(w0, w1, sw, x, xs, M, N, K, out, hq, hs, act, st);
+    }
 }
 
 template <typename T>
@@ -371,7 +380,7 @@ struct Epi8Gate {
 
 template <int BP, int BQ, int WP, int WQ, bool GATED, bool EXACT, typename Epi>
 int launch8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const FfScales& sq, int M, int N, int K, const Epi& epi, hipStream_t st) {
-    constexpr int RING = 4 * (BP + BQ) * 64 + 4 * (BP + BQ) * 4, OUT = ff_output_bytes<BP, BQ, WP, WQ>(), LDS = RING > OUT ? RING : OUT, COLS = GATED ? BP / 2 : BP;
+    constexpr int RING = 2 * (BP + BQ) * 128 + 2 * (BP + BQ) * 4, OUT = ff_output_bytes<BP, BQ, WP, WQ>(), LDS = RING > OUT ? RING : OUT, COLS = GATED ? BP / 2 : BP;
     static bool set[NF_MAX_DEVICES];
     const int dev = nf_current_device();
     const auto kernel = k_ff_gemm8<BP, BQ, WP, WQ, GATED, EXACT, Epi>;
