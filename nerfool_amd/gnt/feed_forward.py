@@ -6,7 +6,7 @@ other layers.
     y, h = rms_norm(x, weight, residual=r)                      # h = x + r, y = weight * h / sqrt(mean(h^2) + eps)
     out = gated_feed_forward(y, w_gate, w_up, w_down)           # (act(y Wg^T) * (y Wu^T)) Wd^T
 
-Both have a backward pass (not a second one: differentiating a gradient raises).  On 8 bits, for inference:
+Both have a backward pass, and no second one: backward() and grad() with create_graph raise.  On 8 bits, for inference:
 
     q, scale, h = rms_norm_8bit(x, weight, residual=r)
     out = gated_feed_forward_8bit((q, scale), quantize_8bit(w_gate), quantize_8bit(w_up), quantize_8bit(w_down), dtype=torch.bfloat16)
@@ -19,7 +19,6 @@ current stream; results do not depend on scheduling (no atomics).  In float32 an
 would be infinite: operands are split into parts, and the parts that are zero meet the infinity."""
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -32,6 +31,11 @@ def _rows(t, name):
 
 def _as(t, shape):
     return t if t.dim() == len(shape) else t.reshape(shape)
+
+
+def _first_only():
+    if torch.is_grad_enabled():          # create_graph: the gradients would enter the new graph as constants
+        raise RuntimeError('rms_norm and gated_feed_forward have no second derivative: call backward() or grad() without create_graph')
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -50,8 +54,8 @@ class _RMSNorm(torch.autograd.Function):
         return (y, h) if h is not None else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh=None):
+        _first_only()
         h, residual, weight, rstd = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if dy is None:          # only the sum was used
@@ -103,8 +107,8 @@ class _GatedFeedForward(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_only()
         x, w_gate, w_up, w_down, g, u = ctx.saved_tensors
         return (*ops.gated_ff_bwd(x, w_gate, w_up, w_down, dy, g, u, ctx.activation, ctx.needs_input_grad[:4]), None)
 

@@ -142,3 +142,229 @@ def check_gated_8bit(rows, dim, hidden, device, act='silu', dtype=BF16, seed=0):
     eq = torch.where(unsure, 2 * step + 2.0 ** -9 * s.repeat_interleave(32, dim=1), eq)
     v, e = product8(hq, wd.t(), eq)
     near(out, (v, ref.rounded(v, e, dtype)), 'out')
+
+
+# ---- what a call may look like -----------------------------------------------------------------------------------------------------
+def check_layouts(device, dtype=BF16):
+    """leading axes, slices, transposed and misaligned tensors give what the plain layout gives"""
+    gen = torch.Generator().manual_seed(5)
+    dim, hid = 48, 80
+    base = normal(gen, 6, 7, dim, dtype=dtype, device=device)
+    ws = [normal(gen, *s, dtype=dtype, device=device, scale=0.2) for s in ((hid, dim), (hid, dim), (dim, hid))]
+    want = ff.gated_feed_forward(base.reshape(-1, dim).contiguous(), *ws)
+    wide = torch.zeros(6, 7, dim + 5, dtype=dtype, device=device)
+    wide[..., 3:3 + dim] = base
+    flat = torch.zeros(6 * 7 * dim + 1, dtype=dtype, device=device)
+    flat[1:] = base.reshape(-1)
+    for x in (base, wide[..., 3:3 + dim], base.transpose(0, 1).contiguous().transpose(0, 1), flat[1:].view(6, 7, dim)):
+        assert torch.equal(ff.gated_feed_forward(x, *ws), want.view(6, 7, dim))
+        assert torch.equal(ff.gated_feed_forward(x, ws[0].t().contiguous().t(), ws[1], ws[2]), want.view(6, 7, dim))
+    assert torch.equal(ff.gated_feed_forward(base[0, 0], *ws), want[0])
+    w = normal(gen, dim, dtype=dtype, device=device)
+    y, h = ff.rms_norm(base.reshape(-1, dim), w, wide[..., :dim].reshape(-1, dim))
+    y2, h2 = ff.rms_norm(flat[1:].view(6, 7, dim), w, wide[..., :dim])
+    assert torch.equal(y2.reshape(-1, dim), y) and torch.equal(h2.reshape(-1, dim), h)
+    q, s = ff.quantize_8bit(base)
+    q2, s2 = ff.quantize_8bit(wide[..., 3:3 + dim])
+    assert q.shape == base.shape and s.shape == (6, 7, 2)
+    assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s.view(torch.uint8), s2.view(torch.uint8))
+    # 8-bit pairs: leading axes, and values and scales that are slices
+    dim, hid = 64, 96
+    x, wg, wu, wd = (ff.quantize_8bit(normal(gen, *shape, device=device, scale=0.3)) for shape in ((6, 7, dim), (hid, dim), (hid, dim), (dim, hid)))
+    want = ff.gated_feed_forward_8bit(x, wg, wu, wd)
+    assert want.shape == (6, 7, dim) and want.dtype == BF16
+    flat = torch.zeros(42 * dim + 3, dtype=torch.uint8, device=device)
+    flat[3:] = x[0].view(torch.uint8).reshape(-1)
+    fs = torch.zeros(42 * 2 + 1, dtype=torch.uint8, device=device)
+    fs[1:] = x[1].view(torch.uint8).reshape(-1)
+    moved = (flat[3:].view(6, 7, dim).view(torch.float8_e4m3fn), fs[1:].view(6, 7, 2).view(torch.float8_e8m0fnu))
+    assert torch.equal(ff.gated_feed_forward_8bit(moved, wg, wu, wd), want)
+
+
+def check_empty(device):
+    """no rows: empty results, zero gradients of the weights"""
+    x = torch.zeros(0, 40, device=device, requires_grad=True)
+    w = torch.ones(40, device=device, requires_grad=True)
+    y, h = ff.rms_norm(x, w, torch.zeros(0, 40, device=device))
+    gx, gw = torch.autograd.grad(y.sum() + h.sum(), (x, w))
+    assert y.shape == h.shape == gx.shape == (0, 40) and torch.equal(gw, torch.zeros_like(w))
+    ws = [torch.ones(s, device=device, requires_grad=True) for s in ((24, 40), (24, 40), (40, 24))]
+    out = ff.gated_feed_forward(x, *ws)
+    grads = torch.autograd.grad(out.sum(), (x, *ws))
+    assert out.shape == (0, 40) and all(torch.equal(g, torch.zeros_like(t)) for g, t in zip(grads, (x, *ws)))
+    q, s = ff.quantize_8bit(torch.zeros(0, 64, device=device))
+    assert q.shape == (0, 64) and s.shape == (0, 2)
+    pairs = [ff.quantize_8bit(torch.ones(*shape, device=device)) for shape in ((32, 64), (32, 64), (64, 32))]
+    assert ff.gated_feed_forward_8bit((q, s), *pairs, dtype=F32).shape == (0, 64)
+
+
+def check_not_finite(device, rows=70, dtype=BF16):
+    """an infinity or a NaN stays in its row (in 8 bits: in its block of 32 values); others are as without it"""
+    gen = torch.Generator().manual_seed(7)
+    dim, hid = 96, 64
+    x = normal(gen, rows, dim, dtype=dtype, device=device)
+    ws = [normal(gen, *s, dtype=dtype, device=device, scale=0.2) for s in ((hid, dim), (hid, dim), (dim, hid))]
+    bad = x.clone()
+    bad[3, 5], bad[9, 40], bad[11, 95] = float('nan'), float('inf'), -float('inf')
+    rest = torch.ones(rows, dtype=torch.bool, device=device)
+    rest[[3, 9, 11]] = False
+    for f in (lambda t: ff.gated_feed_forward(t, *ws), lambda t: ff.rms_norm(t)):
+        got, want = f(bad), f(x)
+        assert torch.equal(got[rest], want[rest]) and not torch.isfinite(got[3]).any()
+    (q, s), (q0, s0) = ff.quantize_8bit(bad), ff.quantize_8bit(x)
+    byte, byte0 = s.view(torch.uint8), s0.view(torch.uint8)
+    marked = torch.zeros_like(byte, dtype=torch.bool)
+    marked[3, 0] = marked[9, 1] = marked[11, 2] = True
+    assert (byte[marked] == 255).all() and torch.equal(byte[~marked], byte0[~marked])
+    wide = marked.repeat_interleave(32, dim=1)
+    assert torch.isnan(q.float()[wide]).all() and torch.equal(q.float()[~wide], q0.float()[~wide])
+    pairs = [ff.quantize_8bit(w.float()) for w in ws]
+    for out in (BF16, F32):
+        got, want = (ff.gated_feed_forward_8bit(t, *pairs, dtype=out) for t in ((q, s), (q0, s0)))
+        assert torch.isnan(got[~rest].float()).all() and torch.equal(got[rest], want[rest])
+
+
+def check_extreme_8bit(device):
+    """zeros, subnormal values, the largest float, and blocks at the border of a scale"""
+    rows = [torch.zeros(32), torch.full((32,), 2.0 ** -149), torch.full((32,), 2.0 ** -130), torch.full((32,), torch.finfo(F32).max),
+            torch.full((32,), 448.0), torch.full((32,), 448.0 * (1 + 2.0 ** -23)), torch.full((32,), -448.0 * 2.0 ** 50), torch.arange(32) * 2.0 ** -100]
+    x = torch.stack(rows).to(device)
+    q, s = ff.quantize_8bit(x)
+    vq, vs = ref.to_8bit(x.double())
+    assert torch.equal(torch.exp2(s.view(torch.uint8).double() - 127), vs) and torch.equal(q.double(), vq)
+    assert s.view(torch.uint8)[:2].flatten().tolist() == [0, 0]
+
+
+def check_differences(device):
+    """the gradient along a direction against central differences of the float32 forward.  Values and weights are O(1), sums of 24 to 40 terms: a step of 2^-7 leaves
+    a third-order term below 2^-14 of the derivative's scale, and float32's 2^-22 of the sum over 2^-6 leaves 2^-16"""
+    gen = torch.Generator().manual_seed(11)
+    x = normal(gen, 5, 24, device=device)
+    r = normal(gen, 5, 24, device=device)
+    ws = [normal(gen, *s, device=device, scale=0.3) for s in ((40, 24), (40, 24), (24, 40))]
+    wn = 1 + 0.1 * normal(gen, 24, device=device)
+    c, ch = normal(gen, 5, 24, device=device), normal(gen, 5, 24, device=device)
+
+    def value(x, r, wn, *ws):
+        y, h = ff.rms_norm(x, wn, r)
+        return (ff.gated_feed_forward(y, *ws, activation='gelu').double() * c).sum() + (h.double() * ch).sum()
+
+    leaves = [t.requires_grad_(True) for t in (x, r, wn, *ws)]
+    grads = torch.autograd.grad(value(*leaves), leaves)
+    for i, (leaf, grad) in enumerate(zip(leaves, grads)):
+        v = torch.randn(leaf.shape, generator=gen).sign().to(device)
+        step = 2.0 ** -7
+        moved = [[t.detach() + (step * k * v if j == i else 0) for j, t in enumerate(leaves)] for k in (1, -1)]
+        with torch.no_grad():
+            slope = (value(*moved[0]) - value(*moved[1])) / (2 * step)
+        along = (grad.double() * v).sum()
+        assert abs(slope - along) <= 2.0 ** -10 * grad.double().abs().sum(), (i, float(slope), float(along))
+
+
+def check_layer(device, dtype=BF16):
+    """a layer's feed-forward half as it is used: norm with the residual's addition, gated block, addition; twice, so that the stream's gradient comes from both; in the
+    modules' own types.  Bounds: each of the 2 x 3 roundings to `dtype` on the way moves a value by half a step of values up to the stream's largest; 16 of them for forward
+    and backward, which are as long again"""
+    gen = torch.Generator().manual_seed(13)
+    dim, hid = 64, 160
+    torch.manual_seed(3)
+    norms = [ff.RMSNorm(dim).to(device).to(dtype) for _ in range(2)]
+    blocks = [ff.GatedFeedForward(dim, hid, 'gelu').to(device).to(dtype) for _ in range(2)]
+    assert [n for n, _ in blocks[0].named_parameters()] == ['gate.weight', 'up.weight', 'down.weight']
+    x, r = (normal(gen, 3, 11, dim, dtype=dtype, device=device).requires_grad_(True) for _ in range(2))
+    dy = normal(gen, 3, 11, dim, dtype=dtype, device=device)
+
+    def run(x, r, norm, block, n, b):
+        stream, add = x, r
+        for i in range(2):
+            y, stream = norm(stream, add, n[i])
+            add = block(y, b[i])
+        return stream + add
+
+    out = run(x, r, lambda x, r, m: m(x, r), lambda y, m: m(y), norms, blocks)
+    params = [p for m in (*norms, *blocks) for p in m.parameters()]
+    grads = torch.autograd.grad(out, [x, r, *params], dy)
+
+    xs = [t.detach().double().requires_grad_(True) for t in (x, r)]
+    ps = [p.detach().double().requires_grad_(True) for p in params]
+
+    def norm64(x, r, w):
+        h = x + r
+        return h * w / torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-6), h
+
+    def block64(y, w):
+        return ((lambda g: ref.act('gelu', g)[0])(y @ w[0].t()) * (y @ w[1].t())) @ w[2].t()
+
+    want = run(*xs, norm64, block64, ps[:2], [ps[2:5], ps[5:8]])
+    wants = torch.autograd.grad(want, [*xs, *ps], dy.double())
+    for a, b in zip((out.detach(), *grads), (want.detach(), *wants)):
+        scale = max(float(b.abs().max()), 1e-30)
+        assert float((a.double() - b).abs().max()) <= 16 * ref.half_step(dtype) * scale
+    assert torch.equal(grads[0], grads[1])          # x and the residual enter as a sum
+
+
+def check_layer_8bit(device):
+    """norm -> 8 bits -> gated block, from the same parts one by one"""
+    gen = torch.Generator().manual_seed(17)
+    dim, hid = 96, 160
+    x, r = normal(gen, 20, dim, dtype=BF16, device=device), normal(gen, 20, dim, dtype=BF16, device=device)
+    w = (1 + 0.1 * torch.randn(dim, generator=gen)).to(BF16).to(device)
+    pairs = [ff.quantize_8bit(normal(gen, *s, device=device, scale=s[1] ** -0.5)) for s in ((hid, dim), (hid, dim), (dim, hid))]
+    q, s, h = ff.rms_norm_8bit(x, w, r)
+    out = ff.gated_feed_forward_8bit((q, s), *pairs, dtype=F32)
+    v, (wg, wu, wd) = value_of(q, s), (value_of(*p) for p in pairs)
+    hq, hs = ref.to_8bit(ref.act('silu', v @ wg.t())[0] * (v @ wu.t()))
+    want = (hq * hs.repeat_interleave(32, dim=1)) @ wd.t()
+    # a value of the middle that lies next to a border of the grid may take the neighbouring step: 2^-3 of it, for at most one in 32 (seen: none)
+    assert float((out.double() - want).norm() / want.norm()) <= 2.0 ** -3 / 32 ** 0.5
+    y, h2 = ff.rms_norm(x, w, r)
+    assert torch.equal(h, h2)
+    assert float((value_of(q, s) - y.double()).abs().max() / y.double().abs().max()) <= 2.0 ** -4 + 2.0 ** -8
+
+
+def check_guards(device, rows, dim, hidden, dtype):
+    """the entry points write their outputs and nothing behind them"""
+    from nerfool_amd import _lib
+    L = _lib.lib()
+    gen = torch.Generator().manual_seed(19)
+    code = {F32: 0, BF16: 1, F16: 2}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream if device != 'cpu' else 0
+    guard = 256
+
+    def out(n, t=dtype):
+        return torch.full((n + guard,), 7.0, dtype=t, device=device) if t != torch.uint8 else torch.full((n + guard,), 77, dtype=t, device=device)
+
+    def intact(*ts):
+        for t, n in ts:
+            tail = t[n:]
+            assert (tail == (77 if t.dtype == torch.uint8 else 7.0)).all()
+
+    x, r, dy = (normal(gen, rows, dim, dtype=dtype, device=device) for _ in range(3))
+    ws = [normal(gen, *s, dtype=dtype, device=device, scale=0.2) for s in ((hidden, dim), (hidden, dim), (dim, hidden))]
+    n, f, w = rows * dim, rows * hidden, dim * hidden
+    y, g, u = out(n), out(f, F32), out(f, F32)
+    need = L.nf_gated_ff_fwd_workspace_bytes(rows, dim, hidden, code)
+    ws_bytes = out(need, torch.uint8)
+    p = lambda t: None if t is None else t.data_ptr()          # noqa: E731
+    _lib.check(L.nf_gated_ff_fwd(p(x), *[p(t) for t in ws], rows, dim, hidden, code, 0, p(y), p(g), p(u), p(ws_bytes), stream), 'fwd')
+    intact((y, n), (g, f), (u, f), (ws_bytes, need))
+    need = L.nf_gated_ff_bwd_workspace_bytes(rows, dim, hidden, code, 1, 1, 1)
+    ws_bytes = out(need, torch.uint8)
+    grads = [out(n), out(w), out(w), out(w)]
+    _lib.check(L.nf_gated_ff_bwd(p(x), *[p(t) for t in ws], p(dy), p(g), p(u), rows, dim, hidden, code, 0, *[p(t) for t in grads], p(ws_bytes), stream), 'bwd')
+    intact((ws_bytes, need), (grads[0], n), *[(t, w) for t in grads[1:]])
+    want = ref.gated(x, *ws, 'silu', dy, dtype)
+    for t, key, shape in zip((y, *grads), ('out', 'dx', 'dw_gate', 'dw_up', 'dw_down'), ((rows, dim), (rows, dim), (hidden, dim), (hidden, dim), (dim, hidden))):
+        near(t[:t.numel() - guard].view(shape), want[key], key)
+    # one of the two gradients that share a product, and no other
+    ws_bytes = out(L.nf_gated_ff_bwd_workspace_bytes(rows, dim, hidden, code, 0, 1, 0), torch.uint8)
+    one = out(w)
+    _lib.check(L.nf_gated_ff_bwd(p(x), *[p(t) for t in ws], p(dy), p(g), p(u), rows, dim, hidden, code, 0, None, None, p(one), None, p(ws_bytes), stream), 'bwd')
+    assert torch.equal(one, grads[2])
+    h, y, rstd, blocks = out(n), out(n), out(rows, F32), (dim + 31) // 32
+    _lib.check(L.nf_rms_norm_fwd(p(x), p(r), None, rows, dim, code, 1e-6, p(h), p(y), None, None, p(rstd), stream), 'norm')
+    q, s = out(n, torch.uint8), out(rows * blocks, torch.uint8)
+    _lib.check(L.nf_rms_norm_fwd(p(x), p(r), None, rows, dim, code, 1e-6, p(h), None, p(q), p(s), None, stream), 'norm')
+    dx, dw, part = out(n), out(dim), out(L.nf_rms_norm_bwd_workspace_floats(dim), F32)
+    _lib.check(L.nf_rms_norm_bwd(p(dy), None, p(h), None, None, p(rstd), rows, dim, code, p(dx), p(dw), p(part), stream), 'norm bwd')
+    intact((h, n), (y, n), (rstd, rows), (q, n), (s, rows * blocks), (dx, n), (dw, dim), (part, part.numel() - guard))
