@@ -438,7 +438,8 @@ int nf_in_act_pad_bwd(const float* dy_padded, const float* d_extra, const float*
  *
  * nf_gated_ff_fwd: out [rows, dim] = (act(x Wg^T) * (x Wu^T)) Wd^T; Wg, Wu [hidden, dim], Wd [dim, hidden].  g_save, u_save (nullable, together):
  *   x Wg^T and x Wu^T in float, [rows, hidden], for the backward pass.  Operand pointers must be 16-byte aligned.
- * nf_gated_ff_bwd: the gradients that are not NULL of dx [rows, dim], dw_gate, dw_up [hidden, dim], dw_down [dim, hidden] from dy, g, u.
+ * nf_gated_ff_bwd: the gradients that are not NULL of dx [rows, dim], dw_gate, dw_up [hidden, dim], dw_down [dim, hidden] from dy, g, u.  Where
+ *   nf_gated_ff_bwd_recomputes(rows, dim, hidden) is not 0 and dx alone is asked for, g and u are made again and may be NULL.
  * nf_gated_ff_fwd_8bit: the block on operands in the 8-bit form above (dim, hidden multiples of 32; scales [rows of the operand, k / 32] bytes); h in
  *   the middle is brought to that form from its float values; out in out_dtype.
  * workspace: as many bytes as the *_workspace_bytes call of the same sizes says (-1: sizes out of range), 256-byte aligned.
@@ -452,6 +453,7 @@ int nf_quantize_8bit(const void* x, int64_t rows, int dim, int dtype, uint8_t* q
 int64_t nf_gated_ff_fwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype);
 int nf_gated_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, int64_t rows, int dim, int hidden, int dtype,
                     int activation, void* out, float* g_save, float* u_save, void* workspace, nf_stream_t stream);
+int nf_gated_ff_bwd_recomputes(int64_t rows, int dim, int hidden);
 int64_t nf_gated_ff_bwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, int want_dx, int want_dw_gate_up, int want_dw_down);
 int nf_gated_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* dy, const float* g, const float* u,
                     int64_t rows, int dim, int hidden, int dtype, int activation, void* dx, void* dw_gate, void* dw_up, void* dw_down,

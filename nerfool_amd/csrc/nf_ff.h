@@ -144,3 +144,28 @@ __device__ __forceinline__ void ff_act(int act, float g, float& a, float& slope)
         slope = g > 0.f ? 1.f : 0.f;
     }
 }
+
+// ---- stores of 4 consecutive values of a row (`left`: how many the row still has)
+template <typename T>
+__device__ __forceinline__ void ff_put(T* p, int left, const ff_f32x4& v) {
+    if (left >= 4) {
+        typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        *reinterpret_cast<V4*>(p) = V4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    } else {
+        for (int c = 0; c < left; ++c) p[c] = (T)v[c];
+    }
+}
+// the three bf16 parts of 4 floats.  The first is cut off, not rounded: near the largest float the rounded part would be infinite; the others are
+// rounded, which makes the third exact.  An infinity or a NaN keeps its value in the first part and zeros in the others.
+__device__ __forceinline__ void ff_split3(float v, ff_bf16* part) {
+    const unsigned u = __float_as_uint(v);
+    float hi = (float)(ff_bf16)v;
+    if (!(fabsf(hi) <= 3.4028235e38f)) hi = __uint_as_float(u & 0xffff0000u);
+    if (v != v) hi = v;
+    float rest = v - hi;
+    if (!(fabsf(v) <= 3.4028235e38f)) rest = 0.f;
+    const float mid = (float)(ff_bf16)rest;
+    part[0] = (ff_bf16)hi;
+    part[1] = (ff_bf16)mid;
+    part[2] = (ff_bf16)(rest - mid);
+}

@@ -11,32 +11,14 @@
 #include "nf_ff_gemm.h"
 #include "nf_ff_rows.h"
 
+// nf_gated_ff_narrow.hip
+bool ff_narrow_fits(int64_t rows, int dim, int hidden);
+int64_t ff_narrow_workspace_bytes(int dim, int hidden, int dtype, bool backward);
+int ff_narrow(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, int64_t rows, int dim, int hidden, int dtype, int act, void* out, void* workspace,
+              hipStream_t st);
+
 namespace {
 
-// ---- stores of 4 consecutive values of a row (`left`: how many the row still has); pitch and address allow one store where `wide`
-template <typename T>
-__device__ __forceinline__ void ff_put(T* p, int left, const ff_f32x4& v) {
-    if (left >= 4) {
-        typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-        *reinterpret_cast<V4*>(p) = V4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-    } else {
-        for (int c = 0; c < left; ++c) p[c] = (T)v[c];
-    }
-}
-// the three bf16 parts of 4 floats.  The first is cut off, not rounded: near the largest float the rounded part would be infinite; the others are
-// rounded, which makes the third exact.  An infinity or a NaN keeps its value in the first part and zeros in the others.
-__device__ __forceinline__ void ff_split3(float v, ff_bf16* part) {
-    const unsigned u = __float_as_uint(v);
-    float hi = (float)(ff_bf16)v;
-    if (!(fabsf(hi) <= 3.4028235e38f)) hi = __uint_as_float(u & 0xffff0000u);
-    if (v != v) hi = v;
-    float rest = v - hi;
-    if (!(fabsf(v) <= 3.4028235e38f)) rest = 0.f;
-    const float mid = (float)(ff_bf16)rest;
-    part[0] = (ff_bf16)hi;
-    part[1] = (ff_bf16)mid;
-    part[2] = (ff_bf16)(rest - mid);
-}
 __device__ __forceinline__ void ff_put3(ff_bf16* p, int64_t plane, int left, const ff_f32x4& v) {
     ff_bf16 t[4][3];
 #pragma unroll
@@ -516,22 +498,31 @@ bool ff_sizes_ok(const char* what, int64_t M, int D, int F, int dtype, int act) 
 extern "C" int64_t nf_gated_ff_fwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype) {
     if (!ff_sizes_ok("nf_gated_ff_fwd_workspace_bytes", rows, dim, hidden, dtype, 0)) return -1;
     if (rows <= FF_ROWS_MAX) return rows * hidden * (dtype == FF_F32 ? 4 : 2);          // h
-    if (dtype == FF_F32) return FwdPlan<float>(nullptr, rows, dim, hidden).bytes;
-    return FwdPlan<ff_bf16>(nullptr, rows, dim, hidden).bytes;
+    const int64_t n = dtype == FF_F32 ? FwdPlan<float>(nullptr, rows, dim, hidden).bytes : FwdPlan<ff_bf16>(nullptr, rows, dim, hidden).bytes;
+    const int64_t narrow = ff_narrow_fits(rows, dim, hidden) ? ff_narrow_workspace_bytes(dim, hidden, dtype, false) : 0;
+    return n > narrow ? n : narrow;          // (which of the two runs depends on whether g and u are saved)
 }
 
 extern "C" int nf_gated_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, int64_t rows, int dim, int hidden, int dtype,
                                int activation, void* out, float* g_save, float* u_save, void* workspace, nf_stream_t stream) {
     if (!ff_sizes_ok("nf_gated_ff_fwd", rows, dim, hidden, dtype, activation)) return 1;
     NF_REQUIRE((g_save != nullptr) == (u_save != nullptr), "nf_gated_ff_fwd: g_save and u_save go together");
+    if (rows > FF_ROWS_MAX && !g_save && ff_narrow_fits(rows, dim, hidden)) {
+        FF_TRY(ff_narrow(x, w_gate, w_up, w_down, nullptr, rows, dim, hidden, dtype, activation, out, workspace, (hipStream_t)stream));
+        NF_LAUNCH_CHECK("nf_gated_ff_fwd");
+        return 0;
+    }
     const auto f = dtype == FF_F32 ? ff_fwd<float> : dtype == FF_BF16 ? ff_fwd<ff_bf16> : ff_fwd<ff_half>;
     FF_TRY(f(x, w_gate, w_up, w_down, (int)rows, dim, hidden, activation, out, g_save, u_save, workspace, (hipStream_t)stream));
     NF_LAUNCH_CHECK("nf_gated_ff_fwd");
     return 0;
 }
 
+extern "C" int nf_gated_ff_bwd_recomputes(int64_t rows, int dim, int hidden) { return ff_narrow_fits(rows, dim, hidden); }
+
 extern "C" int64_t nf_gated_ff_bwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, int want_dx, int want_dw_gate_up, int want_dw_down) {
     if (!ff_sizes_ok("nf_gated_ff_bwd_workspace_bytes", rows, dim, hidden, dtype, 0)) return -1;
+    if (want_dx && !want_dw_gate_up && !want_dw_down && ff_narrow_fits(rows, dim, hidden)) return ff_narrow_workspace_bytes(dim, hidden, dtype, true);
     if (dtype == FF_F32) return BwdPlan<float>(nullptr, rows, dim, hidden, want_dx, want_dw_gate_up, want_dw_down).bytes;
     return BwdPlan<ff_bf16>(nullptr, rows, dim, hidden, want_dx, want_dw_gate_up, want_dw_down).bytes;
 }
@@ -540,6 +531,12 @@ extern "C" int nf_gated_ff_bwd(const void* x, const void* w_gate, const void* w_
                                int64_t rows, int dim, int hidden, int dtype, int activation, void* dx, void* dw_gate, void* dw_up, void* dw_down,
                                void* workspace, nf_stream_t stream) {
     if (!ff_sizes_ok("nf_gated_ff_bwd", rows, dim, hidden, dtype, activation)) return 1;
+    if (dx && !dw_gate && !dw_up && !dw_down && ff_narrow_fits(rows, dim, hidden)) {
+        FF_TRY(ff_narrow(x, w_gate, w_up, w_down, dy, rows, dim, hidden, dtype, activation, dx, workspace, (hipStream_t)stream));
+        NF_LAUNCH_CHECK("nf_gated_ff_bwd");
+        return 0;
+    }
+    NF_REQUIRE(g && u, "nf_gated_ff_bwd: these sizes and gradients need the forward's g and u");
     const auto f = dtype == FF_F32 ? ff_bwd<float> : dtype == FF_BF16 ? ff_bwd<ff_bf16> : ff_bwd<ff_half>;
     FF_TRY(f(x, w_gate, w_up, w_down, dy, g, u, (int)rows, dim, hidden, activation, dx, dw_gate, dw_up, dw_down, workspace, (hipStream_t)stream));
     NF_LAUNCH_CHECK("nf_gated_ff_bwd");

@@ -1,0 +1,232 @@
+// The gated feed-forward block at the widths of the ray transformer (dim <= 64: gnt/transformer_network.py:38-50 has 64 and 256) in one kernel a direction: what the block
+// computes between its input and its output never leaves the registers.
+//
+// A wave owns 32 tokens.  The features are walked in chunks of 32: g and u of the chunk are made as 16 x 16 blocks (weights the A operand, tokens the B operand, so that a
+// lane holds 4 consecutive features of one token), h of the chunk goes back into B operands as it lies -- the lane's 4 features of the first block are its k 0 .. 3 and those of
+// the second its k 4 .. 7; the down projection's records have their features in that order -- and out grows by the chunk's share.  The backward pass to x alone (constant
+// weights, as in an attack) makes g and u again instead of reading them: dx += dg Wg + du Wu the same way, with dh = dy Wd of the chunk between.
+// The weights come as records of operand fragments (k_ff_narrow_pack, per call), 1 KB each, by LDS-DMA, one chunk ahead, for the four waves of a workgroup.  float32: three bf16
+// parts of every operand, six products (nf_gated_ff.hip); h, dg and du are then split, not rounded.  Bound by the matrix instructions and, as much, by the vector
+// instructions of activation and split between them: 32768 x 64 x 256 float32 takes TODO us forward and TODO us backward (in separate products: 69 and 80).
+#include "nf_ff_gemm.h"
+
+namespace {
+
+// ---- records.  A chunk's fragments, KD = padded dim / 32:  gate [2][KD], up [2][KD]; forward: down [2 KD]; backward: down transposed [2][KD], gate and up transposed [2 KD] each
+constexpr int narrow_records(int kd, bool backward) { return (backward ? 10 : 6) * kd; }
+
+template <typename T>
+struct NarrowParts {
+    typedef T E;
+    static constexpr int NP = 1;
+    static __device__ __forceinline__ void split(float v, E* p) { p[0] = (E)v; }
+};
+template <>
+struct NarrowParts<float> {
+    typedef ff_bf16 E;
+    static constexpr int NP = 3;
+    static __device__ __forceinline__ void split(float v, E* p) { ff_split3(v, p); }
+};
+
+// one wave a record: lane l holds row l mod 16, k = 8 (l / 16) + j, j = 0 .. 7 -> [chunk][record][part][lane][8]
+template <typename T>
+__global__ void __launch_bounds__(256) k_ff_narrow_pack(const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ wd, int D, int F, int kd, int backward,
+                                                        typename NarrowParts<T>::E* __restrict__ out) {
+    typedef NarrowParts<T> P;
+    const int per = narrow_records(kd, backward), chunks = (F + 31) / 32;
+    const int rec = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, row = lane & 15, q = lane >> 4;
+    if (rec >= per * chunks) return;
+    const int chunk = rec / per, n = rec - chunk * per;
+    typename P::E part[8][P::NP];
+    for (int j = 0; j < 8; ++j) {
+        const int k = 8 * q + j, f_of_k = 32 * chunk + (j < 4 ? 4 * q + j : 16 + 4 * q + j - 4);
+        float v = 0.f;
+        if (n < 4 * kd) {                       // gate, up: rows are features, k is dim
+            const int i = n % (2 * kd), f = 32 * chunk + 16 * (i / kd) + row, d = 32 * (i % kd) + k;
+            if (f < F && d < D) v = (float)(n < 2 * kd ? wg : wu)[(int64_t)f * D + d];
+        } else if (!backward) {                 // down: rows are dim, k is features
+            const int d = 16 * (n - 4 * kd) + row;
+            if (d < D && f_of_k < F) v = (float)wd[(int64_t)d * F + f_of_k];
+        } else if (n < 6 * kd) {                // down transposed: rows are features, k is dim
+            const int i = n - 4 * kd, f = 32 * chunk + 16 * (i / kd) + row, d = 32 * (i % kd) + k;
+            if (f < F && d < D) v = (float)wd[(int64_t)d * F + f];
+        } else {                                // gate, up transposed: rows are dim, k is features
+            const int i = n - 6 * kd, d = 16 * (i % (2 * kd)) + row;
+            if (d < D && f_of_k < F) v = (float)(i < 2 * kd ? wg : wu)[(int64_t)f_of_k * D + d];
+        }
+        P::split(v, part[j]);
+    }
+    for (int e = 0; e < P::NP; ++e) {
+        typename P::E* o = out + ((int64_t)(rec * P::NP + e) * 64 + lane) * 8;
+        for (int j = 0; j < 8; ++j) o[j] = part[j][e];
+    }
+}
+
+template <typename T, int KD, bool BWD>
+struct Narrow {
+    typedef NarrowParts<T> P;
+    typedef typename P::E E;
+    typedef FfMfma<E> Mfma;
+    typedef typename Mfma::V V;
+    static constexpr int NP = P::NP, RECORDS = narrow_records(KD, BWD), PIECES = RECORDS * NP, CHUNK = PIECES * 1024;
+
+    // this lane's 8 values of a token's row as an operand: k = 32 kd + 8 (l / 16) ..
+    static __device__ __forceinline__ void row(const T* x, int64_t m, int64_t M, int D, int k, V (&v)[NP]) {
+        float f[8];
+        const T* r = x + (m < M ? m : M - 1) * D;
+        constexpr int N = FfVec<T>::N;
+#pragma unroll
+        for (int c = 0; c < 8; c += N) {
+            float t[N];
+            ff_load_row(r, k + c, D, t);
+#pragma unroll
+            for (int j = 0; j < N; ++j) f[c + j] = t[j];
+        }
+        operand(f, v);
+    }
+    static __device__ __forceinline__ void operand(const float (&f)[8], V (&v)[NP]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            E p[NP];
+            P::split(f[j], p);
+#pragma unroll
+            for (int e = 0; e < NP; ++e) v[e][j] = p[e];
+        }
+    }
+    // acc[tt] += record n x b[tt], smallest products first
+    static __device__ __forceinline__ void multiply(const char* lds, int n, int lane, const V (&b0)[NP], const V (&b1)[NP], ff_f32x4& c0, ff_f32x4& c1) {
+        V a[NP];
+#pragma unroll
+        for (int e = 0; e < NP; ++e) a[e] = *reinterpret_cast<const V*>(lds + (n * NP + e) * 1024 + lane * 16);
+#pragma unroll
+        for (int o = NP - 1; o >= 0; --o)
+#pragma unroll
+            for (int e = 0; e <= o; ++e) {
+                c0 = Mfma::mul(a[e], b0[o - e], c0);
+                c1 = Mfma::mul(a[e], b1[o - e], c1);
+            }
+    }
+};
+
+template <typename T, int KD, bool BWD>
+__global__ void __launch_bounds__(256) k_ff_narrow(const T* __restrict__ x, const T* __restrict__ dy, const char* __restrict__ records, int64_t M, int D, int chunks, int act,
+                                                   T* __restrict__ out) {
+    typedef Narrow<T, KD, BWD> N;
+    typedef typename N::V V;
+    constexpr int NP = N::NP;
+    constexpr bool FAST = sizeof(T) == 2;
+    HIP_DYNAMIC_SHARED(char, lds)
+    const int lane = threadIdx.x & 63, wave = ff_wave_index(), q = lane >> 4;
+    const int64_t m0 = (int64_t)blockIdx.x * 128 + wave * 32 + (lane & 15);          // this lane's tokens: m0, m0 + 16
+    auto load_chunk = [&](int c) {
+        const char* src = records + (int64_t)c * N::CHUNK;
+        for (int p = wave; p < N::PIECES; p += 4) ff_dma16(src + p * 1024, (unsigned)lane * 16, lds, (c & 1) * N::CHUNK + p * 1024, lane);
+    };
+    load_chunk(0);
+    V xb[KD][2][NP], yb[BWD ? KD : 1][2][NP];
+#pragma unroll
+    for (int k = 0; k < KD; ++k)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            N::row(x, m0 + 16 * t, M, D, 32 * k + 8 * q, xb[k][t]);
+            if (BWD) N::row(dy, m0 + 16 * t, M, D, 32 * k + 8 * q, yb[BWD ? k : 0][t]);
+        }
+    const ff_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    ff_f32x4 sum[2 * KD][2];
+#pragma unroll
+    for (int i = 0; i < 2 * KD; ++i) sum[i][0] = sum[i][1] = zero;
+    for (int c = 0; c < chunks; ++c) {
+        ff_dma_barrier<0>();          // the chunk has landed for every wave, and the other buffer has been read by every wave
+        if (c + 1 < chunks) load_chunk(c + 1);
+        const char* w = lds + (c & 1) * N::CHUNK;
+        ff_f32x4 g[2][2], u[2][2], dh[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            g[i][0] = g[i][1] = u[i][0] = u[i][1] = dh[i][0] = dh[i][1] = zero;
+#pragma unroll
+            for (int k = 0; k < KD; ++k) {
+                N::multiply(w, i * KD + k, lane, xb[k][0], xb[k][1], g[i][0], g[i][1]);
+                N::multiply(w, (2 + i) * KD + k, lane, xb[k][0], xb[k][1], u[i][0], u[i][1]);
+                if (BWD) N::multiply(w, (4 + i) * KD + k, lane, yb[BWD ? k : 0][0], yb[BWD ? k : 0][1], dh[i][0], dh[i][1]);
+            }
+        }
+        V hb[2][NP], ub[2][NP];          // forward: h; backward: dg and du
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float v[8], w2[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float gv = g[j / 4][t][j % 4], uv = u[j / 4][t][j % 4];
+                float a, slope;
+                ff_act<FAST>(act, gv, a, slope);
+                if (BWD) {
+                    const float d = dh[j / 4][t][j % 4];
+                    v[j] = d * uv * slope;
+                    w2[j] = d * a;
+                } else
+                    v[j] = a * uv;
+            }
+            N::operand(v, hb[t]);
+            if (BWD) N::operand(w2, ub[t]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * KD; ++i) {
+            if (BWD) {
+                N::multiply(w, 6 * KD + i, lane, hb[0], hb[1], sum[i][0], sum[i][1]);
+                N::multiply(w, 8 * KD + i, lane, ub[0], ub[1], sum[i][0], sum[i][1]);
+            } else
+                N::multiply(w, 4 * KD + i, lane, hb[0], hb[1], sum[i][0], sum[i][1]);
+        }
+    }
+    ff_dma_barrier<0>();          // no load may land in LDS that the workgroup has given back
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int64_t m = m0 + 16 * t;
+        if (m >= M) continue;
+#pragma unroll
+        for (int i = 0; i < 2 * KD; ++i) ff_put(out + m * D + 16 * i + 4 * q, D - (16 * i + 4 * q), sum[i][t]);
+    }
+}
+
+template <typename T, int KD, bool BWD>
+int narrow_run(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, int64_t M, int D, int F, int act, void* out, void* workspace, hipStream_t st) {
+    typedef Narrow<T, KD, BWD> N;
+    constexpr int LDS = 2 * N::CHUNK;
+    static bool set[NF_MAX_DEVICES];
+    const int dev = nf_current_device();
+    if (!set[dev]) {
+        const hipError_t e = hipFuncSetAttribute((const void*)k_ff_narrow<T, KD, BWD>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) {
+            nf_set_error("gated feed-forward: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
+            return 2;
+        }
+        set[dev] = true;
+    }
+    const int chunks = (F + 31) / 32, records = N::RECORDS * chunks;
+    hipLaunchKernelGGL((k_ff_narrow_pack<T>), dim3((records + 3) / 4), dim3(256), 0, st, (const T*)wg, (const T*)wu, (const T*)wd, D, F, KD, (int)BWD, (typename N::E*)workspace);
+    hipLaunchKernelGGL((k_ff_narrow<T, KD, BWD>), dim3((unsigned)((M + 127) / 128)), dim3(256), LDS, st, (const T*)x, (const T*)dy, (const char*)workspace, M, D, chunks, act,
+                       (T*)out);
+    return 0;
+}
+template <typename T>
+int narrow_kd(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, int64_t M, int D, int F, int act, void* out, void* workspace, hipStream_t st) {
+    if (D <= 32) return dy ? narrow_run<T, 1, true>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st) : narrow_run<T, 1, false>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st);
+    return dy ? narrow_run<T, 2, true>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st) : narrow_run<T, 2, false>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st);
+}
+
+}  // namespace
+
+// A workgroup walks all features for its 128 rows: where those are many and the rows few, the products of nf_gated_ff.hip, which split the features over the chip, are faster.
+// A chunk takes about 2.5 us, so 16 of them what the products' launches take at their smallest; from 16384 rows on half the CUs are busy here.
+bool ff_narrow_fits(int64_t rows, int dim, int hidden) { return dim <= 64 && (hidden <= 512 || rows >= 16384); }
+
+int64_t ff_narrow_workspace_bytes(int dim, int hidden, int dtype, bool backward) {
+    return (int64_t)((hidden + 31) / 32) * narrow_records(dim <= 32 ? 1 : 2, backward) * (dtype == FF_F32 ? 3 : 1) * 1024;
+}
+
+// dy null: out = the block of x; else out = dx
+int ff_narrow(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, int64_t rows, int dim, int hidden, int dtype, int act, void* out, void* workspace,
+              hipStream_t st) {
+    const auto f = dtype == FF_F32 ? narrow_kd<float> : dtype == FF_BF16 ? narrow_kd<ff_bf16> : narrow_kd<ff_half>;
+    return f(x, wg, wu, wd, dy, rows, dim, hidden, act, out, workspace, st);
+}

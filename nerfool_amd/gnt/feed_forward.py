@@ -100,7 +100,8 @@ class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
         need = any(ctx.needs_input_grad[:4])
-        out, g, u = ops.gated_ff_fwd(x, w_gate, w_up, w_down, activation, save=need)
+        save = need and (any(ctx.needs_input_grad[1:4]) or w_gate.dim() != 2 or not ops.gated_ff_bwd_recomputes(*x.shape, w_gate.shape[0]))
+        out, g, u = ops.gated_ff_fwd(x, w_gate, w_up, w_down, activation, save=save)
         ctx.activation = activation
         if need:
             ctx.save_for_backward(x, w_gate, w_up, w_down, g, u)

@@ -1095,6 +1095,11 @@ def gated_ff_fwd(x, w_gate, w_up, w_down, activation, save=False):
     return out, g, u
 
 
+def gated_ff_bwd_recomputes(rows, dim, hidden):
+    """whether gated_ff_bwd, asked for dx alone, needs no g and u"""
+    return bool(_lib.lib().nf_gated_ff_bwd_recomputes(rows, dim, hidden))
+
+
 def _workspace_bytes(n, name, like):
     if n < 0:
         raise RuntimeError('%s failed: %s' % (name, _lib.lib().nf_last_error().decode()))

@@ -356,6 +356,16 @@ def check_guards(device, rows, dim, hidden, dtype):
     want = ref.gated(x, *ws, 'silu', dy, dtype)
     for t, key, shape in zip((y, *grads), ('out', 'dx', 'dw_gate', 'dw_up', 'dw_down'), ((rows, dim), (rows, dim), (hidden, dim), (hidden, dim), (dim, hidden))):
         near(t[:t.numel() - guard].view(shape), want[key], key)
+    if L.nf_gated_ff_bwd_recomputes(rows, dim, hidden):          # nothing saved, the gradient of x alone
+        need = L.nf_gated_ff_fwd_workspace_bytes(rows, dim, hidden, code), L.nf_gated_ff_bwd_workspace_bytes(rows, dim, hidden, code, 1, 0, 0)
+        w1, w2, y, dx = out(need[0], torch.uint8), out(need[1], torch.uint8), out(n), out(n)
+        _lib.check(L.nf_gated_ff_fwd(p(x), *[p(t) for t in ws], rows, dim, hidden, code, 0, p(y), None, None, p(w1), stream), 'fwd')
+        _lib.check(L.nf_gated_ff_bwd(p(x), *[p(t) for t in ws], p(dy), None, None, rows, dim, hidden, code, 0, p(dx), None, None, None, p(w2), stream), 'bwd')
+        intact((w1, need[0]), (w2, need[1]), (y, n), (dx, n))
+        near(y[:n].view(rows, dim), want['out'], 'out')
+        near(dx[:n].view(rows, dim), want['dx'], 'dx')
+    else:
+        assert L.nf_gated_ff_bwd(p(x), *[p(t) for t in ws], p(dy), None, None, rows, dim, hidden, code, 0, p(grads[0]), None, None, None, p(ws_bytes), stream) != 0
     # one of the two gradients that share a product, and no other
     ws_bytes = out(L.nf_gated_ff_bwd_workspace_bytes(rows, dim, hidden, code, 0, 1, 0), torch.uint8)
     one = out(w)

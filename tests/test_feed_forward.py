@@ -63,6 +63,22 @@ def test_gated(rows, dim, hidden, dtype, act):
     cases.check_gated(rows, dim, hidden, dtype, 'cuda', act=act)
 
 
+FROZEN_SMALL = [(70, 40, 72, F32), (130, 64, 33, BF16), (5, 17, 40, F16), (66, 7, 5, F32)]
+
+
+@pytest.mark.parametrize('rows,dim,hidden,dtype', FROZEN_SMALL)
+def test_gated_constant_weights_standin(emu, rows, dim, hidden, dtype):
+    cases.check_gated(rows, dim, hidden, dtype, emu, act=('silu', 'gelu', 'relu')[rows % 3], frozen=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act', ['silu', 'gelu', 'relu'])
+@pytest.mark.parametrize('rows,dim,hidden,dtype', FROZEN_SMALL + [(1, 64, 256, F32), (4097, 64, 256, F32), (16500, 48, 700, BF16), (300, 64, 512, F16), (300, 64, 513, F32),
+                                                                  (200, 65, 256, F32), (1000, 32, 100, BF16), (40000, 33, 64, F32)])
+def test_gated_constant_weights(rows, dim, hidden, dtype, act):
+    cases.check_gated(rows, dim, hidden, dtype, 'cuda', act=act, frozen=True)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', [F32, BF16, F16])
 def test_gated_large_tiles(dtype):
@@ -235,13 +251,13 @@ def test_forms_of_other_types():
     cases.check_not_finite('cuda', 3000, BF16)
 
 
-@pytest.mark.parametrize('rows,dim,hidden,dtype', [(3, 37, 21, F32), (67, 24, 17, BF16)])
+@pytest.mark.parametrize('rows,dim,hidden,dtype', [(3, 37, 21, F32), (67, 24, 17, BF16), (130, 70, 40, F32)])
 def test_nothing_behind_the_outputs_standin(emu, rows, dim, hidden, dtype):
     cases.check_guards(emu, rows, dim, hidden, dtype)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize('rows,dim,hidden,dtype', [(1, 37, 21, F32), (67, 24, 17, BF16), (300, 129, 515, F16), (700, 1000, 333, F32), (1030, 520, 776, BF16),
+@pytest.mark.parametrize('rows,dim,hidden,dtype', [(1, 37, 21, F32), (67, 24, 17, BF16), (333, 64, 256, F32), (300, 129, 515, F16), (700, 1000, 333, F32), (1030, 520, 776, BF16),
                                                    (2, 4100, 70, F16), (2600, 1160, 1288, BF16)])
 def test_nothing_behind_the_outputs(rows, dim, hidden, dtype):
     cases.check_guards('cuda', rows, dim, hidden, dtype)
