@@ -120,31 +120,34 @@ __device__ __forceinline__ ff_bf16x8 ff_from_e4m3x8(unsigned lo, unsigned hi, un
 enum { FF_F32 = 0, FF_BF16 = 1, FF_F16 = 2 };
 enum { FF_SILU = 0, FF_GELU = 1, FF_RELU = 2 };
 
-// act(g) and act'(g).  FAST (results that are rounded to 16 bits): the hardware's exponential and reciprocal, good to 2^-21
-template <bool FAST>
+// act(g) and act'(g).  The hardware's exponential and reciprocal: good to about (1 + |g|) 2^-23, below what the float32 sums behind g are off by.  gelu's erfc by the
+// Chebyshev fit of Numerical Recipes (section 6.2, erfcc: 1.2e-7 of its value everywhere, so that the tail keeps its digits); the library's erff costs four times
+// the instructions, and beside the products of a narrow block those are what counts.
 __device__ __forceinline__ void ff_act(int act, float g, float& a, float& slope) {
     if (act == FF_SILU) {
-        const float e = 1.f + (FAST ? __expf(-g) : expf(-g)), s = FAST ? nf_rcp(e) : 1.f / e;
+        const float s = nf_rcp(1.f + __expf(-g));
         a = g * s;
         slope = s * (1.f + g * (1.f - s));
     } else if (act == FF_GELU) {
-        const float e = FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g);
-        float cdf;
-        if (FAST) {          // Abramowitz and Stegun 7.1.26 for erf(|g| / sqrt 2): off by at most 1.5e-7
-            const float x = fabsf(g) * 0.70710678118654752f, t = nf_rcp(1.f + 0.3275911f * x);
-            const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-            const float tail = 0.5f * p * e;          // half of erfc(x)
-            cdf = g < 0.f ? tail : 1.f - tail;
-        } else
-            cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+        const float z = fabsf(g) * 0.70710678118654752f, t = nf_rcp(fmaf(0.5f, z, 1.f));
+        float p = fmaf(t, 0.17087277f, -0.82215223f);
+        p = fmaf(t, p, 1.48851587f);
+        p = fmaf(t, p, -1.13520398f);
+        p = fmaf(t, p, 0.27886807f);
+        p = fmaf(t, p, -0.18628806f);
+        p = fmaf(t, p, 0.09678418f);
+        p = fmaf(t, p, 0.37409196f);
+        p = fmaf(t, p, 1.00002368f);
+        p = fmaf(t, p, -1.26551223f);
+        const float tail = 0.5f * t * __expf(fmaf(-z, z, p));          // half of erfc(z)
+        const float cdf = g < 0.f ? tail : 1.f - tail;
         a = g * cdf;
-        slope = cdf + g * (0.39894228040143268f * e);
+        slope = fmaf(g, 0.39894228040143268f * __expf(-z * z), cdf);
     } else {
         a = g > 0.f ? g : (g != g ? g : 0.f);
         slope = g > 0.f ? 1.f : 0.f;
     }
 }
-
 // ---- stores of 4 consecutive values of a row (`left`: how many the row still has)
 template <typename T>
 __device__ __forceinline__ void ff_put(T* p, int left, const ff_f32x4& v) {

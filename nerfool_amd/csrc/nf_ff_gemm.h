@@ -2,6 +2,8 @@
 // element-wise work of the block in its output stage.
 //
 // Operands (16-bit, NP planes: 1, or 3 for a float32 operand held as three bf16 parts, whose six products of order <= 2^-16 give float32-grade sums):
+// The three planes lie in blocks of 32 values along a row, [block][plane][32]: what a step of 32 k reads of a row is 192 bytes in one place (apart, the planes' 64 bytes were half
+// cache lines each, and the L2 gave half its rate); rows are padded to a multiple of 32 values.
 //   k innermost    row r at a + r * pitch, k contiguous.  A gated P has two sources: the features' gate rows in a and their up rows in b.
 //   k outermost    row k at a + k * pitch (k < seg) or b + (k - seg) * pitch, the product's n or m contiguous: the gradients' products read the
 //                  tensors as they lie, the transposition happens in the LDS read (ds_read_b64_tr_b16).
@@ -22,7 +24,7 @@
 
 struct FfOperand {
     const uint16_t *a, *b;
-    int64_t plane, pitch;          // elements
+    int64_t pitch;                 // elements (of all planes)
     int rows;                      // n or m
     int len, seg;                  // k outermost: rows k < len are a's, rows k >= seg are b's, rows between are zeros
 };
@@ -138,16 +140,16 @@ struct FfLoader {
     static constexpr int BYTES = NP * PIECES * 1024;
     static_assert(NP * PIECES % WAVES == 0, "every wave moves the same number of pieces");
     static_assert(!GATED || (WSPAN / 2) % RPP == 0, "a piece's rows are of one source");
+    static constexpr int PER_K = NP == 3 ? 6 : 2;                             // bytes a k
     unsigned off[PER_WAVE];
     const char *a, *b;
-    int64_t plane, pitch;          // bytes
+    int64_t pitch;          // bytes
     int len, seg;
 
     __device__ __forceinline__ void init(const FfOperand& o, int row0, int wave, int lane) {
         const int slot = lane % CH, rr = lane / CH;
         a = (const char*)o.a;
         b = (const char*)o.b;
-        plane = o.plane * 2;
         pitch = o.pitch * 2;
         len = o.len;
         seg = o.seg;
@@ -157,16 +159,16 @@ struct FfLoader {
         }
 #pragma unroll
         for (int i = 0; i < PER_WAVE; ++i) {
-            const int r = (wave * PER_WAVE + i) % PIECES * RPP + rr;
+            const int li = wave * PER_WAVE + i, r = li % PIECES * RPP + rr, plane = li / PIECES;
             // a row, or columns, behind the end: the last ones, whose results are not stored
             if (OUTER) {
                 int col = row0 + 8 * (slot ^ ff_swz_outer<CH>(r));
                 if (col >= o.rows) col = o.rows - 8;
-                off[i] = (unsigned)(r * pitch + 2 * col);
+                off[i] = (unsigned)(r * pitch + (NP == 3 ? col / 32 * 192 + 64 * plane + col % 32 * 2 : 2 * col));
             } else {
                 int row = GATED ? (r / WSPAN) * (WSPAN / 2) + r % (WSPAN / 2) : r;          // a wave's WSPAN rows: half gate, half up, of the same features
                 if (row0 + row >= o.rows) row = o.rows - 1 - row0;
-                off[i] = (unsigned)(row * pitch + 16 * (slot ^ ff_swz_inner<CH>(r)));
+                off[i] = (unsigned)(row * pitch + 64 * plane + 16 * (slot ^ ff_swz_inner<CH>(r)));          // (one plane: plane 0)
             }
         }
     }
@@ -177,8 +179,7 @@ struct FfLoader {
         const int li = wave * PER_WAVE + i;
         const char* base = GATED && li % PIECES * RPP % WSPAN >= WSPAN / 2 ? b : a;
         if (OUTER) base = k0 >= seg ? b + (k0 - seg) * pitch : a + k0 * pitch;
-        else base += 2 * (int64_t)k0;
-        if (NP > 1) base += li / PIECES * plane;
+        else base += PER_K * (int64_t)k0;
         if (WHOLE) {
             ff_dma16(base, off[i], lds, at + li * 1024, lane);
         } else {

@@ -3,7 +3,7 @@
 // out[m][n] = sum over k of X[m][k] W[n][k], m < 16 NT.  A workgroup owns 16 (in 8 bits 32) rows n of the weights -- gate and up rows of the same
 // features --, its waves take turns along k.  A lane loads 16 bytes of a weight row straight into the operand registers of a 16 x 16 matrix
 // instruction (A: 16 weight rows, B: 16 tokens): lane l holds row l mod 16, k = V (l / 16) .. + V - 1 of each step, for both operands alike, so that any
-// order of k inside a step is right.  A wave keeps two units of 4 steps in flight.  The waves' sums meet in LDS, in the order of the waves.
+// order of k inside a step is right.  A wave keeps two units of 4 (2) steps in flight.  The waves' sums meet in LDS, in the order of the waves.
 // Rows may start at any element's address: nothing is padded or copied.
 //
 // float32 uses the float32 matrix instruction (the weights' bytes bound it up to 32 tokens); 8-bit values become bfloat16 operands, exactly.
@@ -50,7 +50,8 @@ __device__ __forceinline__ typename FfRow<T>::V ff_row_load(const T* row, int k,
     return v;
 }
 
-constexpr int FF_ROWS_UNIT = 4;          // steps
+// steps of a unit: two units are in flight in registers
+constexpr int ff_rows_unit(int nt, bool gated) { return gated && nt == 4 ? 2 : 4; }
 // most waves of a workgroup: 64 KB of LDS for their sums, and registers for the two units in flight
 constexpr int ff_rows_most(int nt) { return nt == 1 ? 16 : 8; }
 
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(64 * ff_rows_most(NT)) k_ff_rows(const T* __re
                                                   T* __restrict__ out, float* __restrict__ g_save, float* __restrict__ u_save, int act) {
     typedef FfRow<T> R;
     typedef typename R::V V;
-    constexpr int NW = GATED ? 2 : 1, U = FF_ROWS_UNIT, STEP = 4 * R::KV, UNIT = U * STEP;
+    constexpr int NW = GATED ? 2 : 1, U = ff_rows_unit(NT, GATED), STEP = 4 * R::KV, UNIT = U * STEP;
     HIP_DYNAMIC_SHARED(ff_f32x4, part)
     const int t0 = blockIdx.y * 16 * NT;          // this workgroup's first token
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(64 * ff_rows_most(NT)) k_ff_rows(const T* __re
             float y = v[c];
             if (GATED) {
                 float ac, slope;
-                ff_act<sizeof(T) == 2>(act, v[c], ac, slope);
+                ff_act(act, v[c], ac, slope);
                 y = ac * u[c];
                 if (g_save) {
                     g_save[at] = v[c];
@@ -188,7 +189,7 @@ static inline int ff_rows_tokens(int M, int groups) {
 
 template <typename T, int NT, bool GATED>
 int ff_rows_launch(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, hipStream_t st) {
-    const int groups = (N + 15) / 16, unit = FF_ROWS_UNIT * 4 * FfRow<T>::KV;
+    const int groups = (N + 15) / 16, unit = ff_rows_unit(NT, GATED) * 4 * FfRow<T>::KV;
     const int waves = ff_rows_waves(groups, (K + unit - 1) / unit, ff_rows_most(NT));
     hipLaunchKernelGGL((k_ff_rows<T, NT, GATED>), dim3(groups, (M + 16 * NT - 1) / (16 * NT)), dim3(64 * waves), (size_t)waves * (GATED ? 2 : 1) * NT * 1024, st, (const T*)w0, (const T*)w1,
                        (const T*)x, M, N, K, (T*)out, g_save, u_save, act);

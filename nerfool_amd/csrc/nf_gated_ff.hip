@@ -19,21 +19,18 @@ int ff_narrow(const void* x, const void* wg, const void* wu, const void* wd, con
 
 namespace {
 
-__device__ __forceinline__ void ff_put3(ff_bf16* p, int64_t plane, int left, const ff_f32x4& v) {
+// ... at p, p + 32, p + 64
+__device__ __forceinline__ void ff_put3(ff_bf16* p, int left, const ff_f32x4& v) {
     ff_bf16 t[4][3];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) ff_split3(v[c], t[c]);
+    for (int c = 0; c < 4; ++c) ff_split3(c < left ? v[c] : 0.f, t[c]);          // (behind the row's end: zeros)
 #pragma unroll
     for (int e = 0; e < 3; ++e) {
-        if (left >= 4) {
-            typedef ff_bf16 V4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<V4*>(p + e * plane) = V4{t[0][e], t[1][e], t[2][e], t[3][e]};
-        } else {
-            for (int c = 0; c < 4; ++c) p[e * plane + c] = c < left ? t[c][e] : (ff_bf16)0.f;          // the padding of the row: zeros
-        }
+        typedef ff_bf16 V4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<V4*>(p + 32 * e) = V4{t[0][e], t[1][e], t[2][e], t[3][e]};
     }
 }
-// an operand of a later product: 16-bit values, or three planes of bf16 parts (T = float); rows padded to `pitch`, a multiple of 8
+// an operand of a later product: 16-bit values, or three planes of bf16 parts (T = float); rows padded to `pitch`, a multiple of ff_pad
 template <typename T>
 struct FfMid {
     T* p;
@@ -50,8 +47,8 @@ struct FfMid {
 template <>
 struct FfMid<float> {
     ff_bf16* p;
-    int64_t pitch, plane;
-    __device__ __forceinline__ void put(int64_t m, int n, int left, const ff_f32x4& v) const { ff_put3(p + m * pitch + n, plane, left, v); }
+    int64_t pitch;
+    __device__ __forceinline__ void put(int64_t m, int n, int left, const ff_f32x4& v) const { ff_put3(p + 3 * m * pitch + n / 32 * 96 + n % 32, left, v); }
 };
 
 template <typename T>
@@ -88,7 +85,7 @@ struct EpiGate {
         float a, slope;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            ff_act<sizeof(T) == 2>(act, g[c], a, slope);
+            ff_act(act, g[c], a, slope);
             v[c] = a * u[c];
         }
         h.put(m, n, left, v);
@@ -118,7 +115,7 @@ struct EpiGateBwd {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             float a, slope;
-            ff_act<sizeof(T) == 2>(act, gv[c], a, slope);
+            ff_act(act, gv[c], a, slope);
             hv[c] = a * uv[c];
             dg[c] = dh[c] * uv[c] * slope;
             du[c] = dh[c] * a;
@@ -145,7 +142,7 @@ __global__ void __launch_bounds__(256) k_ff_join(EpiPart parts, int n_parts, int
     }
 }
 
-// rows [R, C] -> rows padded with zeros to `pitch` (a multiple of 8); float -> three planes of bf16 parts.  Up to 5 tensors a launch: blockIdx.y
+// rows [R, C] -> rows padded with zeros to `pitch`; float -> three planes of bf16 parts.  Up to 5 tensors a launch: blockIdx.y
 template <typename T>
 struct FfPackJobs {
     struct Job {
@@ -188,7 +185,11 @@ struct FfElem<float> {
     static constexpr int NP = 3;
 };
 
-int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+// rows of operands: 16-byte chunks; three planes lie in blocks of 32
+template <typename T>
+int64_t ff_pad(int64_t n) {
+    return sizeof(T) == 4 ? (n + 31) / 32 * 32 : (n + 7) / 8 * 8;
+}
 
 // carves a workspace; with base = nullptr it only counts
 struct Carve {
@@ -211,17 +212,16 @@ FfMid<T> mid_at(Carve& ws, int64_t rows, int64_t pitch) {
 template <>
 FfMid<float> mid_at<float>(Carve& ws, int64_t rows, int64_t pitch) {
     FfMid<float> m;
-    m.plane = rows * pitch;
-    m.p = (ff_bf16*)ws.take(3 * m.plane * 2);
+    m.p = (ff_bf16*)ws.take(3 * rows * pitch * 2);
     m.pitch = pitch;
     return m;
 }
 template <typename T>
 FfOperand as_operand(const FfMid<T>& m, int rows) {
-    return FfOperand{(const uint16_t*)m.p, (const uint16_t*)m.p, 0, m.pitch, rows, 0x7fffffff, 0x7fffffff};
+    return FfOperand{(const uint16_t*)m.p, (const uint16_t*)m.p, m.pitch, rows, 0x7fffffff, 0x7fffffff};
 }
 FfOperand as_operand(const FfMid<float>& m, int rows) {
-    return FfOperand{(const uint16_t*)m.p, (const uint16_t*)m.p, m.plane, m.pitch, rows, 0x7fffffff, 0x7fffffff};
+    return FfOperand{(const uint16_t*)m.p, (const uint16_t*)m.p, 3 * m.pitch, rows, 0x7fffffff, 0x7fffffff};
 }
 
 // a tensor [rows, cols] as an operand: itself where the kernel can read it, else a padded (and for float32 split) copy
@@ -235,7 +235,7 @@ FfPacked<T> pack_at(Carve& ws, int64_t rows, int cols) {
     FfPacked<T> p;
     p.copy = sizeof(T) == 4 || cols % 8 != 0;
     if (p.copy)
-        p.mid = mid_at<T>(ws, rows, pad8(cols));
+        p.mid = mid_at<T>(ws, rows, ff_pad<T>(cols));
     else {
         p.mid.p = nullptr;
         p.mid.pitch = cols;
@@ -376,8 +376,8 @@ struct FwdPlan {
         wg = pack_at<T>(ws, F, D);
         wu = pack_at<T>(ws, F, D);
         wd = pack_at<T>(ws, D, F);
-        h = mid_at<T>(ws, M, pad8(F));
-        parts = (float*)ws.take(ff_part_bytes(FfElem<T>::NP == 3, M, D, pad8(F)));
+        h = mid_at<T>(ws, M, ff_pad<T>(F));
+        parts = (float*)ws.take(ff_part_bytes(FfElem<T>::NP == 3, M, D, ff_pad<T>(F)));
         bytes = ws.used;
     }
 };
@@ -430,13 +430,13 @@ struct BwdPlan {
         wd = pack_at<T>(ws, D, F);
         if (dwgu) x = pack_at<T>(ws, M, D);
         if (dx) wg = pack_at<T>(ws, F, D), wu = pack_at<T>(ws, F, D);
-        dgu = mid_at<T>(ws, M, 2 * pad8(F));
-        if (dwd) h = mid_at<T>(ws, M, pad8(F));
+        dgu = mid_at<T>(ws, M, 2 * ff_pad<T>(F));
+        if (dwd) h = mid_at<T>(ws, M, ff_pad<T>(F));
         const bool three = FfElem<T>::NP == 3;
         int64_t most = 0;
-        if (dx) most = ff_part_bytes(three, M, D, pad8(F) + F);
+        if (dx) most = ff_part_bytes(three, M, D, ff_pad<T>(F) + F);
         if (dwgu) {
-            const int64_t n = ff_part_bytes(three, 2 * pad8(F), D, M);
+            const int64_t n = ff_part_bytes(three, 2 * ff_pad<T>(F), D, M);
             most = n > most ? n : most;
         }
         if (dwd) {
@@ -453,7 +453,7 @@ int ff_bwd(const void* x, const void* wg, const void* wu, const void* wd, const 
            int act, void* dx, void* dwg, void* dwu, void* dwd, void* workspace, hipStream_t st) {
     const bool dwgu = dwg || dwu;
     BwdPlan<T> f((char*)workspace, M, D, F, dx != nullptr, dwgu, dwd != nullptr);
-    const int Fp = (int)pad8(F);
+    const int Fp = (int)ff_pad<T>(F);
     Packing<T> pack;
     pack.add(dy, M, D, f.dy);
     pack.add(wd, D, F, f.wd);

@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(64 * ff_rows8_most(NT, GATED)) k_ff_rows8(cons
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float ac, slope;
-                    ff_act<false>(act, v[h][c], ac, slope);
+                    ff_act(act, v[h][c], ac, slope);
                     v[h][c] = ac * u[c];
                     top = fmaxf(top, fabsf(v[h][c]));
                     bad |= !(fabsf(v[h][c]) <= 3.4028235e38f);
@@ -348,7 +348,6 @@ struct Epi8Store {
     __device__ __forceinline__ void gated(int, int, int, int, bool, const ff_f32x4&, const ff_f32x4&) const {}
 };
 
-template <bool FAST>
 struct Epi8Gate {
     uint8_t *q, *scale;
     int64_t F, scale_pitch;
@@ -360,7 +359,7 @@ struct Epi8Gate {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             float a, slope;
-            ff_act<FAST>(act, g[c], a, slope);
+            ff_act(act, g[c], a, slope);
             v[c] = a * u[c];
             top = fmaxf(top, fabsf(v[c]));
             bad |= !(fabsf(v[c]) <= 3.4028235e38f);
@@ -409,7 +408,7 @@ int product8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const F
 }
 
 FfOperand operand8(const void* a, const void* b, int rows, int K) {
-    return FfOperand{(const uint16_t*)a, (const uint16_t*)b, 0, K / 2, rows, 0x7fffffff, 0x7fffffff};
+    return FfOperand{(const uint16_t*)a, (const uint16_t*)b, K / 2, rows, 0x7fffffff, 0x7fffffff};
 }
 
 // the workspace of the tiled form: h in 8 bits, and the scales whose rows are no multiple of 4 bytes
@@ -466,8 +465,8 @@ extern "C" int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const
     const FfOperand pg = operand8(w_gate, w_up, F, D), qx = operand8(x, x, M, D);
     const FfScales sqx = {padded_scales(x_scale, M, D / 32, f.dp, f.xs, st), nullptr, f.dp, M};
     const FfScales spg = {padded_scales(gate_scale, F, D / 32, f.dp, f.gs, st), padded_scales(up_scale, F, D / 32, f.dp, f.us, st), f.dp, F};
-    int rc = out_dtype == FF_BF16 ? product8<true, false>(pg, qx, spg, sqx, M, F, D, Epi8Gate<true>{f.hq, f.hs, F, f.fp, activation}, st)
-                                  : product8<true, true>(pg, qx, spg, sqx, M, F, D, Epi8Gate<false>{f.hq, f.hs, F, f.fp, activation}, st);
+    int rc = out_dtype == FF_BF16 ? product8<true, false>(pg, qx, spg, sqx, M, F, D, Epi8Gate{f.hq, f.hs, F, f.fp, activation}, st)
+                                  : product8<true, true>(pg, qx, spg, sqx, M, F, D, Epi8Gate{f.hq, f.hs, F, f.fp, activation}, st);
     if (rc) return rc;
     const FfOperand p = operand8(w_down, w_down, D, F), q = operand8(f.hq, f.hq, M, F);
     const FfScales sp = {padded_scales(down_scale, D, F / 32, f.fp, f.ds, st), nullptr, f.fp, D}, sq = {f.hs, f.hs, f.fp, M};

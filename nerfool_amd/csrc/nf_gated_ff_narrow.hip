@@ -1,13 +1,14 @@
 // The gated feed-forward block at the widths of the ray transformer (dim <= 64: gnt/transformer_network.py:38-50 has 64 and 256) in one kernel a direction: what the block
 // computes between its input and its output never leaves the registers.
 //
-// A wave owns 32 tokens.  The features are walked in chunks of 32: g and u of the chunk are made as 16 x 16 blocks (weights the A operand, tokens the B operand, so that a
+// A wave owns 16 tokens.  The features are walked in chunks of 32: g and u of the chunk are made as 16 x 16 blocks (weights the A operand, tokens the B operand, so that a
 // lane holds 4 consecutive features of one token), h of the chunk goes back into B operands as it lies -- the lane's 4 features of the first block are its k 0 .. 3 and those of
 // the second its k 4 .. 7; the down projection's records have their features in that order -- and out grows by the chunk's share.  The backward pass to x alone (constant
 // weights, as in an attack) makes g and u again instead of reading them: dx += dg Wg + du Wu the same way, with dh = dy Wd of the chunk between.
-// The weights come as records of operand fragments (k_ff_narrow_pack, per call), 1 KB each, by LDS-DMA, one chunk ahead, for the four waves of a workgroup.  float32: three bf16
+// The weights come as records of operand fragments (k_ff_narrow_pack, per call), 1 KB each, by LDS-DMA, one chunk ahead, for the eight waves of a workgroup.  float32: three bf16
 // parts of every operand, six products (nf_gated_ff.hip); h, dg and du are then split, not rounded.  Bound by the matrix instructions and, as much, by the vector
-// instructions of activation and split between them: 32768 x 64 x 256 float32 takes TODO us forward and TODO us backward (in separate products: 69 and 80).
+// instructions of activation and split between them: 32768 x 64 x 256 float32 takes 30 us forward and 43
+// backward, and 5 each for the records (in separate products: 69 and 80; four waves of 32 tokens, one a SIMD: 47 and 67).
 #include "nf_ff_gemm.h"
 
 namespace {
@@ -93,99 +94,83 @@ struct Narrow {
             for (int e = 0; e < NP; ++e) v[e][j] = p[e];
         }
     }
-    // acc[tt] += record n x b[tt], smallest products first
-    static __device__ __forceinline__ void multiply(const char* lds, int n, int lane, const V (&b0)[NP], const V (&b1)[NP], ff_f32x4& c0, ff_f32x4& c1) {
+    // c += record n x b, smallest products first
+    static __device__ __forceinline__ void multiply(const char* lds, int n, int lane, const V (&b)[NP], ff_f32x4& c) {
         V a[NP];
 #pragma unroll
         for (int e = 0; e < NP; ++e) a[e] = *reinterpret_cast<const V*>(lds + (n * NP + e) * 1024 + lane * 16);
 #pragma unroll
         for (int o = NP - 1; o >= 0; --o)
 #pragma unroll
-            for (int e = 0; e <= o; ++e) {
-                c0 = Mfma::mul(a[e], b0[o - e], c0);
-                c1 = Mfma::mul(a[e], b1[o - e], c1);
-            }
+            for (int e = 0; e <= o; ++e) c = Mfma::mul(a[e], b[o - e], c);
     }
 };
 
 template <typename T, int KD, bool BWD>
-__global__ void __launch_bounds__(256) k_ff_narrow(const T* __restrict__ x, const T* __restrict__ dy, const char* __restrict__ records, int64_t M, int D, int chunks, int act,
+__global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, const T* __restrict__ dy, const char* __restrict__ records, int64_t M, int D, int chunks, int act,
                                                    T* __restrict__ out) {
     typedef Narrow<T, KD, BWD> N;
     typedef typename N::V V;
-    constexpr int NP = N::NP;
-    constexpr bool FAST = sizeof(T) == 2;
+    constexpr int NP = N::NP, WAVES = 8;
     HIP_DYNAMIC_SHARED(char, lds)
     const int lane = threadIdx.x & 63, wave = ff_wave_index(), q = lane >> 4;
-    const int64_t m0 = (int64_t)blockIdx.x * 128 + wave * 32 + (lane & 15);          // this lane's tokens: m0, m0 + 16
+    const int64_t m = (int64_t)blockIdx.x * (16 * WAVES) + wave * 16 + (lane & 15);          // this lane's token
     auto load_chunk = [&](int c) {
         const char* src = records + (int64_t)c * N::CHUNK;
-        for (int p = wave; p < N::PIECES; p += 4) ff_dma16(src + p * 1024, (unsigned)lane * 16, lds, (c & 1) * N::CHUNK + p * 1024, lane);
+        for (int p = wave; p < N::PIECES; p += WAVES) ff_dma16(src + p * 1024, (unsigned)lane * 16, lds, (c & 1) * N::CHUNK + p * 1024, lane);
     };
     load_chunk(0);
-    V xb[KD][2][NP], yb[BWD ? KD : 1][2][NP];
+    V xb[KD][NP], yb[BWD ? KD : 1][NP];
 #pragma unroll
-    for (int k = 0; k < KD; ++k)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            N::row(x, m0 + 16 * t, M, D, 32 * k + 8 * q, xb[k][t]);
-            if (BWD) N::row(dy, m0 + 16 * t, M, D, 32 * k + 8 * q, yb[BWD ? k : 0][t]);
-        }
+    for (int k = 0; k < KD; ++k) {
+        N::row(x, m, M, D, 32 * k + 8 * q, xb[k]);
+        if (BWD) N::row(dy, m, M, D, 32 * k + 8 * q, yb[BWD ? k : 0]);
+    }
     const ff_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    ff_f32x4 sum[2 * KD][2];
+    ff_f32x4 sum[2 * KD];
 #pragma unroll
-    for (int i = 0; i < 2 * KD; ++i) sum[i][0] = sum[i][1] = zero;
+    for (int i = 0; i < 2 * KD; ++i) sum[i] = zero;
     for (int c = 0; c < chunks; ++c) {
         ff_dma_barrier<0>();          // the chunk has landed for every wave, and the other buffer has been read by every wave
         if (c + 1 < chunks) load_chunk(c + 1);
         const char* w = lds + (c & 1) * N::CHUNK;
-        ff_f32x4 g[2][2], u[2][2], dh[2][2];
+        ff_f32x4 g[2], u[2], dh[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            g[i][0] = g[i][1] = u[i][0] = u[i][1] = dh[i][0] = dh[i][1] = zero;
+            g[i] = u[i] = dh[i] = zero;
 #pragma unroll
             for (int k = 0; k < KD; ++k) {
-                N::multiply(w, i * KD + k, lane, xb[k][0], xb[k][1], g[i][0], g[i][1]);
-                N::multiply(w, (2 + i) * KD + k, lane, xb[k][0], xb[k][1], u[i][0], u[i][1]);
-                if (BWD) N::multiply(w, (4 + i) * KD + k, lane, yb[BWD ? k : 0][0], yb[BWD ? k : 0][1], dh[i][0], dh[i][1]);
+                N::multiply(w, i * KD + k, lane, xb[k], g[i]);
+                N::multiply(w, (2 + i) * KD + k, lane, xb[k], u[i]);
+                if (BWD) N::multiply(w, (4 + i) * KD + k, lane, yb[BWD ? k : 0], dh[i]);
             }
         }
-        V hb[2][NP], ub[2][NP];          // forward: h; backward: dg and du
+        V hb[NP], ub[NP];          // forward: h; backward: dg and du
+        float v[8], v2[8];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            float v[8], w2[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float gv = g[j / 4][t][j % 4], uv = u[j / 4][t][j % 4];
-                float a, slope;
-                ff_act<FAST>(act, gv, a, slope);
-                if (BWD) {
-                    const float d = dh[j / 4][t][j % 4];
-                    v[j] = d * uv * slope;
-                    w2[j] = d * a;
-                } else
-                    v[j] = a * uv;
-            }
-            N::operand(v, hb[t]);
-            if (BWD) N::operand(w2, ub[t]);
+        for (int j = 0; j < 8; ++j) {
+            const float gv = g[j / 4][j % 4], uv = u[j / 4][j % 4];
+            float a, slope;
+            ff_act(act, gv, a, slope);
+            if (BWD) {
+                const float d = dh[j / 4][j % 4];
+                v[j] = d * uv * slope;
+                v2[j] = d * a;
+            } else
+                v[j] = a * uv;
         }
+        N::operand(v, hb);
+        if (BWD) N::operand(v2, ub);
 #pragma unroll
         for (int i = 0; i < 2 * KD; ++i) {
-            if (BWD) {
-                N::multiply(w, 6 * KD + i, lane, hb[0], hb[1], sum[i][0], sum[i][1]);
-                N::multiply(w, 8 * KD + i, lane, ub[0], ub[1], sum[i][0], sum[i][1]);
-            } else
-                N::multiply(w, 4 * KD + i, lane, hb[0], hb[1], sum[i][0], sum[i][1]);
+            N::multiply(w, (BWD ? 6 : 4) * KD + i, lane, hb, sum[i]);
+            if (BWD) N::multiply(w, 8 * KD + i, lane, ub, sum[i]);
         }
     }
     ff_dma_barrier<0>();          // no load may land in LDS that the workgroup has given back
+    if (m >= M) return;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int64_t m = m0 + 16 * t;
-        if (m >= M) continue;
-#pragma unroll
-        for (int i = 0; i < 2 * KD; ++i) ff_put(out + m * D + 16 * i + 4 * q, D - (16 * i + 4 * q), sum[i][t]);
-    }
+    for (int i = 0; i < 2 * KD; ++i) ff_put(out + m * D + 16 * i + 4 * q, D - (16 * i + 4 * q), sum[i]);
 }
 
 template <typename T, int KD, bool BWD>
@@ -204,7 +189,7 @@ int narrow_run(const void* x, const void* wg, const void* wu, const void* wd, co
     }
     const int chunks = (F + 31) / 32, records = N::RECORDS * chunks;
     hipLaunchKernelGGL((k_ff_narrow_pack<T>), dim3((records + 3) / 4), dim3(256), 0, st, (const T*)wg, (const T*)wu, (const T*)wd, D, F, KD, (int)BWD, (typename N::E*)workspace);
-    hipLaunchKernelGGL((k_ff_narrow<T, KD, BWD>), dim3((unsigned)((M + 127) / 128)), dim3(256), LDS, st, (const T*)x, (const T*)dy, (const char*)workspace, M, D, chunks, act,
+    hipLaunchKernelGGL((k_ff_narrow<T, KD, BWD>), dim3((unsigned)((M + 127) / 128)), dim3(512), LDS, st, (const T*)x, (const T*)dy, (const char*)workspace, M, D, chunks, act,
                        (T*)out);
     return 0;
 }
@@ -217,7 +202,7 @@ int narrow_kd(const void* x, const void* wg, const void* wu, const void* wd, con
 }  // namespace
 
 // A workgroup walks all features for its 128 rows: where those are many and the rows few, the products of nf_gated_ff.hip, which split the features over the chip, are faster.
-// A chunk takes about 2.5 us, so 16 of them what the products' launches take at their smallest; from 16384 rows on half the CUs are busy here.
+// A chunk takes 2 to 4 us, so 16 of them what the products' launches take at their smallest; from 16384 rows on half the CUs are busy here.
 bool ff_narrow_fits(int64_t rows, int dim, int hidden) { return dim <= 64 && (hidden <= 512 || rows >= 16384); }
 
 int64_t ff_narrow_workspace_bytes(int dim, int hidden, int dtype, bool backward) {
