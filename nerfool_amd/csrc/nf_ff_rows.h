@@ -6,6 +6,9 @@
 // order of k inside a step is right.  A wave keeps two units of 4 (2) steps in flight.  The waves' sums meet in LDS, in the order of the waves.
 // Rows may start at any element's address: nothing is padded or copied.
 //
+// 1 x 4096 x 8192 bf16: gate and up 29 to 32 us, down 14 us (4.2 to 4.8 TB/s; a copy reaches 5.1); 40 x 2048 x 5504 float16: 23 and 17 us, where the tokens' rows, read again by
+// every workgroup through the L2, are as many bytes as the weights.
+//
 // float32 uses the float32 matrix instruction (the weights' bytes bound it up to 32 tokens); 8-bit values become bfloat16 operands, exactly.
 #pragma once
 

@@ -8,6 +8,10 @@
 // makes out.  Backward: dh's product stores [dg | du] (one [M, 2F] tensor) and h again; then dx (k = 2F over [Wg; Wu]), [dWg; dWu] and dWd.
 // h, dg and du are rounded once, to the inputs' type, because they are operands of a matrix product in that type.  float32 inputs are split into
 // three bf16 parts (8 + 8 + 8 bits, exact) and multiplied as six products of order <= 2^-16: float32-grade sums at 16 / 6 of the float32 pipe's rate.
+//
+// Bound by the matrix instructions at the clock that the card keeps under them, and by the L2's rate for the tiles.  4096 x 4096 x 8192 bf16: gate and up 442 us (1.24
+// PFLOP/s), down 212 us (1.30; a library product of that size 1.45).  4096 x 2048 x 8192, all gradients: forward 281 + 125 + 14 (joining two parts of k), dh and its output
+// stage 212, dx 242 + 14, [dWg; dWu] 225, dWd 118.  float32 1500 x 500 x 1333: products of 19 to 38 us, of which about 8 are not the k loop.
 #include "nf_ff_gemm.h"
 #include "nf_ff_rows.h"
 

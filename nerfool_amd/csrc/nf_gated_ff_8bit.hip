@@ -11,6 +11,9 @@
 // neighbouring step.  Beside a bfloat16 result's rounding that is small (0.0020 against 0.0017 from the exact sums at 4096 x 4096 x 8192); beside a float16
 // or float32 result's it is not.  For those the values are multiplied as bfloat16, which holds value and scale exactly, on
 // v_mfma_f32_32x32x16_bf16: float32 sums, at half the rate; v_cvt_scalef32_pk_bf16_fp8 makes two operands of two values and their scale.
+//
+// 4096 x 4096 x 8192: gate and up 305 us (1.8 PFLOP/s), down 131 us (2.1; a library product of 8192^3 2.65): two waves a SIMD whose fragment reads wait in front of their
+// products -- put between them, as the 16-bit kernels do, they need more registers than there are.  4 x 4096 x 8192: 22 and 11 us, 3 TB/s of weights.
 #include "nf_ff_gemm.h"
 #include "nf_ff_rows.h"
 

@@ -5,8 +5,10 @@
 //   dx = dr = rstd (w dy - xhat mean(w dy xhat)) + dh,  dw = sum over rows of dy xhat,  xhat = h rstd
 //
 // HBM bounds it: every tensor is read or written once.  A row's values stay in registers between the statistics and their use; a row is
-// owned by 8 to 64 lanes of a wave (rows up to 512 vectors of 16 bytes, where there are enough rows to fill the chip) or by a workgroup;
-// rows longer than 8192 vectors are read twice.  The squares and sums are float; y is made from the float sum x + r, not from h as rounded.
+// owned by 8 to 64 lanes of a wave or, above 64 (128 where there are many rows) vectors of 16 bytes, by a workgroup; rows longer than 4096 vectors are
+// read twice.  The squares and sums are float; y is made from the float sum x + r, not from h as rounded.
+// 8192 x 4096 bf16 with a residual to 8 bits: 49 us, 4.8 TB/s of the 5.1 that a copy reaches; 32768 x 64 float32: forward 8.6 us, backward 8.9 + 2.4 us for dw's
+// partial sums; one row of 4096: 3.2 us, a launch.
 #include "nf_ff.h"
 
 namespace {
@@ -353,8 +355,9 @@ int64_t rms_grid(int64_t rows, int rows_per_block, int64_t most) {
     return g < most ? g : most;
 }
 
-// vectors of 16 bytes in a row -> threads a row and vectors a thread.  Up to 64 vectors the row is a part of a wave; up to 512 a wave owns it
-// where there are 2048 rows or more (8 waves a CU; the sums need no barrier), else, and above, a workgroup does.
+// vectors of 16 bytes in a row -> threads a row and vectors a thread.  Up to 64 vectors the row is a part of a wave; up to 128 a wave owns it where there are 2048 rows
+// or more (8 waves a CU; the sums need no barrier), else, and above, a workgroup does: of 512 vectors a wave holds 240 registers and reads 8192 rows in 138 us,
+// a workgroup of four waves in 48.
 #define RMS_DISPATCH(VECS, ROWS, GO, LONG)          \
     do {                                            \
         const int nv_ = (VECS);                     \
