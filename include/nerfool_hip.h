@@ -437,7 +437,7 @@ int nf_in_act_pad_bwd(const float* dy_padded, const float* d_extra, const float*
  * nf_quantize_8bit: x itself in that 8-bit form.
  *
  * nf_gated_ff_fwd: out [rows, dim] = (act(x Wg^T) * (x Wu^T)) Wd^T; Wg, Wu [hidden, dim], Wd [dim, hidden].  g_save, u_save (nullable, together):
- *   x Wg^T and x Wu^T in float, [rows, hidden], for the backward pass.  Operand pointers must be 16-byte aligned.
+ *   x Wg^T and x Wu^T in float, [rows, hidden], for the backward pass; with relu the sign of g is the exact sum's.  Operand pointers must be 16-byte aligned.
  * nf_gated_ff_bwd: the gradients that are not NULL of dx [rows, dim], dw_gate, dw_up [hidden, dim], dw_down [dim, hidden] from dy, g, u.  Where
  *   nf_gated_ff_bwd_recomputes(rows, dim, hidden) is not 0 and dx alone is asked for, g and u are made again and may be NULL.
  * nf_gated_ff_fwd_8bit: the block on operands in the 8-bit form above (dim, hidden multiples of 32; scales [rows of the operand, k / 32] bytes); h in

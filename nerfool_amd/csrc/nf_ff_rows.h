@@ -13,6 +13,7 @@
 #pragma once
 
 #include "nf_ff.h"
+#include "nf_ff_sides.h"
 
 template <typename T>
 struct FfRow;          // a step: 16 bytes a lane of each operand
@@ -84,9 +85,9 @@ struct FfRounds {
     }
 };
 
-template <typename T, int NT, bool GATED>
+template <typename T, int NT, bool GATED, bool SIDES>
 __global__ void __launch_bounds__(64 * ff_rows_most(NT)) k_ff_rows(const T* __restrict__ w0, const T* __restrict__ w1, const T* __restrict__ x, int M, int N, int K,
-                                                  T* __restrict__ out, float* __restrict__ g_save, float* __restrict__ u_save, int act) {
+                                                  T* __restrict__ out, float* __restrict__ g_save, float* __restrict__ u_save, int act, FfSides sides) {
     typedef FfRow<T> R;
     typedef typename R::V V;
     constexpr int NW = GATED ? 2 : 1, U = ff_rows_unit(NT, GATED), STEP = 4 * R::KV, UNIT = U * STEP;
@@ -153,9 +154,13 @@ __global__ void __launch_bounds__(64 * ff_rows_most(NT)) k_ff_rows(const T* __re
     __syncthreads();
     for (int t = wave; t < NT; t += waves) {
         const int m = t0 + 16 * t + r, nn = n0 + 4 * (lane >> 4);
-        const ff_f32x4 v = ff_rows_total(part, waves, FRAGS, t, lane);
+        ff_f32x4 v = ff_rows_total(part, waves, FRAGS, t, lane);
         ff_f32x4 u = v;
         if (GATED) u = ff_rows_total(part, waves, FRAGS, (NW - 1) * NT + t, lane);
+        if constexpr (SIDES) {          // (as a branch at run time it costs one token 47 -> 50 us)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = ff_side<T>(sides, m < M && nn + c < N, m, nn + c, v[c]);
+        }
         if (m >= M) continue;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -190,11 +195,11 @@ static inline int ff_rows_tokens(int M, int groups) {
     return groups >= 256 ? all : (all + (256 + groups - 1) / groups - 1) / ((256 + groups - 1) / groups);
 }
 
-template <typename T, int NT, bool GATED>
-int ff_rows_launch(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, hipStream_t st) {
+template <typename T, int NT, bool GATED, bool SIDES>
+int ff_rows_launch(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, const FfSides& sides, hipStream_t st) {
     const int groups = (N + 15) / 16, unit = ff_rows_unit(NT, GATED) * 4 * FfRow<T>::KV;
     const int waves = ff_rows_waves(groups, (K + unit - 1) / unit, ff_rows_most(NT));
-    hipLaunchKernelGGL((k_ff_rows<T, NT, GATED>), dim3(groups, (M + 16 * NT - 1) / (16 * NT)), dim3(64 * waves), (size_t)waves * (GATED ? 2 : 1) * NT * 1024, st, (const T*)w0, (const T*)w1,
-                       (const T*)x, M, N, K, (T*)out, g_save, u_save, act);
+    hipLaunchKernelGGL((k_ff_rows<T, NT, GATED, SIDES>), dim3(groups, (M + 16 * NT - 1) / (16 * NT)), dim3(64 * waves), (size_t)waves * (GATED ? 2 : 1) * NT * 1024, st, (const T*)w0, (const T*)w1,
+                       (const T*)x, M, N, K, (T*)out, g_save, u_save, act, sides);
     return 0;
 }

@@ -17,7 +17,7 @@
 
 // nf_gated_ff_narrow.hip
 bool ff_narrow_fits(int64_t rows, int dim, int hidden);
-int64_t ff_narrow_workspace_bytes(int dim, int hidden, int dtype, bool backward);
+int64_t ff_narrow_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, bool backward);
 int ff_narrow(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, int64_t rows, int dim, int hidden, int dtype, int act, void* out, void* workspace,
               hipStream_t st);
 
@@ -77,13 +77,18 @@ struct EpiPart {
     }
     __device__ __forceinline__ void gated(int, int, int, int, bool, const ff_f32x4&, const ff_f32x4&) const {}
 };
-template <typename T>
+template <typename T, bool SIDES>
 struct EpiGate {
     FfMid<T> h;
     float *g_save, *u_save;          // [M, F], nullable
     int64_t F;
     int act;
-    __device__ __forceinline__ void gated(int, int m, int n, int left, bool inside, const ff_f32x4& g, const ff_f32x4& u) const {
+    FfSides sides;
+    __device__ __forceinline__ void gated(int, int m, int n, int left, bool inside, ff_f32x4 g, const ff_f32x4& u) const {
+        if constexpr (SIDES) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) g[c] = ff_side<T>(sides, inside && c < left, m, n + c, g[c]);
+        }
         if (!inside) return;
         ff_f32x4 v;
         float a, slope;
@@ -372,7 +377,7 @@ template <typename T>
 struct FwdPlan {
     FfPacked<T> x, wg, wu, wd;
     FfMid<T> h;
-    float* parts;
+    float *parts, *norms;
     int64_t bytes;
     FwdPlan(char* base, int64_t M, int D, int F) {
         Carve ws{base};
@@ -382,6 +387,7 @@ struct FwdPlan {
         wd = pack_at<T>(ws, D, F);
         h = mid_at<T>(ws, M, ff_pad<T>(F));
         parts = (float*)ws.take(ff_part_bytes(FfElem<T>::NP == 3, M, D, ff_pad<T>(F)));
+        norms = (float*)ws.take((M + F) * 4);
         bytes = ws.used;
     }
 };
@@ -389,24 +395,35 @@ struct FwdPlan {
 // Up to this many rows the weights' bytes bound the block and k_ff_rows streams them; above, the tiles of k_ff_gemm read them once for more tokens.
 constexpr int FF_ROWS_MAX = 64;
 
-template <typename T, bool GATED>
-int few_rows(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, hipStream_t st) {
+// ... whose h begins the workspace
+int64_t ff_few_rows_h_bytes(int64_t M, int F, int value_bytes) { return (M * F * value_bytes + 255) / 256 * 256; }
+
+template <typename T, bool GATED, bool SIDES>
+int few_rows(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, const FfSides& sides, hipStream_t st) {
     switch (ff_rows_tokens(M, (N + 15) / 16)) {
-        case 1: return ff_rows_launch<T, 1, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
-        case 2: return ff_rows_launch<T, 2, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
-        case 3: return ff_rows_launch<T, 3, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
-        default: return ff_rows_launch<T, 4, GATED>(w0, w1, x, M, N, K, out, g_save, u_save, act, st);
+        case 1: return ff_rows_launch<T, 1, GATED, SIDES>(w0, w1, x, M, N, K, out, g_save, u_save, act, sides, st);
+        case 2: return ff_rows_launch<T, 2, GATED, SIDES>(w0, w1, x, M, N, K, out, g_save, u_save, act, sides, st);
+        case 3: return ff_rows_launch<T, 3, GATED, SIDES>(w0, w1, x, M, N, K, out, g_save, u_save, act, sides, st);
+        default: return ff_rows_launch<T, 4, GATED, SIDES>(w0, w1, x, M, N, K, out, g_save, u_save, act, sides, st);
     }
 }
 
 template <typename T>
 int ff_fwd(const void* x, const void* wg, const void* wu, const void* wd, int M, int D, int F, int act, void* out, float* g_save, float* u_save,
            void* workspace, hipStream_t st) {
+    // relu's sides are asked for by a backward pass only
+    const bool border = act == FF_RELU && g_save;
+    FfSides sides = {};
     if (M <= FF_ROWS_MAX) {
-        FF_TRY((few_rows<T, true>(wg, wu, x, M, F, D, workspace, g_save, u_save, act, st)));
-        return few_rows<T, false>(wd, nullptr, workspace, M, D, F, out, nullptr, nullptr, 0, st);
+        if (border) {
+            sides = ff_sides<T>(x, wg, M, F, D, sizeof(T) == 4 ? D / 4 : D / 32, (float*)((char*)workspace + ff_few_rows_h_bytes(M, F, sizeof(T))), st);
+            FF_TRY((few_rows<T, true, true>(wg, wu, x, M, F, D, workspace, g_save, u_save, act, sides, st)));
+        } else
+            FF_TRY((few_rows<T, true, false>(wg, wu, x, M, F, D, workspace, g_save, u_save, act, sides, st)));
+        return few_rows<T, false, false>(wd, nullptr, workspace, M, D, F, out, nullptr, nullptr, 0, sides, st);
     }
     FwdPlan<T> f((char*)workspace, M, D, F);
+    if (border) sides = ff_sides<T>(x, wg, M, F, D, FfElem<T>::NP == 3 ? 6 * D / 32 : D / 32, f.norms, st);
     Packing<T> pack;
     pack.add(x, M, D, f.x);
     pack.add(wg, F, D, f.wg);
@@ -415,8 +432,9 @@ int ff_fwd(const void* x, const void* wg, const void* wu, const void* wd, int M,
     pack.run(st);
     FfOperand p = as_operand(f.wg.mid, F);
     p.b = (const uint16_t*)f.wu.mid.p;
-    const EpiGate<T> gate = {f.h, g_save, u_save, F, act};
-    FF_TRY((product<T, false, false, true>(p, as_operand(f.x.mid, M), M, F, (int)f.h.pitch, (int)f.x.mid.pitch, gate, st)));
+    const FfOperand q = as_operand(f.x.mid, M);
+    if (border) FF_TRY((product<T, false, false, true>(p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, true>{f.h, g_save, u_save, F, act, sides}, st)));
+    else FF_TRY((product<T, false, false, true>(p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, false>{f.h, g_save, u_save, F, act, sides}, st)));
     const EpiStore<T> store = {(T*)out, nullptr, D, M, 0x7fffffff};
     FF_TRY((product_split<T, false, false>(as_operand(f.wd.mid, D), as_operand(f.h, M), M, D, (int)f.h.pitch, store, f.parts, st)));
     return 0;
@@ -501,9 +519,9 @@ bool ff_sizes_ok(const char* what, int64_t M, int D, int F, int dtype, int act) 
 
 extern "C" int64_t nf_gated_ff_fwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype) {
     if (!ff_sizes_ok("nf_gated_ff_fwd_workspace_bytes", rows, dim, hidden, dtype, 0)) return -1;
-    if (rows <= FF_ROWS_MAX) return rows * hidden * (dtype == FF_F32 ? 4 : 2);          // h
+    if (rows <= FF_ROWS_MAX) return ff_few_rows_h_bytes(rows, hidden, dtype == FF_F32 ? 4 : 2) + (rows + hidden) * 4;
     const int64_t n = dtype == FF_F32 ? FwdPlan<float>(nullptr, rows, dim, hidden).bytes : FwdPlan<ff_bf16>(nullptr, rows, dim, hidden).bytes;
-    const int64_t narrow = ff_narrow_fits(rows, dim, hidden) ? ff_narrow_workspace_bytes(dim, hidden, dtype, false) : 0;
+    const int64_t narrow = ff_narrow_fits(rows, dim, hidden) ? ff_narrow_workspace_bytes(rows, dim, hidden, dtype, false) : 0;
     return n > narrow ? n : narrow;          // (which of the two runs depends on whether g and u are saved)
 }
 
@@ -526,7 +544,7 @@ extern "C" int nf_gated_ff_bwd_recomputes(int64_t rows, int dim, int hidden) { r
 
 extern "C" int64_t nf_gated_ff_bwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, int want_dx, int want_dw_gate_up, int want_dw_down) {
     if (!ff_sizes_ok("nf_gated_ff_bwd_workspace_bytes", rows, dim, hidden, dtype, 0)) return -1;
-    if (want_dx && !want_dw_gate_up && !want_dw_down && ff_narrow_fits(rows, dim, hidden)) return ff_narrow_workspace_bytes(dim, hidden, dtype, true);
+    if (want_dx && !want_dw_gate_up && !want_dw_down && ff_narrow_fits(rows, dim, hidden)) return ff_narrow_workspace_bytes(rows, dim, hidden, dtype, true);
     if (dtype == FF_F32) return BwdPlan<float>(nullptr, rows, dim, hidden, want_dx, want_dw_gate_up, want_dw_down).bytes;
     return BwdPlan<ff_bf16>(nullptr, rows, dim, hidden, want_dx, want_dw_gate_up, want_dw_down).bytes;
 }

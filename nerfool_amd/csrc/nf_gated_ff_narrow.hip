@@ -10,6 +10,7 @@
 // instructions of activation and split between them: 32768 x 64 x 256 float32 takes 30 us forward and 43
 // backward, and 5 each for the records (in separate products: 69 and 80; four waves of 32 tokens, one a SIMD: 47 and 67).
 #include "nf_ff_gemm.h"
+#include "nf_ff_sides.h"
 
 namespace {
 
@@ -106,9 +107,9 @@ struct Narrow {
     }
 };
 
-template <typename T, int KD, bool BWD>
-__global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, const T* __restrict__ dy, const char* __restrict__ records, int64_t M, int D, int chunks, int act,
-                                                   T* __restrict__ out) {
+template <typename T, int KD, bool BWD, bool SIDES>
+__global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, const T* __restrict__ dy, const char* __restrict__ records, int64_t M, int D, int F, int act,
+                                                   T* __restrict__ out, FfSides sides) {
     typedef Narrow<T, KD, BWD> N;
     typedef typename N::V V;
     constexpr int NP = N::NP, WAVES = 8;
@@ -126,6 +127,7 @@ __global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, cons
         N::row(x, m, M, D, 32 * k + 8 * q, xb[k]);
         if (BWD) N::row(dy, m, M, D, 32 * k + 8 * q, yb[BWD ? k : 0]);
     }
+    const int chunks = (F + 31) / 32;
     const ff_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     ff_f32x4 sum[2 * KD];
 #pragma unroll
@@ -143,6 +145,13 @@ __global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, cons
                 N::multiply(w, i * KD + k, lane, xb[k], g[i]);
                 N::multiply(w, (2 + i) * KD + k, lane, xb[k], u[i]);
                 if (BWD) N::multiply(w, (4 + i) * KD + k, lane, yb[BWD ? k : 0], dh[i]);
+            }
+        }
+        if constexpr (SIDES) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int f = 32 * c + 16 * (j / 4) + 4 * q + j % 4;
+                g[j / 4][j % 4] = ff_side<T>(sides, m < M && f < F, m, f, g[j / 4][j % 4]);
             }
         }
         V hb[NP], ub[NP];          // forward: h; backward: dg and du
@@ -173,30 +182,37 @@ __global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, cons
     for (int i = 0; i < 2 * KD; ++i) ff_put(out + m * D + 16 * i + 4 * q, D - (16 * i + 4 * q), sum[i]);
 }
 
-template <typename T, int KD, bool BWD>
+template <typename T, int KD, bool BWD, bool SIDES>
 int narrow_run(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, int64_t M, int D, int F, int act, void* out, void* workspace, hipStream_t st) {
     typedef Narrow<T, KD, BWD> N;
     constexpr int LDS = 2 * N::CHUNK;
     static bool set[NF_MAX_DEVICES];
     const int dev = nf_current_device();
     if (!set[dev]) {
-        const hipError_t e = hipFuncSetAttribute((const void*)k_ff_narrow<T, KD, BWD>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        const hipError_t e = hipFuncSetAttribute((const void*)k_ff_narrow<T, KD, BWD, SIDES>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) {
             nf_set_error("gated feed-forward: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
             return 2;
         }
         set[dev] = true;
     }
-    const int chunks = (F + 31) / 32, records = N::RECORDS * chunks;
+    const int records = N::RECORDS * ((F + 31) / 32);
+    FfSides sides = {};
+    if (SIDES) sides = ff_sides<T>(x, wg, M, F, D, N::NP == 3 ? 12 : 2, (float*)((char*)workspace + (int64_t)records * N::NP * 1024), st);
     hipLaunchKernelGGL((k_ff_narrow_pack<T>), dim3((records + 3) / 4), dim3(256), 0, st, (const T*)wg, (const T*)wu, (const T*)wd, D, F, KD, (int)BWD, (typename N::E*)workspace);
-    hipLaunchKernelGGL((k_ff_narrow<T, KD, BWD>), dim3((unsigned)((M + 127) / 128)), dim3(512), LDS, st, (const T*)x, (const T*)dy, (const char*)workspace, M, D, chunks, act,
-                       (T*)out);
+    hipLaunchKernelGGL((k_ff_narrow<T, KD, BWD, SIDES>), dim3((unsigned)((M + 127) / 128)), dim3(512), LDS, st, (const T*)x, (const T*)dy, (const char*)workspace, M, D, F, act,
+                       (T*)out, sides);
     return 0;
+}
+template <typename T, int KD>
+int narrow_way(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, int64_t M, int D, int F, int act, void* out, void* workspace, hipStream_t st) {
+    if (!dy) return narrow_run<T, KD, false, false>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st);
+    if (act == FF_RELU) return narrow_run<T, KD, true, true>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st);
+    return narrow_run<T, KD, true, false>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st);
 }
 template <typename T>
 int narrow_kd(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, int64_t M, int D, int F, int act, void* out, void* workspace, hipStream_t st) {
-    if (D <= 32) return dy ? narrow_run<T, 1, true>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st) : narrow_run<T, 1, false>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st);
-    return dy ? narrow_run<T, 2, true>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st) : narrow_run<T, 2, false>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st);
+    return D <= 32 ? narrow_way<T, 1>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st) : narrow_way<T, 2>(x, wg, wu, wd, dy, M, D, F, act, out, workspace, st);
 }
 
 }  // namespace
@@ -205,8 +221,8 @@ int narrow_kd(const void* x, const void* wg, const void* wu, const void* wd, con
 // A chunk takes 2 to 4 us, so 16 of them what the products' launches take at their smallest; from 16384 rows on half the CUs are busy here.
 bool ff_narrow_fits(int64_t rows, int dim, int hidden) { return dim <= 64 && (hidden <= 512 || rows >= 16384); }
 
-int64_t ff_narrow_workspace_bytes(int dim, int hidden, int dtype, bool backward) {
-    return (int64_t)((hidden + 31) / 32) * narrow_records(dim <= 32 ? 1 : 2, backward) * (dtype == FF_F32 ? 3 : 1) * 1024;
+int64_t ff_narrow_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, bool backward) {
+    return (int64_t)((hidden + 31) / 32) * narrow_records(dim <= 32 ? 1 : 2, backward) * (dtype == FF_F32 ? 3 : 1) * 1024 + (backward ? (rows + hidden) * 4 : 0);
 }
 
 // dy null: out = the block of x; else out = dx

@@ -75,8 +75,8 @@ def _product(a, ea, b, eb, parts):
     return a @ b, bound
 
 
-def gated(x, w_gate, w_up, w_down, name, dy=None, dtype=torch.float32):
-    """-> {name: (value, bound)}"""
+def gated(x, w_gate, w_up, w_down, name, dy=None, dtype=torch.float32, sides=False):
+    """-> {name: (value, bound)}; sides: relu's side of zero has to be the exact sum's, also where that is below what a float32 sum is off by"""
     parts = dtype == torch.float32
     x, wg, wu, wd = (t.double() for t in (x, w_gate, w_up, w_down))
     l1, l2 = LIPSCHITZ[name]
@@ -92,7 +92,7 @@ def gated(x, w_gate, w_up, w_down, name, dy=None, dtype=torch.float32):
         return got
     dy = dy.double()
     dh, edh = _product(dy, None, wd, None, parts)
-    es = l2 * eg + 16 * U * (1 + g.abs()) + ((g.abs() <= eg).double() if name == 'relu' else 0)
+    es = l2 * eg + 16 * U * (1 + g.abs()) + ((g.abs() <= eg).double() if name == 'relu' and not sides else 0)
     dg, du = dh * u * slope, dh * a
     edg = edh * (u.abs() + eu) * (slope.abs() + es) + dh.abs() * (eu * (slope.abs() + es) + u.abs() * es) + 4 * U * dg.abs()
     edu = edh * (a.abs() + ea) + dh.abs() * ea + 4 * U * du.abs()

@@ -96,6 +96,17 @@ static inline T __shfl_down(T v, unsigned d, int width = 64) { (void)width; int 
 template <typename T>
 static inline T __shfl(T v, int src, int width = 64) { (void)width; return hip_emu::exchange(v, src & 63); }
 
+static inline uint64_t __ballot(int pred) {
+    uint64_t* sl = hip_emu::wave_slots();
+    sl[hip_emu::lane()] = pred ? 1 : 0;
+    hip_emu::wave_barrier();
+    uint64_t got = 0;
+    for (int l = 0; l < 64; ++l) got |= sl[l] << l;
+    hip_emu::wave_barrier();
+    return got;
+}
+static inline int __ffsll(unsigned long long v) { return v ? __builtin_ctzll(v) + 1 : 0; }
+
 // data-parallel-primitive lane patterns (quad_perm 0x00-0xFF, row_half_mirror 0x141, row_mirror 0x140) and gfx950's
 // v_permlane32_swap, as used by nf_common.h
 static inline int __builtin_amdgcn_update_dpp(int, int src, int ctrl, int, int, bool) {

@@ -1,0 +1,57 @@
+"""The feed-forward operators where a value, a layout or a mode is at the edge of what a call may be: against float64 forms, on the GPU and (small
+cases) on the CPU stand-in build of the same kernel sources."""
+import pytest
+import torch
+
+from feed_forward_cases import BF16, F16, F32, near, normal
+from nerfool_amd.gnt import feed_forward as ff
+from oracle import feed_forward_ref as ref
+from test_feed_forward import emu  # noqa: F401  (a fixture)
+
+
+# ---- relu's side ----------------------------------------------------------------------------------------------------------------------
+def border_inputs(gen, rows, dim, hidden, dtype, device):
+    """x, w_gate with one unit a row whose exact sum is as near to zero as the type can say: the last columns of w_gate are 1, those of x the sum of the others in as many
+    parts of the type as hold 22 to 24 bits of it.  What is left is about 2^-24 of the sum, as large as what float32 sums are off by or smaller"""
+    parts = {F32: 1, BF16: 3, F16: 2}[dtype]
+    x = torch.randn(rows, dim, generator=gen).to(dtype)
+    w = (torch.randn(hidden, dim, generator=gen) * dim ** -0.5).to(dtype)
+    w[:, dim - parts:] = 1.0
+    rest = -(x[:, :dim - parts].double() * w[torch.arange(rows) % hidden, :dim - parts].double()).sum(1)
+    for c in range(dim - parts, dim):
+        x[:, c] = rest.to(dtype)
+        rest = rest - x[:, c].double()
+    return x.to(device), w.to(device)
+
+
+def check_relu_border(device, rows, dim, hidden, dtype, frozen):
+    gen = torch.Generator().manual_seed(23 + rows)
+    x, wg = border_inputs(gen, rows, dim, hidden, dtype, device)
+    wu, wd = (normal(gen, *s, dtype=dtype, device=device, scale=s[1] ** -0.5) for s in ((hidden, dim), (dim, hidden)))
+    dy = normal(gen, rows, dim, dtype=dtype, device=device)
+    g = x.double() @ wg.double().t()
+    at = torch.arange(rows, device=device)
+    assert (g[at, at % hidden].abs() <= 2.0 ** -20 * x.double().norm(dim=1) * wg.double().norm(dim=1)[at % hidden]).all()
+    want = ref.gated(x, wg, wu, wd, 'relu', dy, dtype, sides=True)
+    ws = [t.requires_grad_(not frozen) for t in (wg, wu, wd)]
+    out = ff.gated_feed_forward(x.requires_grad_(True), *ws, activation='relu')
+    near(out.detach(), want['out'], 'out')
+    for key, got in zip(('dx', 'dw_gate', 'dw_up', 'dw_down'), torch.autograd.grad(out, [x] if frozen else [x, *ws], dy)):
+        near(got, want[key], key)
+
+
+RELU_SMALL = [(5, 41, 24, F32, False), (40, 40, 33, BF16, False), (70, 37, 40, F32, False), (70, 43, 40, F16, False), (70, 40, 72, F32, True), (66, 64, 33, BF16, True),
+              (3, 20, 40, F16, True)]
+
+
+@pytest.mark.parametrize('rows,dim,hidden,dtype,frozen', RELU_SMALL)
+def test_relu_border_standin(emu, rows, dim, hidden, dtype, frozen):  # noqa: F811
+    check_relu_border(emu, rows, dim, hidden, dtype, frozen)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,dim,hidden,dtype,frozen', RELU_SMALL + [
+    (1, 1000, 300, BF16, False), (64, 515, 130, F32, False), (1500, 500, 1333, F32, False), (700, 1160, 520, F16, False), (2569, 1160, 2568, BF16, False),
+    (2569, 1160, 2568, F32, True), (4099, 64, 256, F32, True), (4099, 30, 100, F16, True)])
+def test_relu_border(rows, dim, hidden, dtype, frozen):
+    check_relu_border('cuda', rows, dim, hidden, dtype, frozen)
