@@ -28,9 +28,14 @@ import torch.nn as nn
 from .. import ops
 
 
-def _rows(t, name):
+def _last_axis(t, name):
     if t.dim() < 1 or not t.shape[-1]:
         raise ValueError('%s must have a last axis of at least one value (got the shape %s)' % (name, tuple(t.shape)))
+    return t
+
+
+def _rows(t, name):
+    _last_axis(t, name)
     return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])          # (a view is a node of its own in the backward pass)
 
 
@@ -44,6 +49,8 @@ def _first_only():
 
 
 class _RMSNorm(torch.autograd.Function):
+    # takes x and the residual in their own shapes: their gradient is one tensor, and a view between it and a leaf would hide from the leaf's accumulation that the other
+    # leaf has it too (both .grad would be one memory, and the next pass would add to it twice)
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         need = any(ctx.needs_input_grad[:3])
@@ -73,10 +80,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
     """x, residual [..., dim], weight [dim] -> y, or (y, h) with a residual: h = x + residual in the inputs' type, y from the sum before that rounding"""
     if residual is not None and residual.shape != x.shape:
         raise ValueError('residual has the shape %s, x %s' % (tuple(residual.shape), tuple(x.shape)))
-    got = _RMSNorm.apply(_rows(x, 'x'), weight, None if residual is None else _rows(residual, 'residual'), float(eps))
-    if residual is None:
-        return _as(got, x.shape)
-    return _as(got[0], x.shape), _as(got[1], x.shape)
+    return _RMSNorm.apply(_last_axis(x, 'x'), weight, residual, float(eps))
 
 
 def _no_gradient(what, tensors):

@@ -1011,10 +1011,11 @@ def ff_activation(name):
 
 
 def rms_norm_fwd(x, weight, residual, eps, quantize=False, want_rstd=False):
-    """x, residual [rows, dim], weight [dim] (residual, weight: or None) -> (h or None, y, rstd or None); quantize: y is (q, scale), float8_e4m3fn
-    [rows, dim] and float8_e8m0fnu [rows, ceil(dim / 32)]"""
+    """x, residual [..., dim], weight [dim] (residual, weight: or None) -> (h or None, y, rstd or None), h and y in x's shape, rstd [rows]; quantize: y is (q, scale),
+    float8_e4m3fn [rows, dim] and float8_e8m0fnu [rows, ceil(dim / 32)]"""
     x = _ff(x, 'x')
-    rows, dim = x.shape
+    dim = x.shape[-1]
+    rows = x.numel() // dim
     if residual is not None:
         residual = _ff_shape(_ff(residual, 'residual', x), x.shape, 'residual')
     if weight is not None:
@@ -1047,7 +1048,8 @@ def rms_norm_bwd(dy, dh, h, residual, weight, rstd, want_dweight):
         dh = _ff_shape(_ff(dh, 'dh', h), h.shape, 'dh')
     if weight is not None:
         weight = _ff(weight, 'weight', h)
-    rows, dim = h.shape
+    dim = h.shape[-1]
+    rows = h.numel() // dim
     dx = torch.empty_like(h)
     if rows == 0:
         return dx, torch.zeros(dim, dtype=h.dtype, device=h.device) if want_dweight else None

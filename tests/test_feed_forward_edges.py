@@ -55,3 +55,33 @@ def test_relu_border_standin(emu, rows, dim, hidden, dtype, frozen):  # noqa: F8
     (2569, 1160, 2568, F32, True), (4099, 64, 256, F32, True), (4099, 30, 100, F16, True)])
 def test_relu_border(rows, dim, hidden, dtype, frozen):
     check_relu_border('cuda', rows, dim, hidden, dtype, frozen)
+
+
+# ---- gradients that x and the residual share ----------------------------------------------------------------------------------------------
+def check_shared_gradient(device):
+    """leaves of any number of axes: two passes into .grad give twice the gradient, and neither leaf's .grad is the other's memory; the sum alone used, as well"""
+    gen = torch.Generator().manual_seed(29)
+    for shape in ((24,), (5, 24), (2, 3, 24), (2, 1, 3, 24)):
+        for use_y in (True, False):
+            x, r = (normal(gen, *shape, device=device).requires_grad_(True) for _ in range(2))
+            c = normal(gen, *shape, device=device)
+            for k in (1, 2, 3):
+                y, h = ff.rms_norm(x, None, r)
+                assert y.shape == h.shape == shape
+                (((y if use_y else h) * c).sum() + (h * h).sum()).backward()
+                if k == 1:
+                    once = x.grad.clone()
+                    want, = torch.autograd.grad(((ff.rms_norm(x, None, r)[0 if use_y else 1] * c).sum() + (ff.rms_norm(x, None, r)[1] ** 2).sum()), x)
+                    assert torch.allclose(once, want, rtol=2.0 ** -20, atol=2.0 ** -20)
+                assert x.grad.data_ptr() != r.grad.data_ptr()
+                # the passes are the same pass: k sums of one value, a rounding each
+                assert torch.allclose(x.grad, k * once, rtol=k * 2.0 ** -23, atol=0) and torch.equal(x.grad, r.grad)
+
+
+def test_shared_gradient_standin(emu):  # noqa: F811
+    check_shared_gradient(emu)
+
+
+@pytest.mark.gpu
+def test_shared_gradient():
+    check_shared_gradient('cuda')
