@@ -24,6 +24,7 @@ current stream; results do not depend on scheduling (no atomics).  In float32 an
 would be infinite: operands are split into parts, and the parts that are zero meet the infinity."""
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from .. import ops
 
@@ -41,6 +42,18 @@ def _rows(t, name):
 
 def _as(t, shape):
     return t if t.dim() == len(shape) else t.reshape(shape)
+
+
+def _differentiated(*tensors):
+    """whether the call is part of a gradient: decided here, as a Function's needs_input_grad says the same under no_grad, where nothing is to be kept.  (Forward mode goes through
+    the Function too, which refuses it.)"""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _first_only():
@@ -80,7 +93,11 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
     """x, residual [..., dim], weight [dim] -> y, or (y, h) with a residual: h = x + residual in the inputs' type, y from the sum before that rounding"""
     if residual is not None and residual.shape != x.shape:
         raise ValueError('residual has the shape %s, x %s' % (tuple(residual.shape), tuple(x.shape)))
-    return _RMSNorm.apply(_last_axis(x, 'x'), weight, residual, float(eps))
+    _last_axis(x, 'x')
+    if _differentiated(x, weight, residual):
+        return _RMSNorm.apply(x, weight, residual, float(eps))
+    h, y, _ = ops.rms_norm_fwd(x, weight, residual, eps)
+    return y if residual is None else (y, h)
 
 
 def _no_gradient(what, tensors):
@@ -127,7 +144,10 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation='silu'):
     """x [..., dim], w_gate, w_up [hidden, dim], w_down [dim, hidden] -> [..., dim]; activation: 'silu', 'gelu' (the error function), 'relu'.
     Constant weights (requires_grad False, as everywhere in an attack) cost no gradient of their own."""
     ops.ff_activation(activation)
-    return _as(_GatedFeedForward.apply(_rows(x, 'x'), w_gate, w_up, w_down, activation), x.shape)
+    rows = _rows(x, 'x')
+    if _differentiated(x, w_gate, w_up, w_down):
+        return _as(_GatedFeedForward.apply(rows, w_gate, w_up, w_down, activation), x.shape)
+    return _as(ops.gated_ff_fwd(rows, w_gate, w_up, w_down, activation)[0], x.shape)
 
 
 def gated_feed_forward_8bit(x, w_gate, w_up, w_down, activation='silu', dtype=torch.bfloat16):

@@ -85,3 +85,68 @@ def test_shared_gradient_standin(emu):  # noqa: F811
 @pytest.mark.gpu
 def test_shared_gradient():
     check_shared_gradient('cuda')
+
+
+# ---- calls that are no part of a gradient ---------------------------------------------------------------------------------------------------
+class no_requirement:
+    """nothing requires a gradient"""
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *_):
+        return False
+
+
+def check_nothing_kept(device, monkeypatch, rows, dim, hidden, dtype):
+    """modules (whose weights are Parameters) under no_grad and inference_mode, and constant weights under neither: the forward without what a backward pass reads"""
+    from nerfool_amd import ops
+    kept = []
+    gated, norm = ops.gated_ff_fwd, ops.rms_norm_fwd
+    monkeypatch.setattr(ops, 'gated_ff_fwd', lambda *a, save=False: (kept.append(save), gated(*a, save=save))[1])
+    monkeypatch.setattr(ops, 'rms_norm_fwd', lambda *a, want_rstd=False, **k: (kept.append(want_rstd), norm(*a, want_rstd=want_rstd, **k))[1])
+    gen = torch.Generator().manual_seed(31)
+    torch.manual_seed(5)
+    block, rms = ff.GatedFeedForward(dim, hidden, 'gelu').to(device).to(dtype), ff.RMSNorm(dim).to(device).to(dtype)
+    x, r = (normal(gen, rows, dim, dtype=dtype, device=device) for _ in range(2))
+    ws = [m.weight.detach() for m in (block.gate, block.up, block.down)]
+    with torch.no_grad():
+        want = ref.norm(x, rms.weight, r, 1e-6, dtype=dtype)
+    for mode in (torch.no_grad, torch.inference_mode, no_requirement):
+        with mode():
+            if mode is no_requirement:
+                block.requires_grad_(False), rms.requires_grad_(False)
+            y, h = rms(x, r)
+            out = block(y)
+            assert not out.requires_grad and not h.requires_grad and out.shape == x.shape
+            near(y, want['y'], 'y'), near(h, want['h'], 'h')
+            near(out, ref.gated(y, *ws, 'gelu', dtype=dtype)['out'], 'out')
+            assert rms(x).shape == x.shape
+    assert kept == [False] * 9
+    kept.clear()
+    block.requires_grad_(True)
+    block(rms(x)).float().sum().backward()
+    assert kept == [False, True] and block.gate.weight.grad is not None
+
+
+@pytest.mark.parametrize('rows,dim,hidden,dtype', [(70, 40, 33, F32), (3, 40, 33, BF16)])
+def test_nothing_kept_standin(emu, monkeypatch, rows, dim, hidden, dtype):  # noqa: F811
+    check_nothing_kept(emu, monkeypatch, rows, dim, hidden, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,dim,hidden,dtype', [(70, 40, 33, F32), (3, 40, 33, BF16), (300, 64, 256, F32), (1100, 520, 264, F16), (4100, 1160, 1288, BF16)])
+def test_nothing_kept(monkeypatch, rows, dim, hidden, dtype):
+    check_nothing_kept('cuda', monkeypatch, rows, dim, hidden, dtype)
+
+
+def test_forward_mode_is_refused(emu):  # noqa: F811
+    from torch.autograd import forward_ad
+    x = torch.randn(3, 16)
+    ws = [torch.randn(s) for s in ((8, 16), (8, 16), (16, 8))]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for f in (lambda t: ff.rms_norm(t), lambda t: ff.gated_feed_forward(t, *ws)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                f(dual)
+            with torch.no_grad():
+                f(x)
