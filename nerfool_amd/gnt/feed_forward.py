@@ -153,6 +153,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation='silu'):
 def gated_feed_forward_8bit(x, w_gate, w_up, w_down, activation='silu', dtype=torch.bfloat16):
     """`gated_feed_forward` on 8-bit pairs (q, scale), dim and hidden multiples of 32: x [..., dim] -> [..., dim] in dtype.  The product in the
     middle is brought to 8 bits by the same rule from its float32 values.  No backward pass."""
+    _no_gradient('gated_feed_forward_8bit', (*x, *w_gate, *w_up, *w_down))
     (q, scale), lead = x, x[0].shape[:-1]
     if scale.shape[:-1] != lead:
         raise ValueError("x: the scales' leading axes %s are not the values' %s" % (tuple(scale.shape[:-1]), tuple(lead)))

@@ -150,3 +150,14 @@ def test_forward_mode_is_refused(emu):  # noqa: F811
                 f(dual)
             with torch.no_grad():
                 f(x)
+
+
+def test_8bit_block_refuses_a_gradient(emu):  # noqa: F811
+    """a float8 tensor can require a gradient, and the block has none to give"""
+    pairs = [ff.quantize_8bit(torch.ones(s)) for s in ((4, 32), (64, 32), (64, 32), (32, 64))]
+    for i in range(4):
+        leaf = [(q.clone().requires_grad_(True), s) if j == i else (q, s) for j, (q, s) in enumerate(pairs)]
+        with pytest.raises(RuntimeError, match='gated_feed_forward_8bit has no backward pass'):
+            ff.gated_feed_forward_8bit(*leaf)
+        with torch.no_grad():
+            assert torch.equal(ff.gated_feed_forward_8bit(*leaf), ff.gated_feed_forward_8bit(*pairs))
