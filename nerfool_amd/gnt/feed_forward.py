@@ -70,9 +70,9 @@ class _RMSNorm(torch.autograd.Function):
         h, y, rstd = ops.rms_norm_fwd(x, weight, residual, eps, want_rstd=need)
         ctx.set_materialize_grads(False)
         if need:
-            # the gradient of the weight is a sum of dy * xhat over the rows: from h as rounded to 16 bits it would carry that rounding beside its own,
-            # so x and the residual are kept and added again; in float32, and for the gradient of x alone, h as stored is as good and half the reading
-            if h is None or (ctx.needs_input_grad[1] and x.dtype != torch.float32):
+            # from h as rounded to 16 bits both gradients would carry that rounding beside their own -- dx many times over where dy lies along xhat, which it subtracts -- so x and
+            # the residual are kept and added again; in float32 h as stored is their sum, and half the reading
+            if h is None or x.dtype != torch.float32:
                 ctx.save_for_backward(x, residual, weight, rstd)
             else:
                 ctx.save_for_backward(h, None, weight, rstd)

@@ -35,8 +35,8 @@ def act(name, g):
     return g.clamp(min=0), (g > 0).to(g.dtype)
 
 
-def norm(x, weight, residual, eps, dy=None, dh=None, dtype=torch.float32):
-    """-> {name: (value, bound)}; sums over a row are trees of at most 64 links plus the row's 16-byte vectors a thread"""
+def norm(x, weight, residual, eps, dy=None, dh=None, dtype=torch.float32, lost=None):
+    """-> {name: (value, bound)}; lost: what the h that the backward pass reads is off by, relative (None: a rounding to dtype); sums over a row are trees of at most 64 links plus the row's 16-byte vectors a thread"""
     x, r = x.double(), None if residual is None else residual.double()
     w = torch.ones(x.shape[1], dtype=torch.float64, device=x.device) if weight is None else weight.double()
     h = x if r is None else x + r
@@ -49,7 +49,8 @@ def norm(x, weight, residual, eps, dy=None, dh=None, dtype=torch.float32):
     if dy is None:
         return got
     dy = dy.double()
-    lost = half_step(dtype) if r is not None else 0.0          # the backward pass reads h as it was stored
+    if lost is None:
+        lost = half_step(dtype) if r is not None else 0.0
     g = dy * w
     mean = (g * xhat).mean(1, keepdim=True)
     mean_abs = (g * xhat).abs().mean(1, keepdim=True)

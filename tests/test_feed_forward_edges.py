@@ -161,3 +161,62 @@ def test_8bit_block_refuses_a_gradient(emu):  # noqa: F811
             ff.gated_feed_forward_8bit(*leaf)
         with torch.no_grad():
             assert torch.equal(ff.gated_feed_forward_8bit(*leaf), ff.gated_feed_forward_8bit(*pairs))
+
+
+# ---- the norm's gradients are those of x + r, not of h as rounded to 16 bits ------------------------------------------------------------------
+def check_norm_from_the_sum(device, rows, dim, dtype):
+    """dy along xhat, where dx is a small difference of large values, and in the first column one sum x + r that a rounding moves by nearly half a step, for all rows alike; the
+    weight a constant (as in an attack) and not: the same dx"""
+    gen = torch.Generator().manual_seed(37 + rows)
+    x, r = (normal(gen, rows, dim, dtype=dtype, device=device) for _ in range(2))
+    eps = torch.finfo(dtype).eps
+    x[:, 0], r[:, 0] = 1.0, 0.4375 * eps
+    w = (1 + 0.2 * torch.randn(dim, generator=gen)).to(dtype).to(device)
+    h = x.double() + r.double()
+    xhat = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-5)
+    dy = (xhat / w.double()).to(dtype)
+    dh = torch.zeros_like(dy)
+    want = ref.norm(x, w, r, 1e-5, dy, dh, dtype, lost=0.0)
+    got = []
+    for trained in (False, True):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, r)] + [w.detach().clone().requires_grad_(trained)]
+        y, _ = ff.rms_norm(leaves[0], leaves[2], leaves[1], eps=1e-5)
+        got.append(torch.autograd.grad(y, leaves if trained else leaves[:2], dy))
+    near(got[0][0], want['dx'], 'dx, constant weight'), near(got[1][0], want['dx'], 'dx')
+    near(got[1][2], want['dweight'], 'dweight')
+    assert torch.equal(got[0][0], got[1][0])
+    # the bound is close enough to tell: dx of h as rounded is outside of it
+    assert ((ref.norm(h.to(dtype), w, None, 1e-5, dy, None, dtype)['dx'][0] - want['dx'][0]).abs() > want['dx'][1]).any()
+
+
+def check_dweight_from_the_sum(device, rows, dim, dtype):
+    """half of the columns hold sums that a rounding to the type moves by 7 / 16 of a step, all the same way: with the rounding of dweight itself some of them come out beyond
+    its half step if they are made from h as rounded"""
+    gen = torch.Generator().manual_seed(41 + rows)
+    x, r = (normal(gen, rows, dim, dtype=dtype, device=device) for _ in range(2))
+    eps = torch.finfo(dtype).eps
+    x[:, ::2] = (1 + eps * torch.arange((dim + 1) // 2).remainder(100)).to(dtype).to(device)
+    r[:, ::2] = 0.4375 * eps
+    w = torch.ones(dim, dtype=dtype, device=device).requires_grad_(True)
+    dy = torch.ones_like(x)
+    want = ref.norm(x, w.detach(), r, 1e-5, dy, torch.zeros_like(dy), dtype, lost=0.0)['dweight']
+    got, = torch.autograd.grad(ff.rms_norm(x, w, r, eps=1e-5)[0], w, dy)
+    near(got, want, 'dweight')
+    lost = ref.norm((x.double() + r.double()).to(dtype), w.detach(), None, 1e-5, dy, None, dtype)['dweight'][0]
+    assert ((lost.to(dtype).double() - want[0]).abs() > want[1]).any()
+
+
+SUMS_SMALL = [(1, 64, BF16), (9, 520, BF16), (3, 129, F16), (40, 24, BF16)]
+
+
+@pytest.mark.parametrize('rows,dim,dtype', SUMS_SMALL)
+def test_norm_from_the_sum_standin(emu, rows, dim, dtype):  # noqa: F811
+    check_norm_from_the_sum(emu, rows, dim, dtype)
+    check_dweight_from_the_sum(emu, rows, dim, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,dim,dtype', SUMS_SMALL + [(513, 520, BF16), (300, 4100, F16), (3, 40000, BF16)])
+def test_norm_from_the_sum(rows, dim, dtype):
+    check_norm_from_the_sum('cuda', rows, dim, dtype)
+    check_dweight_from_the_sum('cuda', rows, dim, dtype)
