@@ -172,3 +172,11 @@ __device__ __forceinline__ void ff_split3(float v, ff_bf16* part) {
     part[1] = (ff_bf16)mid;
     part[2] = (ff_bf16)(rest - mid);
 }
+
+// A float16 backward pass multiplies dg and du as float16 values, and with gradients as small as they are without a loss scale these fall among the subnormal ones: at dy = 1e-5 a
+// tenth of their bits.  They are linear in dy, so they are made of dy times a power of two and the results divided by it, exactly.  The largest |dy| goes to 2^-4 .. 2^-3: dg and du
+// may be 2^19 times as large as it, and are normal numbers down to 2^-11 of it.  Never below 1: larger gradients are as they were.
+__device__ __forceinline__ float ff_grad_scale(float top) {
+    const unsigned e = (__float_as_uint(top) >> 23) & 255u;
+    return top > 0.f && e < 123u ? __uint_as_float((250u - e) << 23) : 1.f;          // 2^(-4 - (e - 127)); zeros, infinities: 1
+}

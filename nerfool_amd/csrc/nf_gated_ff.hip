@@ -60,7 +60,9 @@ struct EpiStore {
     T *out, *out2;          // nullable
     int64_t pitch;
     int len, split_m;          // rows m < len go to out, rows m >= split_m to out2, at most len of them
-    __device__ __forceinline__ void plain(int, int m, int n, int left, bool inside, const ff_f32x4& v) const {
+    const float* scale;          // [1] times the values (float16 gradients), or null
+    __device__ __forceinline__ void plain(int, int m, int n, int left, bool inside, ff_f32x4 v) const {
+        if (std::is_same<T, ff_half>::value && scale) v *= scale[1];
         const bool second = m >= split_m;
         const int r = second ? m - split_m : m;
         T* o = second ? out2 : out;
@@ -111,8 +113,10 @@ struct EpiGateBwd {
     const float *g, *u;
     int64_t F, Fp;
     int act, want_h;
+    const float* scale;          // float16: [0] times dg and du
     __device__ __forceinline__ void plain(int, int m, int n, int left, bool inside, const ff_f32x4& dh) const {
         if (!inside) return;
+        const float s = std::is_same<T, ff_half>::value ? scale[0] : 1.f;
         ff_f32x4 gv = {0.f, 0.f, 0.f, 0.f}, uv = gv, dg, du, hv;
         const float *gp = g + m * F + n, *up = u + m * F + n;
         if (left >= 4) {
@@ -128,6 +132,7 @@ struct EpiGateBwd {
             hv[c] = a * uv[c];
             dg[c] = dh[c] * uv[c] * slope;
             du[c] = dh[c] * a;
+            if (std::is_same<T, ff_half>::value) dg[c] *= s, du[c] *= s;
         }
         dgu.put(m, n, left, dg);
         dgu.put(m, (int)Fp + n, left, du);
@@ -180,6 +185,33 @@ __global__ void __launch_bounds__(256) k_ff_pack(FfPackJobs<T> jobs) {
             for (int j = 0; j < 4; ++j) v[j] = j < left ? (float)s[j] : 0.f;
         job.dst.put(r, c, left > 0 ? left : 0, v);
     }
+}
+
+// ---- float16 gradients: the power of two by which dg and du are held (ff_grad_scale), of the largest |dy|.  Two launches: 4096 x 2048 x 8192 with all gradients 1244 -> 1273 us,
+//      40 x 2048 x 5504 149 -> 159
+constexpr int FF_SCALE_PARTS = 256;
+__global__ void __launch_bounds__(256) k_ff_grad_top(const ff_half* __restrict__ dy, int64_t n, float* __restrict__ part) {
+    constexpr int N = FfVec<ff_half>::N;
+    __shared__ float tops[4];
+    float top = 0.f;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N; i < n; i += (int64_t)gridDim.x * 256 * N) {
+        float v[N];
+        ff_load_row(dy + i, 0, n - i < N ? (int)(n - i) : N, v);
+#pragma unroll
+        for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(v[j]));
+    }
+    top = nf_wave_max(top);
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+}
+// out[0] = the scale, out[1] = 1 / it
+__global__ void __launch_bounds__(64) k_ff_grad_scale(const float* __restrict__ part, float* __restrict__ out) {
+    float top = 0.f;
+    for (int i = threadIdx.x; i < FF_SCALE_PARTS; i += 64) top = fmaxf(top, part[i]);
+    top = nf_wave_max(top);
+    const float s = ff_grad_scale(top);
+    if (threadIdx.x == 0) out[0] = s, out[1] = 1.f / s;
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------------
@@ -435,7 +467,7 @@ int ff_fwd(const void* x, const void* wg, const void* wu, const void* wd, int M,
     const FfOperand q = as_operand(f.x.mid, M);
     if (border) FF_TRY((product<T, false, false, true>(p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, true>{f.h, g_save, u_save, F, act, sides}, st)));
     else FF_TRY((product<T, false, false, true>(p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, false>{f.h, g_save, u_save, F, act, sides}, st)));
-    const EpiStore<T> store = {(T*)out, nullptr, D, M, 0x7fffffff};
+    const EpiStore<T> store = {(T*)out, nullptr, D, M, 0x7fffffff, nullptr};
     FF_TRY((product_split<T, false, false>(as_operand(f.wd.mid, D), as_operand(f.h, M), M, D, (int)f.h.pitch, store, f.parts, st)));
     return 0;
 }
@@ -445,6 +477,7 @@ struct BwdPlan {
     FfPacked<T> x, wg, wu, wd, dy;
     FfMid<T> dgu, h;
     float* parts;          // of one product at a time
+    float* scale;          // float16
     int64_t bytes;
     BwdPlan(char* base, int64_t M, int D, int F, bool dx, bool dwgu, bool dwd) {
         Carve ws{base};
@@ -466,6 +499,7 @@ struct BwdPlan {
             most = n > most ? n : most;
         }
         parts = (float*)ws.take(most);
+        scale = (float*)ws.take(sizeof(T) == 2 ? (2 + FF_SCALE_PARTS) * 4 : 0);
         bytes = ws.used;
     }
 };
@@ -486,22 +520,28 @@ int ff_bwd(const void* x, const void* wg, const void* wu, const void* wd, const 
     if (dwgu) pack.add(x, M, D, f.x);
     pack.run(st);
     // dh[m][f] = sum over d of dy[m][d] Wd[d][f]
-    const EpiGateBwd<T> gate = {f.dgu, f.h, g, u, F, Fp, act, dwd != nullptr};
+    const float* scale = nullptr;
+    if (std::is_same<T, ff_half>::value) {
+        hipLaunchKernelGGL(k_ff_grad_top, dim3(FF_SCALE_PARTS), dim3(256), 0, st, (const ff_half*)dy, (int64_t)M * D, f.scale + 2);
+        hipLaunchKernelGGL(k_ff_grad_scale, dim3(1), dim3(64), 0, st, (const float*)f.scale + 2, f.scale);
+        scale = f.scale;
+    }
+    const EpiGateBwd<T> gate = {f.dgu, f.h, g, u, F, Fp, act, dwd != nullptr, scale};
     FfOperand p = as_operand(f.wd.mid, (int)f.wd.mid.pitch);
     FF_TRY((product<T, true, false, false>(p, as_operand(f.dy.mid, M), M, F, Fp, D, gate, st)));
     if (dx) {          // dx[m][d] = sum over k of dgu[m][k] [Wg; zeros up to Fp; Wu][k][d]
         p = as_operand(f.wg.mid, (int)f.wg.mid.pitch);
         p.b = (const uint16_t*)f.wu.mid.p;
         p.len = F, p.seg = Fp;
-        const EpiStore<T> store = {(T*)dx, nullptr, D, M, 0x7fffffff};
+        const EpiStore<T> store = {(T*)dx, nullptr, D, M, 0x7fffffff, scale};
         FF_TRY((product_split<T, true, false>(p, as_operand(f.dgu, M), M, D, Fp + F, store, f.parts, st)));
     }
     if (dwgu) {          // [dWg; dWu][f][d] = sum over m of dgu[m][f] x[m][d]
-        const EpiStore<T> store = {(T*)dwg, (T*)dwu, D, F, Fp};
+        const EpiStore<T> store = {(T*)dwg, (T*)dwu, D, F, Fp, scale};
         FF_TRY((product_split<T, true, true>(as_operand(f.x.mid, (int)f.x.mid.pitch), as_operand(f.dgu, 2 * Fp), 2 * Fp, D, M, store, f.parts, st)));
     }
     if (dwd) {          // dWd[d][f] = sum over m of dy[m][d] h[m][f]
-        const EpiStore<T> store = {(T*)dwd, nullptr, F, D, 0x7fffffff};
+        const EpiStore<T> store = {(T*)dwd, nullptr, F, D, 0x7fffffff, nullptr};
         FF_TRY((product_split<T, true, true>(as_operand(f.h, Fp), as_operand(f.dy.mid, (int)f.dy.mid.pitch), D, F, M, store, f.parts, st)));
     }
     return 0;

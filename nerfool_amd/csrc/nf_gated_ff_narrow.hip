@@ -127,6 +127,17 @@ __global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, cons
         N::row(x, m, M, D, 32 * k + 8 * q, xb[k]);
         if (BWD) N::row(dy, m, M, D, 32 * k + 8 * q, yb[BWD ? k : 0]);
     }
+    float scale = 1.f;          // float16: of the token's dg and du (ff_grad_scale; its dy lies on 4 lanes)
+    if constexpr (BWD && std::is_same<T, ff_half>::value) {
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < KD; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf((float)yb[k][0][j]));
+        top = fmaxf(top, __shfl_xor(top, 16, NF_WAVE));
+        top = fmaxf(top, __shfl_xor(top, 32, NF_WAVE));
+        scale = ff_grad_scale(top);
+    }
     const int chunks = (F + 31) / 32;
     const ff_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     ff_f32x4 sum[2 * KD];
@@ -165,6 +176,7 @@ __global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, cons
                 const float d = dh[j / 4][j % 4];
                 v[j] = d * uv * slope;
                 v2[j] = d * a;
+                if (std::is_same<T, ff_half>::value) v[j] *= scale, v2[j] *= scale;
             } else
                 v[j] = a * uv;
         }
@@ -179,7 +191,10 @@ __global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, cons
     ff_dma_barrier<0>();          // no load may land in LDS that the workgroup has given back
     if (m >= M) return;
 #pragma unroll
-    for (int i = 0; i < 2 * KD; ++i) ff_put(out + m * D + 16 * i + 4 * q, D - (16 * i + 4 * q), sum[i]);
+    for (int i = 0; i < 2 * KD; ++i) {
+        if (BWD && std::is_same<T, ff_half>::value) sum[i] *= 1.f / scale;
+        ff_put(out + m * D + 16 * i + 4 * q, D - (16 * i + 4 * q), sum[i]);
+    }
 }
 
 template <typename T, int KD, bool BWD, bool SIDES>

@@ -14,7 +14,8 @@ Both have a backward pass, and no second one: backward() and grad() with create_
 An 8-bit tensor is a pair: the values, float8_e4m3fn [..., n], and the scales, float8_e8m0fnu [..., ceil(n / 32)] -- 32 consecutive values of the
 last axis share a power of two, the least 2^e with max|block| <= 448 * 2^e.  A block that holds an infinity or a NaN is NaN as a whole.
 
-In float16 and bfloat16 the product in the middle, and its gradients, are rounded to that type (in float16: infinite beyond 65504); sums are float32.  relu's gradient takes the side of zero on which the
+In float16 and bfloat16 the product in the middle, and its gradients, are rounded to that type (in float16: infinite beyond 65504, the gradients
+held times a power of two that keeps those of a small dy from the subnormal values); sums are float32.  relu's gradient takes the side of zero on which the
 exact sum x Wg^T lies: one that a float32 sum cannot tell from zero is summed again in double.  Where weights need
 gradients, or dim is above 64, the forward keeps x Wg^T and x Wu^T in float32 for the backward pass; for constant weights at dim <= 64 nothing is kept (rows and hidden
 permitting: `ops.gated_ff_bwd_recomputes`).

@@ -20,9 +20,9 @@ def floor_step(dtype):
     return 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
 
 
-def rounded(value, bound, dtype):
-    """value +- bound, rounded to dtype"""
-    return bound + half_step(dtype) * (value.abs() + bound) + floor_step(dtype)
+def rounded(value, bound, dtype, scale=1.0):
+    """value +- bound, rounded to dtype, as held times `scale`"""
+    return bound + half_step(dtype) * (value.abs() + bound) + floor_step(dtype) / scale
 
 
 def act(name, g):
@@ -76,8 +76,9 @@ def _product(a, ea, b, eb, parts):
     return a @ b, bound
 
 
-def gated(x, w_gate, w_up, w_down, name, dy=None, dtype=torch.float32, sides=False):
-    """-> {name: (value, bound)}; sides: relu's side of zero has to be the exact sum's, also where that is below what a float32 sum is off by"""
+def gated(x, w_gate, w_up, w_down, name, dy=None, dtype=torch.float32, sides=False, scale=1.0):
+    """-> {name: (value, bound)}; sides: relu's side of zero has to be the exact sum's, also where that is below what a float32 sum is off by;
+    scale: dg and du have to be held times at least that"""
     parts = dtype == torch.float32
     x, wg, wu, wd = (t.double() for t in (x, w_gate, w_up, w_down))
     l1, l2 = LIPSCHITZ[name]
@@ -97,7 +98,7 @@ def gated(x, w_gate, w_up, w_down, name, dy=None, dtype=torch.float32, sides=Fal
     dg, du = dh * u * slope, dh * a
     edg = edh * (u.abs() + eu) * (slope.abs() + es) + dh.abs() * (eu * (slope.abs() + es) + u.abs() * es) + 4 * U * dg.abs()
     edu = edh * (a.abs() + ea) + dh.abs() * ea + 4 * U * du.abs()
-    edg, edu = rounded(dg, edg, dtype), rounded(du, edu, dtype)
+    edg, edu = rounded(dg, edg, dtype, scale), rounded(du, edu, dtype, scale)
     v1, b1 = _product(torch.cat([dg, du], 1), torch.cat([edg, edu], 1), torch.cat([wg, wu], 0), None, parts)
     got['dx'] = (v1, rounded(v1, b1, dtype))
     for key, (d, e), other in (('dw_gate', (dg, edg), x), ('dw_up', (du, edu), x)):

@@ -220,3 +220,31 @@ def test_norm_from_the_sum_standin(emu, rows, dim, dtype):  # noqa: F811
 def test_norm_from_the_sum(rows, dim, dtype):
     check_norm_from_the_sum('cuda', rows, dim, dtype)
     check_dweight_from_the_sum('cuda', rows, dim, dtype)
+
+
+# ---- float16 gradients without a loss scale ------------------------------------------------------------------------------------------------------
+def check_small_gradients(device, rows, dim, hidden, frozen, size):
+    """dy of `size`: dg and du have to be held as well as those of a larger dy, whatever the results are rounded to.  Where all rows are alike in size, of the power of two
+    that brings the largest |dy| to 2^-4, half of it (a row's own largest may decide)"""
+    gen = torch.Generator().manual_seed(43 + rows)
+    x = normal(gen, rows, dim, dtype=F16, device=device).requires_grad_(True)
+    ws = [normal(gen, *s, dtype=F16, device=device, scale=s[1] ** -0.5).requires_grad_(not frozen) for s in ((hidden, dim), (hidden, dim), (dim, hidden))]
+    dy = normal(gen, rows, dim, dtype=F16, device=device, scale=size)
+    for dy in (dy, dy * 2.0 ** 6):
+        want = ref.gated(x.detach(), *(w.detach() for w in ws), 'silu', dy, F16, scale=max(1.0, 2.0 ** -5 / float(dy.abs().max())))
+        for key, g in zip(('dx', 'dw_gate', 'dw_up', 'dw_down'), torch.autograd.grad(ff.gated_feed_forward(x, *ws), [x] if frozen else [x, *ws], dy)):
+            near(g, want[key], key)
+
+
+SMALL_DY = [(70, 72, 40, False, 1e-5), (130, 80, 24, False, 2e-6), (70, 40, 72, True, 1e-5), (20, 24, 40, True, 1e-6), (5, 72, 33, False, 1e-4), (66, 72, 33, False, 10.0)]
+
+
+@pytest.mark.parametrize('rows,dim,hidden,frozen,size', SMALL_DY)
+def test_small_gradients_standin(emu, rows, dim, hidden, frozen, size):  # noqa: F811
+    check_small_gradients(emu, rows, dim, hidden, frozen, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,dim,hidden,frozen,size', SMALL_DY + [(1025, 520, 260, False, 1e-5), (2569, 1160, 1288, False, 1e-5), (4097, 64, 256, True, 1e-5)])
+def test_small_gradients(rows, dim, hidden, frozen, size):
+    check_small_gradients('cuda', rows, dim, hidden, frozen, size)
