@@ -441,17 +441,26 @@ const uint8_t* padded_scales(const uint8_t* src, int64_t rows, int blocks, int64
     return to;
 }
 
+bool sizes_ok8(const char* what, int64_t rows, int dim, int hidden, int out_dtype, int activation) {
+    if (rows >= 1 && rows <= (1 << 30) && dim >= 32 && hidden >= 32 && dim % 32 == 0 && hidden % 32 == 0 && dim <= (1 << 20) && hidden <= (1 << 20) && out_dtype >= FF_F32 &&
+        out_dtype <= FF_F16 && activation >= FF_SILU && activation <= FF_RELU)
+        return true;
+    nf_set_error("%s: need 1 <= rows <= 2^30, dim and hidden multiples of 32 up to 2^20, dtype and activation in 0 .. 2 (got rows %lld dim %d hidden %d dtype %d activation %d)", what,
+                 (long long)rows, dim, hidden, out_dtype, activation);
+    return false;
+}
+
 }  // namespace
 
-extern "C" int64_t nf_gated_ff_fwd_8bit_workspace_bytes(int64_t rows, int dim, int hidden) { return Plan8(nullptr, rows, dim, hidden).bytes; }
+extern "C" int64_t nf_gated_ff_fwd_8bit_workspace_bytes(int64_t rows, int dim, int hidden) {
+    if (!sizes_ok8("nf_gated_ff_fwd_8bit_workspace_bytes", rows, dim, hidden, 0, 0)) return -1;
+    return Plan8(nullptr, rows, dim, hidden).bytes;
+}
 
 extern "C" int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const void* w_gate, const uint8_t* gate_scale, const void* w_up,
                                     const uint8_t* up_scale, const void* w_down, const uint8_t* down_scale, int64_t rows, int dim, int hidden,
                                     int out_dtype, int activation, void* out, void* workspace, nf_stream_t stream) {
-    NF_REQUIRE(rows >= 1 && rows <= (1 << 30) && dim >= 32 && hidden >= 32 && dim % 32 == 0 && hidden % 32 == 0 && dim <= (1 << 20) &&
-                   hidden <= (1 << 20) && out_dtype >= FF_F32 && out_dtype <= FF_F16 && activation >= FF_SILU && activation <= FF_RELU,
-               "nf_gated_ff_fwd_8bit: need 1 <= rows <= 2^30, dim and hidden multiples of 32 up to 2^20, dtype and activation in 0 .. 2 (got rows %lld dim %d "
-               "hidden %d dtype %d activation %d)", (long long)rows, dim, hidden, out_dtype, activation);
+    if (!sizes_ok8("nf_gated_ff_fwd_8bit", rows, dim, hidden, out_dtype, activation)) return 1;
     hipStream_t st = (hipStream_t)stream;
     const int M = (int)rows, D = dim, F = hidden;
     const Plan8 f((uint8_t*)workspace, rows, dim, hidden);

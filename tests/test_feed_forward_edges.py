@@ -248,3 +248,12 @@ def test_small_gradients_standin(emu, rows, dim, hidden, frozen, size):  # noqa:
 @pytest.mark.parametrize('rows,dim,hidden,frozen,size', SMALL_DY + [(1025, 520, 260, False, 1e-5), (2569, 1160, 1288, False, 1e-5), (4097, 64, 256, True, 1e-5)])
 def test_small_gradients(rows, dim, hidden, frozen, size):
     check_small_gradients('cuda', rows, dim, hidden, frozen, size)
+
+
+def test_8bit_workspace_refuses_sizes(emu):  # noqa: F811
+    from nerfool_amd import _lib
+    L = _lib.lib()
+    for rows, dim, hidden in ((0, 32, 32), (-5, 32, 64), (2 ** 31, 32, 32), (1, 40, 32), (1, 32, 8), (1, 0, 32), (1, 32, 2 ** 21)):
+        assert L.nf_gated_ff_fwd_8bit_workspace_bytes(rows, dim, hidden) == -1, (rows, dim, hidden)
+        assert b'nf_gated_ff_fwd_8bit_workspace_bytes' in L.nf_last_error()
+    assert L.nf_gated_ff_fwd_8bit_workspace_bytes(1, 32, 32) > 0
