@@ -442,6 +442,9 @@ int nf_in_act_pad_bwd(const float* dy_padded, const float* d_extra, const float*
  *   nf_gated_ff_bwd_recomputes(rows, dim, hidden) is not 0 and dx alone is asked for, g and u are made again and may be NULL.
  * nf_gated_ff_fwd_8bit: the block on operands in the 8-bit form above (dim, hidden multiples of 32; scales [rows of the operand, k / 32] bytes); h in
  *   the middle is brought to that form from its float values; out in out_dtype.
+ * nf_gated_ff_form, nf_gated_ff_8bit_form: which form a product of the block takes at these sizes (no launch): 0 the one for few rows, else the edge of its tiles (128 or 256) in
+ *   the low 16 bits and above them the parts into which its sum is cut; -1 for sizes out of range.  product: 0 gate and up, 1 down, 2 dh, 3 dx, 4 dw_gate and dw_up, 5 dw_down (8
+ *   bits: 0 and 1).
  * workspace: as many bytes as the *_workspace_bytes call of the same sizes says (-1: sizes out of range), 256-byte aligned.
  * ---------------------------------------------------------------------------------------------------------------- */
 int nf_rms_norm_fwd(const void* x, const void* residual, const void* weight, int64_t rows, int dim, int dtype, float eps, void* h, void* y,
@@ -458,6 +461,8 @@ int64_t nf_gated_ff_bwd_workspace_bytes(int64_t rows, int dim, int hidden, int d
 int nf_gated_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* dy, const float* g, const float* u,
                     int64_t rows, int dim, int hidden, int dtype, int activation, void* dx, void* dw_gate, void* dw_up, void* dw_down,
                     void* workspace, nf_stream_t stream);
+int nf_gated_ff_form(int64_t rows, int dim, int hidden, int dtype, int product);
+int nf_gated_ff_8bit_form(int64_t rows, int dim, int hidden, int product);
 int64_t nf_gated_ff_fwd_8bit_workspace_bytes(int64_t rows, int dim, int hidden);
 int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const void* w_gate, const uint8_t* gate_scale, const void* w_up,
                          const uint8_t* up_scale, const void* w_down, const uint8_t* down_scale, int64_t rows, int dim, int hidden, int out_dtype,

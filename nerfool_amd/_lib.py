@@ -132,6 +132,8 @@ _PROTOTYPES = {
     'nf_gated_ff_bwd_recomputes': (c_int, [c_int64, c_int, c_int]),
     'nf_gated_ff_bwd_workspace_bytes': (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int]),
     'nf_gated_ff_bwd': (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P]),
+    'nf_gated_ff_form': (c_int, [c_int64, c_int, c_int, c_int, c_int]),
+    'nf_gated_ff_8bit_form': (c_int, [c_int64, c_int, c_int, c_int]),
     'nf_gated_ff_fwd_8bit_workspace_bytes': (c_int64, [c_int64, c_int, c_int]),
     'nf_gated_ff_fwd_8bit': (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, _P, _P, _P]),
     'nf_pgd_sign_step': (c_int, [_P, _P, _P, c_int64, c_float, c_float, c_float, c_float, _P]),

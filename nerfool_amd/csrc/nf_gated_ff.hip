@@ -364,14 +364,27 @@ FfChoice ff_choose(bool three, int64_t M, int64_t N, int64_t K, bool may_split) 
     return best;
 }
 int64_t pad4(int64_t n) { return (n + 3) / 4 * 4; }
-// bytes of the parts of a product that may be split
-int64_t ff_part_bytes(bool three, int64_t M, int64_t N, int64_t K) {
-    const FfChoice c = ff_choose(three, M, N, K, true);
-    return c.parts > 1 ? c.parts * M * pad4(N) * 4 : 0;
+// ... of each product of the block
+enum { FF_GATE_UP, FF_DOWN, FF_DH, FF_DX, FF_DW_GATE_UP, FF_DW_DOWN };
+template <typename T>
+FfChoice ff_choice_of(int product, int64_t M, int64_t D, int64_t F) {
+    const bool three = FfElem<T>::NP == 3;
+    const int64_t Dp = ff_pad<T>(D), Fp = ff_pad<T>(F);
+    switch (product) {
+        case FF_GATE_UP: return ff_choose(three, M, 2 * F, Dp, false);
+        case FF_DOWN: return ff_choose(three, M, D, Fp, true);
+        case FF_DH: return ff_choose(three, M, F, D, false);
+        case FF_DX: return ff_choose(three, M, D, Fp + F, true);
+        case FF_DW_GATE_UP: return ff_choose(three, 2 * Fp, D, M, true);
+        default: return ff_choose(three, D, F, M, true);
+    }
 }
 
+// bytes of the parts
+int64_t ff_part_bytes(const FfChoice& c, int64_t M, int64_t N) { return c.parts > 1 ? c.parts * M * pad4(N) * 4 : 0; }
+
 template <typename T, bool PO, bool QO, bool GATED, typename Epi>
-int product_as(const FfChoice& c, const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
+int product(const FfChoice& c, const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
     typedef typename FfElem<T>::E E;
     if constexpr (FfElem<T>::NP == 3) {
         return launch<E, 3, 128, 128, 2, 4, 32, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
@@ -380,18 +393,12 @@ int product_as(const FfChoice& c, const FfOperand& p, const FfOperand& q, int M,
         return launch<E, 1, 128, 128, 2, 2, 64, PO, QO, GATED>(p, q, M, N, n_end, K, c.parts, epi, st);
     }
 }
-// the whole sum over k in one tile
-template <typename T, bool PO, bool QO, bool GATED, typename Epi>
-int product(const FfOperand& p, const FfOperand& q, int M, int N, int n_end, int K, const Epi& epi, hipStream_t st) {
-    return product_as<T, PO, QO, GATED>(ff_choose(FfElem<T>::NP == 3, M, GATED ? 2 * (int64_t)N : N, K, false), p, q, M, N, n_end, K, epi, st);
-}
-// ... or in parts: `parts` has room for ff_part_bytes
+// ... which may be in parts: `parts` has room for ff_part_bytes
 template <typename T, bool PO, bool QO>
-int product_split(const FfOperand& p, const FfOperand& q, int M, int N, int K, const EpiStore<T>& epi, float* parts, hipStream_t st) {
-    const FfChoice c = ff_choose(FfElem<T>::NP == 3, M, N, K, true);
-    if (c.parts == 1) return product_as<T, PO, QO, false>(c, p, q, M, N, N, K, epi, st);
+int product_split(const FfChoice& c, const FfOperand& p, const FfOperand& q, int M, int N, int K, const EpiStore<T>& epi, float* parts, hipStream_t st) {
+    if (c.parts == 1) return product<T, PO, QO, false>(c, p, q, M, N, N, K, epi, st);
     const EpiPart part = {parts, pad4(N), M * pad4(N)};
-    const int rc = product_as<T, PO, QO, false>(c, p, q, M, N, N, K, part, st);
+    const int rc = product<T, PO, QO, false>(c, p, q, M, N, N, K, part, st);
     if (rc) return rc;
     int64_t blocks = (M * (part.pitch / 4) + 255) / 256;
     if (blocks > 256 * 16) blocks = 256 * 16;
@@ -418,7 +425,7 @@ struct FwdPlan {
         wu = pack_at<T>(ws, F, D);
         wd = pack_at<T>(ws, D, F);
         h = mid_at<T>(ws, M, ff_pad<T>(F));
-        parts = (float*)ws.take(ff_part_bytes(FfElem<T>::NP == 3, M, D, ff_pad<T>(F)));
+        parts = (float*)ws.take(ff_part_bytes(ff_choice_of<T>(FF_DOWN, M, D, F), M, D));
         norms = (float*)ws.take((M + F) * 4);
         bytes = ws.used;
     }
@@ -465,10 +472,11 @@ int ff_fwd(const void* x, const void* wg, const void* wu, const void* wd, int M,
     FfOperand p = as_operand(f.wg.mid, F);
     p.b = (const uint16_t*)f.wu.mid.p;
     const FfOperand q = as_operand(f.x.mid, M);
-    if (border) FF_TRY((product<T, false, false, true>(p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, true>{f.h, g_save, u_save, F, act, sides}, st)));
-    else FF_TRY((product<T, false, false, true>(p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, false>{f.h, g_save, u_save, F, act, sides}, st)));
+    const FfChoice c = ff_choice_of<T>(FF_GATE_UP, M, D, F);
+    if (border) FF_TRY((product<T, false, false, true>(c, p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, true>{f.h, g_save, u_save, F, act, sides}, st)));
+    else FF_TRY((product<T, false, false, true>(c, p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, false>{f.h, g_save, u_save, F, act, sides}, st)));
     const EpiStore<T> store = {(T*)out, nullptr, D, M, 0x7fffffff, nullptr};
-    FF_TRY((product_split<T, false, false>(as_operand(f.wd.mid, D), as_operand(f.h, M), M, D, (int)f.h.pitch, store, f.parts, st)));
+    FF_TRY((product_split<T, false, false>(ff_choice_of<T>(FF_DOWN, M, D, F), as_operand(f.wd.mid, D), as_operand(f.h, M), M, D, (int)f.h.pitch, store, f.parts, st)));
     return 0;
 }
 
@@ -487,17 +495,14 @@ struct BwdPlan {
         if (dx) wg = pack_at<T>(ws, F, D), wu = pack_at<T>(ws, F, D);
         dgu = mid_at<T>(ws, M, 2 * ff_pad<T>(F));
         if (dwd) h = mid_at<T>(ws, M, ff_pad<T>(F));
-        const bool three = FfElem<T>::NP == 3;
         int64_t most = 0;
-        if (dx) most = ff_part_bytes(three, M, D, ff_pad<T>(F) + F);
-        if (dwgu) {
-            const int64_t n = ff_part_bytes(three, 2 * ff_pad<T>(F), D, M);
+        const auto room = [&](int product, int64_t rows, int64_t cols) {
+            const int64_t n = ff_part_bytes(ff_choice_of<T>(product, M, D, F), rows, cols);
             most = n > most ? n : most;
-        }
-        if (dwd) {
-            const int64_t n = ff_part_bytes(three, D, F, M);
-            most = n > most ? n : most;
-        }
+        };
+        if (dx) room(FF_DX, M, D);
+        if (dwgu) room(FF_DW_GATE_UP, 2 * ff_pad<T>(F), D);
+        if (dwd) room(FF_DW_DOWN, D, F);
         parts = (float*)ws.take(most);
         scale = (float*)ws.take(sizeof(T) == 2 ? (2 + FF_SCALE_PARTS) * 4 : 0);
         bytes = ws.used;
@@ -528,21 +533,23 @@ int ff_bwd(const void* x, const void* wg, const void* wu, const void* wd, const 
     }
     const EpiGateBwd<T> gate = {f.dgu, f.h, g, u, F, Fp, act, dwd != nullptr, scale};
     FfOperand p = as_operand(f.wd.mid, (int)f.wd.mid.pitch);
-    FF_TRY((product<T, true, false, false>(p, as_operand(f.dy.mid, M), M, F, Fp, D, gate, st)));
+    FF_TRY((product<T, true, false, false>(ff_choice_of<T>(FF_DH, M, D, F), p, as_operand(f.dy.mid, M), M, F, Fp, D, gate, st)));
     if (dx) {          // dx[m][d] = sum over k of dgu[m][k] [Wg; zeros up to Fp; Wu][k][d]
         p = as_operand(f.wg.mid, (int)f.wg.mid.pitch);
         p.b = (const uint16_t*)f.wu.mid.p;
         p.len = F, p.seg = Fp;
         const EpiStore<T> store = {(T*)dx, nullptr, D, M, 0x7fffffff, scale};
-        FF_TRY((product_split<T, true, false>(p, as_operand(f.dgu, M), M, D, Fp + F, store, f.parts, st)));
+        FF_TRY((product_split<T, true, false>(ff_choice_of<T>(FF_DX, M, D, F), p, as_operand(f.dgu, M), M, D, Fp + F, store, f.parts, st)));
     }
     if (dwgu) {          // [dWg; dWu][f][d] = sum over m of dgu[m][f] x[m][d]
         const EpiStore<T> store = {(T*)dwg, (T*)dwu, D, F, Fp, scale};
-        FF_TRY((product_split<T, true, true>(as_operand(f.x.mid, (int)f.x.mid.pitch), as_operand(f.dgu, 2 * Fp), 2 * Fp, D, M, store, f.parts, st)));
+        FF_TRY((product_split<T, true, true>(ff_choice_of<T>(FF_DW_GATE_UP, M, D, F), as_operand(f.x.mid, (int)f.x.mid.pitch), as_operand(f.dgu, 2 * Fp), 2 * Fp, D, M, store,
+                                                  f.parts, st)));
     }
     if (dwd) {          // dWd[d][f] = sum over m of dy[m][d] h[m][f]
         const EpiStore<T> store = {(T*)dwd, nullptr, F, D, 0x7fffffff, nullptr};
-        FF_TRY((product_split<T, true, true>(as_operand(f.h, Fp), as_operand(f.dy.mid, (int)f.dy.mid.pitch), D, F, M, store, f.parts, st)));
+        FF_TRY((product_split<T, true, true>(ff_choice_of<T>(FF_DW_DOWN, M, D, F), as_operand(f.h, Fp), as_operand(f.dy.mid, (int)f.dy.mid.pitch), D, F, M, store, f.parts,
+                                                  st)));
     }
     return 0;
 }
@@ -603,4 +610,15 @@ extern "C" int nf_gated_ff_bwd(const void* x, const void* w_gate, const void* w_
     FF_TRY(f(x, w_gate, w_up, w_down, dy, g, u, (int)rows, dim, hidden, activation, dx, dw_gate, dw_up, dw_down, workspace, (hipStream_t)stream));
     NF_LAUNCH_CHECK("nf_gated_ff_bwd");
     return 0;
+}
+
+extern "C" int nf_gated_ff_form(int64_t rows, int dim, int hidden, int dtype, int product) {
+    if (!ff_sizes_ok("nf_gated_ff_form", rows, dim, hidden, dtype, 0)) return -1;
+    if (product < 0 || product > 5) {
+        nf_set_error("nf_gated_ff_form: product in 0 .. 5 (got %d)", product);
+        return -1;
+    }
+    if (product <= FF_DOWN && rows <= FF_ROWS_MAX) return 0;
+    const FfChoice c = dtype == FF_F32 ? ff_choice_of<float>(product, rows, dim, hidden) : ff_choice_of<ff_bf16>(product, rows, dim, hidden);
+    return c.parts << 16 | (c.tile == TILE_256 ? 256 : 128);
 }

@@ -403,10 +403,10 @@ int launch8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const Ff
 }
 
 // tile: 256 x 256 where that gives most of the 256 CUs a tile, else 128 x 128
+bool big_tiles8(int64_t M, int64_t N) { return ((M + 255) / 256) * ((N + 255) / 256) >= 160; }
 template <bool GATED, bool EXACT, typename Epi>
 int product8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const FfScales& sq, int M, int N, int K, const Epi& epi, hipStream_t st) {
-    const int64_t big = (int64_t)((M + 255) / 256) * ((N * (GATED ? 2 : 1) + 255) / 256);
-    if (big >= 160) return launch8<256, 256, 2, 4, GATED, EXACT>(p, q, sp, sq, M, N, K, epi, st);
+    if (big_tiles8(M, N * (GATED ? 2 : 1))) return launch8<256, 256, 2, 4, GATED, EXACT>(p, q, sp, sq, M, N, K, epi, st);
     return launch8<128, 128, 2, 2, GATED, EXACT>(p, q, sp, sq, M, N, K, epi, st);
 }
 
@@ -488,4 +488,14 @@ extern "C" int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const
     if (rc) return rc;
     NF_LAUNCH_CHECK("nf_gated_ff_fwd_8bit");
     return 0;
+}
+
+extern "C" int nf_gated_ff_8bit_form(int64_t rows, int dim, int hidden, int product) {
+    if (!sizes_ok8("nf_gated_ff_8bit_form", rows, dim, hidden, 0, 0)) return -1;
+    if (product < 0 || product > 1) {
+        nf_set_error("nf_gated_ff_8bit_form: product 0 or 1 (got %d)", product);
+        return -1;
+    }
+    if (rows <= 64) return 0;
+    return 1 << 16 | (big_tiles8(rows, product ? dim : 2 * (int64_t)hidden) ? 256 : 128);
 }

@@ -3,7 +3,7 @@ cases) on the CPU stand-in build of the same kernel sources."""
 import pytest
 import torch
 
-from feed_forward_cases import BF16, F16, F32, near, normal, value_of
+from feed_forward_cases import BF16, F16, F32, check_gated, near, normal, value_of
 from nerfool_amd.gnt import feed_forward as ff
 from oracle import feed_forward_ref as ref
 from test_feed_forward import emu  # noqa: F401  (a fixture)
@@ -329,3 +329,42 @@ def test_8bit_tiles(rows, dim, hidden):
         check_8bit_exact_products('cuda', rows, dim, hidden, dtype)
     for act in ('silu', 'gelu', 'relu'):
         check_8bit_norm('cuda', rows, dim, hidden, act)
+
+
+# ---- every form of the largest tile ---------------------------------------------------------------------------------------------------------------
+GATE_UP, DOWN, DH, DX, DW_GATE_UP, DW_DOWN = range(6)
+# sizes, ragged each way, and the products that take 256 x 256 tiles there, with the sum in one part or in several
+LARGE = [((2569, 520, 4104), {GATE_UP: 1, DOWN: 7, DH: 1, DX: 7, DW_GATE_UP: 2}), ((4105, 2053, 264), {DOWN: 1, DX: 1}),
+         ((521, 2053, 4104), {DW_GATE_UP: 1, DW_DOWN: 1}), ((4105, 520, 2568), {GATE_UP: 1, DH: 1, DX: 5, DW_GATE_UP: 4, DW_DOWN: 7})]
+
+
+def form(rows, dim, hidden, dtype, product):
+    from nerfool_amd import _lib
+    f = _lib.lib().nf_gated_ff_form(rows, dim, hidden, {F32: 0, BF16: 1, F16: 2}[dtype], product)
+    return f & 0xffff, f >> 16
+
+
+def test_large_tiles_cover_every_form(emu):  # noqa: F811
+    for dtype in (BF16, F16):
+        reached = set()
+        for sizes, products in LARGE:
+            for product, parts in products.items():
+                assert form(*sizes, dtype, product) == (256, parts), (sizes, product)
+                reached.add((product, parts > 1))
+        assert reached == {(GATE_UP, False), (DH, False)} | {(p, split) for p in (DOWN, DX, DW_GATE_UP, DW_DOWN) for split in (False, True)}
+    assert form(64, 520, 4104, BF16, DOWN) == (0, 0) and form(64, 520, 4104, F32, DX)[0] == 128
+    from nerfool_amd import _lib
+    L = _lib.lib()
+    assert L.nf_gated_ff_8bit_form(4100, 2592, 288, 1) == L.nf_gated_ff_8bit_form(2569, 1184, 2592, 0) == 1 << 16 | 256
+    assert L.nf_gated_ff_8bit_form(64, 96, 160, 0) == 0 and L.nf_gated_ff_8bit_form(65, 96, 160, 0) == 1 << 16 | 128
+    for bad in ((0, 8, 8, 0, 0), (1, 8, 8, 3, 0), (1, 8, 8, 0, 6), (1, 8, 8, 0, -1)):
+        assert L.nf_gated_ff_form(*bad) == -1 and b'nf_gated_ff_form' in L.nf_last_error()
+    for bad in ((0, 32, 32, 0), (1, 40, 32, 0), (1, 32, 32, 2)):
+        assert L.nf_gated_ff_8bit_form(*bad) == -1 and b'nf_gated_ff_8bit_form' in L.nf_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('sizes', [s for s, _ in LARGE])
+def test_large_tiles(sizes, dtype):
+    check_gated(*sizes, dtype, 'cuda', act='silu')
