@@ -67,33 +67,29 @@ class _RMSNorm(torch.autograd.Function):
     # leaf has it too (both .grad would be one memory, and the next pass would add to it twice)
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        need = any(ctx.needs_input_grad[:3])
-        h, y, rstd = ops.rms_norm_fwd(x, weight, residual, eps, want_rstd=need)
+        h, y, rstd = ops.rms_norm_fwd(x, weight, residual, eps, want_rstd=True)
         ctx.set_materialize_grads(False)
-        if need:
-            # from h as rounded to 16 bits both gradients would carry that rounding beside their own -- dx many times over where dy lies along xhat, which it subtracts -- so x and
-            # the residual are kept and added again; in float32 h as stored is their sum, and half the reading
-            if h is None or x.dtype != torch.float32:
-                ctx.save_for_backward(x, residual, weight, rstd)
-            else:
-                ctx.save_for_backward(h, None, weight, rstd)
-        return (y, h) if h is not None else y
+        # from h as rounded to 16 bits both gradients would carry that rounding beside their own -- dx many times over where dy lies along xhat, which it subtracts -- so x and
+        # the residual are kept and added again; in float32 h as stored is their sum, and half the reading
+        if h is None or x.dtype != torch.float32:
+            ctx.save_for_backward(x, residual, weight, rstd)
+        else:
+            ctx.save_for_backward(h, None, weight, rstd)
+        return y if h is None else (y, h)
 
     @staticmethod
     def backward(ctx, dy, dh=None):
         _first_only()
+        need_x, need_w, need_r, _ = ctx.needs_input_grad
         h, residual, weight, rstd = ctx.saved_tensors
-        need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if dy is None:          # only the sum was used
             return (dh if need_x else None, torch.zeros_like(weight) if need_w else None, dh if need_r else None, None)
-        dx, dw = ops.rms_norm_bwd(dy, dh, h, residual, weight, rstd, need_w)
+        dx, dw = ops.rms_norm_bwd_saved(dy, dh, h, residual, weight, rstd, need_w)
         return dx if need_x else None, dw, dx if need_r else None, None
 
 
 def rms_norm(x, weight=None, residual=None, eps=1e-6):
     """x, residual [..., dim], weight [dim] -> y, or (y, h) with a residual: h = x + residual in the inputs' type, y from the sum before that rounding"""
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError('residual has the shape %s, x %s' % (tuple(residual.shape), tuple(x.shape)))
     _last_axis(x, 'x')
     if _differentiated(x, weight, residual):
         return _RMSNorm.apply(x, weight, residual, float(eps))

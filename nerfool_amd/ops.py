@@ -976,11 +976,11 @@ _FF_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FF_ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
 
 
-def _ff_launch(name, t, meta, *args):
-    """_launch, bracketed for a kernel timer only where one runs: the context manager costs a tenth of a one-token call"""
+def _ff_launch(name, t, sizes, *args):
+    """_launch, bracketed for a kernel timer only where one runs: the context manager costs a tenth of a one-token call.  sizes: rows, dim, hidden"""
     if prof._active is None:
         return _launch(getattr(_lib.lib(), name), name, t, *args)
-    with prof.launch(name, t, **meta):
+    with prof.launch(name, t, **dict(zip(('rows', 'dim', 'hidden'), sizes))):
         _launch(getattr(_lib.lib(), name), name, t, *args)
 
 
@@ -990,12 +990,25 @@ def _ff(t, name, like=None):
         raise TypeError('%s must be float32, bfloat16 or float16 (got %s)' % (name, t.dtype))
     if not t.is_cuda and not _lib.emulated():
         raise RuntimeError('%s is on %s: the nerfool_amd kernels run on the GPU only (no CPU fallback)' % (name, t.device))
-    if like is not None and t.dtype != like.dtype:
-        raise TypeError('%s is %s, but the call is in %s' % (name, t.dtype, like.dtype))
-    if like is not None and t.device != like.device:
-        raise ValueError('%s is on %s, but the call is on %s' % (name, t.device, like.device))
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if like is not None:
+        if t.dtype is not like.dtype:
+            raise TypeError('%s is %s, but the call is in %s' % (name, t.dtype, like.dtype))
+        if t.get_device() != like.get_device():
+            raise ValueError('%s is on %s, but the call is on %s' % (name, t.device, like.device))
+    return _ff_laid(t)
+
+
+def _ff_laid(t):
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
+def _ff_like(t, name, like):
+    """_ff of a tensor of the shape of `like`, which _ff has taken"""
+    if t.dtype is like.dtype and t.shape == like.shape and t.get_device() == like.get_device() and t.is_contiguous() and not t.data_ptr() & 15:
+        return t
+    return _ff_shape(_ff(t, name, like), like.shape, name)
 
 
 def _ff_shape(t, shape, name):
@@ -1016,20 +1029,21 @@ def rms_norm_fwd(x, weight, residual, eps, quantize=False, want_rstd=False):
     x = _ff(x, 'x')
     dim = x.shape[-1]
     rows = x.numel() // dim
+    h = rstd = y = q = scale = None
     if residual is not None:
-        residual = _ff_shape(_ff(residual, 'residual', x), x.shape, 'residual')
+        residual = _ff_like(residual, 'residual', x)
+        h = torch.empty_like(x)
     if weight is not None:
         weight = _ff_shape(_ff(weight, 'weight', x), (dim,), 'weight')
-    h = torch.empty_like(x) if residual is not None else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
-    y = q = scale = None
+    if want_rstd:
+        rstd = x.new_empty(rows, dtype=torch.float32)
     if quantize:
         q, scale = _empty_8bit(rows, dim, x.device)
     else:
         y = torch.empty_like(x)
     if rows:
-        _ff_launch('nf_rms_norm_fwd', x, dict(rows=rows, dim=dim), _ptr(x), _ptr(residual), _ptr(weight), rows, dim, _FF_DTYPES[x.dtype], float(eps),
-                    _ptr(h), _ptr(y), _ptr(q), _ptr(scale), _ptr(rstd))
+        _ff_launch('nf_rms_norm_fwd', x, (rows, dim), x.data_ptr(), _ptr(residual), _ptr(weight), rows, dim, _FF_DTYPES[x.dtype], float(eps),
+                   _ptr(h), _ptr(y), _ptr(q), _ptr(scale), _ptr(rstd))
     return h, (q, scale) if quantize else y, rstd
 
 
@@ -1042,24 +1056,44 @@ def rms_norm_bwd(dy, dh, h, residual, weight, rstd, want_dweight):
     """h: the sum as stored, or x with its residual (else None) -> (dx, dweight or None); dh: or None"""
     h = _ff(h, 'h')
     if residual is not None:
-        residual = _ff(residual, 'residual', h)
-    dy = _ff_shape(_ff(dy, 'dy', h), h.shape, 'dy')
-    if dh is not None:
-        dh = _ff_shape(_ff(dh, 'dh', h), h.shape, 'dh')
+        residual = _ff_shape(_ff(residual, 'residual', h), h.shape, 'residual')
     if weight is not None:
-        weight = _ff(weight, 'weight', h)
+        weight = _ff_shape(_ff(weight, 'weight', h), h.shape[-1:], 'weight')
+    return rms_norm_bwd_saved(dy, dh, h, residual, weight, rstd, want_dweight)
+
+
+def rms_norm_bwd_saved(dy, dh, h, residual, weight, rstd, want_dweight):
+    """rms_norm_bwd on operands that rms_norm_fwd has taken: they are not checked a second time, only laid out as there.  (A backward pass runs on a thread of its own, where each
+    object of the forward's thread that it looks at is a cache miss.)"""
+    h = _ff_laid(h)
+    if residual is not None:
+        residual = _ff_laid(residual)
+    if weight is not None:
+        weight = _ff_laid(weight)
+    dy = _ff_like(dy, 'dy', h)
+    if dh is not None:
+        dh = _ff_like(dh, 'dh', h)
     dim = h.shape[-1]
     rows = h.numel() // dim
     dx = torch.empty_like(h)
-    if rows == 0:
-        return dx, torch.zeros(dim, dtype=h.dtype, device=h.device) if want_dweight else None
     dw = ws = None
     if want_dweight:
-        dw = torch.empty(dim, dtype=h.dtype, device=h.device)
-        ws = torch.empty(_lib.lib().nf_rms_norm_bwd_workspace_floats(dim), dtype=torch.float32, device=h.device)
-    _ff_launch('nf_rms_norm_bwd', h, dict(rows=rows, dim=dim), _ptr(dy), _ptr(dh), _ptr(h), _ptr(residual), _ptr(weight), _ptr(rstd), rows, dim, _FF_DTYPES[h.dtype],
-                _ptr(dx), _ptr(dw), _ptr(ws))
+        dw = h.new_empty(dim) if rows else h.new_zeros(dim)
+        ws = h.new_empty(_rms_norm_bwd_floats(dim), dtype=torch.float32)
+    if rows:
+        _ff_launch('nf_rms_norm_bwd', h, (rows, dim), dy.data_ptr(), _ptr(dh), h.data_ptr(), _ptr(residual), _ptr(weight), rstd.data_ptr(), rows, dim, _FF_DTYPES[h.dtype],
+                   dx.data_ptr(), _ptr(dw), _ptr(ws))
     return dx, dw
+
+
+_rms_norm_floats = {}
+
+
+def _rms_norm_bwd_floats(dim):
+    n = _rms_norm_floats.get(dim)
+    if n is None:
+        n = _rms_norm_floats[dim] = _lib.lib().nf_rms_norm_bwd_workspace_floats(dim)
+    return n
 
 
 def quantize_8bit(x):
@@ -1068,7 +1102,7 @@ def quantize_8bit(x):
     rows, dim = x.shape
     q, scale = _empty_8bit(rows, dim, x.device)
     if rows:
-        _ff_launch('nf_quantize_8bit', x, dict(rows=rows, dim=dim), _ptr(x), rows, dim, _FF_DTYPES[x.dtype], _ptr(q), _ptr(scale))
+        _ff_launch('nf_quantize_8bit', x, (rows, dim), _ptr(x), rows, dim, _FF_DTYPES[x.dtype], _ptr(q), _ptr(scale))
     return q, scale
 
 
@@ -1092,7 +1126,7 @@ def gated_ff_fwd(x, w_gate, w_up, w_down, activation, save=False):
     if rows:
         L = _lib.lib()
         ws = _workspace_bytes(L.nf_gated_ff_fwd_workspace_bytes(rows, dim, hidden, _FF_DTYPES[x.dtype]), 'nf_gated_ff_fwd', x)
-        _ff_launch('nf_gated_ff_fwd', x, dict(rows=rows, dim=dim, hidden=hidden), _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), rows, dim, hidden, _FF_DTYPES[x.dtype], act,
+        _ff_launch('nf_gated_ff_fwd', x, (rows, dim, hidden), _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), rows, dim, hidden, _FF_DTYPES[x.dtype], act,
                     _ptr(out), _ptr(g), _ptr(u), _ptr(ws))
     return out, g, u
 
@@ -1121,7 +1155,7 @@ def gated_ff_bwd(x, w_gate, w_up, w_down, dy, g, u, activation, want):
         L = _lib.lib()
         ws = _workspace_bytes(L.nf_gated_ff_bwd_workspace_bytes(rows, dim, hidden, _FF_DTYPES[x.dtype], int(bool(want[0])), int(bool(want[1] or want[2])),
                                                                 int(bool(want[3]))), 'nf_gated_ff_bwd', x)
-        _ff_launch('nf_gated_ff_bwd', x, dict(rows=rows, dim=dim, hidden=hidden), _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(dy), _ptr(g), _ptr(u), rows, dim, hidden,
+        _ff_launch('nf_gated_ff_bwd', x, (rows, dim, hidden), _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(dy), _ptr(g), _ptr(u), rows, dim, hidden,
                     _FF_DTYPES[x.dtype], act, *[_ptr(t) for t in grads], _ptr(ws))
     return grads
 
@@ -1159,6 +1193,6 @@ def gated_ff_fwd_8bit(x, w_gate, w_up, w_down, activation, dtype):
     if rows:
         L = _lib.lib()
         ws = _workspace_bytes(L.nf_gated_ff_fwd_8bit_workspace_bytes(rows, dim, hidden), 'nf_gated_ff_fwd_8bit', out)
-        _ff_launch('nf_gated_ff_fwd_8bit', out, dict(rows=rows, dim=dim, hidden=hidden), *[_ptr(t) for pair in (x, w_gate, w_up, w_down) for t in pair], rows, dim, hidden,
+        _ff_launch('nf_gated_ff_fwd_8bit', out, (rows, dim, hidden), *[_ptr(t) for pair in (x, w_gate, w_up, w_down) for t in pair], rows, dim, hidden,
                     _FF_DTYPES[dtype], act, _ptr(out), _ptr(ws))
     return out
