@@ -1,7 +1,7 @@
 // The gated feed-forward block's products for few rows (new tokens): the weights, read once, are all that counts.
 //
-// out[m][n] = sum over k of X[m][k] W[n][k], m < 16 NT.  A workgroup owns 16 (in 8 bits 32) rows n of the weights -- gate and up rows of the same
-// features --, its waves take turns along k.  A lane loads 16 bytes of a weight row straight into the operand registers of a 16 x 16 matrix
+// out[m][n] = sum over k of X[m][k] W[n][k], m < 16 NT.  A workgroup owns 16 rows n of the weights (gated: gate and up rows of the same 16 features, in 8 bits of the 32
+// features of a block), its waves take turns along k.  A lane loads 16 bytes of a weight row straight into the operand registers of a 16 x 16 matrix
 // instruction (A: 16 weight rows, B: 16 tokens): lane l holds row l mod 16, k = V (l / 16) .. + V - 1 of each step, for both operands alike, so that any
 // order of k inside a step is right.  A wave keeps two units of 4 (2) steps in flight.  The waves' sums meet in LDS, in the order of the waves.
 // Rows may start at any element's address: nothing is padded or copied.
@@ -56,8 +56,8 @@ __device__ __forceinline__ typename FfRow<T>::V ff_row_load(const T* row, int k,
 
 // steps of a unit: two units are in flight in registers
 constexpr int ff_rows_unit(int nt, bool gated) { return gated && nt == 4 ? 2 : 4; }
-// most waves of a workgroup: 64 KB of LDS for their sums, and registers for the two units in flight
-constexpr int ff_rows_most(int nt) { return nt == 1 ? 16 : 8; }
+// most waves of a workgroup: 64 KB of LDS for their sums, and registers for the two units in flight (and for relu's sides)
+constexpr int ff_rows_most(int nt, bool sides) { return nt == 1 && !sides ? 16 : 8; }
 
 // the waves' sums of fragment f: part[wave][f][lane]
 __device__ __forceinline__ ff_f32x4 ff_rows_total(const ff_f32x4* part, int waves, int frags, int f, int lane) {
@@ -86,7 +86,7 @@ struct FfRounds {
 };
 
 template <typename T, int NT, bool GATED, bool SIDES>
-__global__ void __launch_bounds__(64 * ff_rows_most(NT)) k_ff_rows(const T* __restrict__ w0, const T* __restrict__ w1, const T* __restrict__ x, int M, int N, int K,
+__global__ void __launch_bounds__(64 * ff_rows_most(NT, SIDES)) k_ff_rows(const T* __restrict__ w0, const T* __restrict__ w1, const T* __restrict__ x, int M, int N, int K,
                                                   T* __restrict__ out, float* __restrict__ g_save, float* __restrict__ u_save, int act, FfSides sides) {
     typedef FfRow<T> R;
     typedef typename R::V V;
@@ -198,7 +198,7 @@ static inline int ff_rows_tokens(int M, int groups) {
 template <typename T, int NT, bool GATED, bool SIDES>
 int ff_rows_launch(const void* w0, const void* w1, const void* x, int M, int N, int K, void* out, float* g_save, float* u_save, int act, const FfSides& sides, hipStream_t st) {
     const int groups = (N + 15) / 16, unit = ff_rows_unit(NT, GATED) * 4 * FfRow<T>::KV;
-    const int waves = ff_rows_waves(groups, (K + unit - 1) / unit, ff_rows_most(NT));
+    const int waves = ff_rows_waves(groups, (K + unit - 1) / unit, ff_rows_most(NT, SIDES));
     hipLaunchKernelGGL((k_ff_rows<T, NT, GATED, SIDES>), dim3(groups, (M + 16 * NT - 1) / (16 * NT)), dim3(64 * waves), (size_t)waves * (GATED ? 2 : 1) * NT * 1024, st, (const T*)w0, (const T*)w1,
                        (const T*)x, M, N, K, (T*)out, g_save, u_save, act, sides);
     return 0;

@@ -19,6 +19,17 @@ struct FfSides {
     float scale;                // of |x| |w|
 };
 
+// N elements of a row from c on, zeros behind its end
+template <typename T>
+__device__ __forceinline__ typename FfVec<T>::V ff_side_load(const T* row, int c, int dim) {
+    constexpr int N = FfVec<T>::N;
+    if (c + N <= dim) return *reinterpret_cast<const typename FfVec<T>::V*>(row + c);
+    typename FfVec<T>::V v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = c + j < dim ? row[c + j] : (T)0.f;
+    return v;
+}
+
 // every lane of the wave calls this; `ask`: the lane has a unit (m, n) with the float32 sum g
 template <typename T>
 __device__ __forceinline__ float ff_side(const FfSides& s, bool ask, int64_t m, int64_t n, float g) {
@@ -33,11 +44,11 @@ __device__ __forceinline__ float ff_side(const FfSides& s, bool ask, int64_t m, 
         double sum = 0;
         constexpr int AHEAD = 4;          // loads under way together: the wave waits for these, not for the sums
         for (int c0 = lane * N; c0 < s.D; c0 += AHEAD * 64 * N) {
-            float a[AHEAD][N], b[AHEAD][N];
+            typename FfVec<T>::V a[AHEAD], b[AHEAD];          // (as loaded: converted they would take twice the registers)
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
-                ff_load_row(x, c0 + i * 64 * N, s.D, a[i]);
-                ff_load_row(w, c0 + i * 64 * N, s.D, b[i]);
+                a[i] = ff_side_load(x, c0 + i * 64 * N, s.D);
+                b[i] = ff_side_load(w, c0 + i * 64 * N, s.D);
             }
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
