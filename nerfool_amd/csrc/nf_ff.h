@@ -148,6 +148,7 @@ __device__ __forceinline__ void ff_act(int act, float g, float& a, float& slope)
         slope = g > 0.f ? 1.f : 0.f;
     }
 }
+
 // ---- stores of 4 consecutive values of a row (`left`: how many the row still has)
 template <typename T>
 __device__ __forceinline__ void ff_put(T* p, int left, const ff_f32x4& v) {
@@ -158,8 +159,8 @@ __device__ __forceinline__ void ff_put(T* p, int left, const ff_f32x4& v) {
         for (int c = 0; c < left; ++c) p[c] = (T)v[c];
     }
 }
-// the three bf16 parts of 4 floats.  The first is cut off, not rounded: near the largest float the rounded part would be infinite; the others are
-// rounded, which makes the third exact.  An infinity or a NaN keeps its value in the first part and zeros in the others.
+// the three bf16 parts of a float, each rounded, which makes the third exact.  Where the first would round to an infinity, near the largest float, it is cut off instead: the rest is
+// then positive and of 16 bits, and the other two hold it.  An infinity or a NaN keeps its value in the first part and zeros in the others.
 __device__ __forceinline__ void ff_split3(float v, ff_bf16* part) {
     const unsigned u = __float_as_uint(v);
     float hi = (float)(ff_bf16)v;

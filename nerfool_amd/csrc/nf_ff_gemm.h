@@ -16,6 +16,8 @@
 // P is the A operand of v_mfma_f32_16x16x32 (rows in registers), Q the B operand (columns on lanes): a lane ends with one m and 4 consecutive n.
 // The results go through LDS, 32 rows of every wave at a time, so that the output stage reads and writes whole rows: from the fragments directly a
 // wave's 16-byte accesses lie in 16 or 32 rows, and the stage of dh's product (g, u in, three tensors out) took twice the time of its 64 k steps.
+// The 256 x 256 form takes all 256 registers of its lanes; where an operand is k outermost (the backward pass) 2 to 6 of their load offsets wait in scratch memory and come back
+// between the products of each step.
 #pragma once
 
 #include <type_traits>

@@ -431,7 +431,9 @@ struct FwdPlan {
     }
 };
 
-// Up to this many rows the weights' bytes bound the block and k_ff_rows streams them; above, the tiles of k_ff_gemm read them once for more tokens.
+// Up to this many rows the weights' bytes bound the block and k_ff_rows streams them; above, the tiles of k_ff_gemm read them once for more tokens.  4096 x 8192 bf16, us: 16 rows
+// 50 (tiles 87), 48 rows 77 (90), 64 rows 88 (90), 65 rows 131 (90), 128 rows 169 (96); 2048 x 5504 float16: 32 rows 32 (40), 64 rows 45 (42), 65 rows 57 (42).  Short weights and
+// float32, whose tiles make six products, would bear more: 520 x 1032 bf16 64 rows 13 (20), 96 rows 14 (21), 128 rows 24 (23); 1024 x 4096 float32 64 rows 36 (87), 128 rows 61 (88).
 constexpr int FF_ROWS_MAX = 64;
 
 // ... whose h begins the workspace

@@ -1,6 +1,6 @@
 // The gated feed-forward block on 8-bit operands (e4m3 with a power-of-two scale per 32 values along k: nf_ff.h), forward only:
-// h = act(x Wg^T) * (x Wu^T) is brought to the same form in the output stage of its product -- 32 consecutive features of a row are one 32 x 32
-// block's rows, so that a block's maximum is a lane's 16 registers and one exchange -- and out = h Wd^T is made from it.
+// h = act(x Wg^T) * (x Wu^T) is brought to the same form in the output stage of its product -- there 8 neighbouring lanes hold the 32 features of a block of a row, so that its
+// maximum is three exchanges -- and out = h Wd^T is made from it.
 //
 // v_mfma_scale_f32_32x32x64_f8f6f4 multiplies the scales in: lane l holds row l mod 32, k = 16 (l / 32) .. + 15 and 32 + 16 (l / 32) .. + 15 of the
 // instruction's 64, and its scale operand is that of the row's block l / 32 (k 0 .. 31 or 32 .. 63).  A k step of the tile is 128 values: 128
@@ -13,7 +13,8 @@
 // v_mfma_f32_32x32x16_bf16: float32 sums, at half the rate; v_cvt_scalef32_pk_bf16_fp8 makes two operands of two values and their scale.
 //
 // 4096 x 4096 x 8192: gate and up 305 us (1.8 PFLOP/s), down 131 us (2.1; a library product of 8192^3 2.65): two waves a SIMD whose fragment reads wait in front of their
-// products -- put between them, as the 16-bit kernels do, they need more registers than there are.  4 x 4096 x 8192: 22 and 11 us, 3 TB/s of weights.
+// products -- put between them, as the 16-bit kernels do, they need more registers than there are (as it is, 2 and 5 of a lane's offsets wait in scratch memory and one or two come
+// back every step).  4 x 4096 x 8192: 22 and 11 us, 3 TB/s of weights.
 #include "nf_ff_gemm.h"
 #include "nf_ff_rows.h"
 
@@ -402,7 +403,8 @@ int launch8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const Ff
     return 0;
 }
 
-// tile: 256 x 256 where that gives most of the 256 CUs a tile, else 128 x 128
+// tile: 256 x 256 where that gives most of the 256 CUs a tile, else 128 x 128.  Rows x 4096 x 4096, gate and up on so many tiles of 256 (down half of them), us with 128 and 256: 128
+// tiles 80 and 106, 160 tiles 108 and 106, 256 tiles 138 and 120, 512 tiles 261 and 201; with bfloat16 operands 113 and 161, 155 and 162, 199 and 190, 383 and 330.
 bool big_tiles8(int64_t M, int64_t N) { return ((M + 255) / 256) * ((N + 255) / 256) >= 160; }
 template <bool GATED, bool EXACT, typename Epi>
 int product8(const FfOperand& p, const FfOperand& q, const FfScales& sp, const FfScales& sq, int M, int N, int K, const Epi& epi, hipStream_t st) {
@@ -464,6 +466,7 @@ extern "C" int nf_gated_ff_fwd_8bit(const void* x, const uint8_t* x_scale, const
     hipStream_t st = (hipStream_t)stream;
     const int M = (int)rows, D = dim, F = hidden;
     const Plan8 f((uint8_t*)workspace, rows, dim, hidden);
+    // few rows: as FF_ROWS_MAX (nf_gated_ff.hip); 4096 x 8192, us: 16 rows 36 (tiles 70), 64 rows 61 (73), 65 rows 95 (73), 128 rows 116 (78)
     if (M <= 64) {
         const FfScales spg = {gate_scale, up_scale, D / 32, F};
         few_rows8<true, float>(w_gate, w_up, spg, x, x_scale, M, F, D, nullptr, f.hq, f.hs, activation, st);

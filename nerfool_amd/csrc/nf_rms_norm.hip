@@ -357,7 +357,8 @@ int64_t rms_grid(int64_t rows, int rows_per_block, int64_t most) {
 
 // vectors of 16 bytes in a row -> threads a row and vectors a thread.  Up to 64 vectors the row is a part of a wave; up to 128 a wave owns it where there are 2048 rows
 // or more (8 waves a CU; the sums need no barrier), else, and above, a workgroup does: of 512 vectors a wave holds 240 registers and reads 8192 rows in 138 us,
-// a workgroup of four waves in 48.
+// a workgroup of four waves in 48.  The border of 2048 rows, of 125 vectors in bf16, us with a workgroup and a wave a row: forward 1024 rows 4.4 and 4.7, 1536 rows 5.1 and 5.1, 2048
+// rows 5.9 and 5.4, 8192 rows 14.5 and 11.7; backward 512 rows 8.7 and 8.6, 1024 rows 9.9 and 8.6, 2048 rows 12.2 and 10.2, 8192 rows 31.8 and 19.1.
 #define RMS_DISPATCH(VECS, ROWS, GO, LONG)          \
     do {                                            \
         const int nv_ = (VECS);                     \
