@@ -368,3 +368,85 @@ def test_large_tiles_cover_every_form(emu):  # noqa: F811
 @pytest.mark.parametrize('sizes', [s for s, _ in LARGE])
 def test_large_tiles(sizes, dtype):
     check_gated(*sizes, dtype, 'cuda', act='silu')
+
+
+# ---- graphs, and offsets beyond 32 bits ------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,dim,hidden,dtype,frozen', [(3, 72, 104, F16, False), (70, 192, 416, F16, False), (700, 192, 416, F32, False), (300, 64, 256, F16, True),
+                                                          (300, 64, 256, F32, True)])
+def test_relu_captured_into_a_graph(rows, dim, hidden, dtype, frozen):
+    """what relu and float16 add to a pass (row norms, sums in double, the gradients' power of two) is made anew by each replay: dy a thousand times smaller, units on the border"""
+    gen = torch.Generator().manual_seed(59)
+    x, wg = border_inputs(gen, rows, dim, hidden, dtype, 'cuda')
+    ws = [t.requires_grad_(not frozen) for t in (wg, *(normal(gen, *s, dtype=dtype, device='cuda', scale=s[1] ** -0.5) for s in ((hidden, dim), (dim, hidden))))]
+    x.requires_grad_(True)
+    dy = normal(gen, rows, dim, dtype=dtype, device='cuda')
+
+    def train():
+        out = ff.gated_feed_forward(x, *ws, activation='relu')
+        return (out, *torch.autograd.grad(out, [x] if frozen else [x, *ws], dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            train()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = train()
+    for k in range(4):
+        fresh, other = border_inputs(gen, rows, dim, hidden, dtype, 'cuda')
+        with torch.no_grad():
+            x.copy_(fresh), wg.copy_(other), dy.copy_(normal(gen, rows, dim, device='cuda', scale=1000.0 ** -(k % 2)))
+        want = [t.clone() for t in train()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), k
+
+
+def ends(rows, n=40):
+    return torch.cat([torch.arange(n), torch.arange(rows - n, rows)]).cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,dim,hidden,dtype,frozen,act', [(262300, 72, 8200, BF16, False, 'relu'), ((1 << 25) + 77, 64, 40, BF16, True, 'gelu')])
+def test_gated_offsets_beyond_32_bits(rows, dim, hidden, dtype, frozen, act):
+    """rows x hidden, or rows x dim, above 2^31 values: the first and the last rows"""
+    gen = torch.Generator(device='cuda').manual_seed(61)
+    x = torch.randn(rows, dim, generator=gen, device='cuda', dtype=dtype).requires_grad_(True)
+    dy = torch.randn(rows, dim, generator=gen, device='cuda', dtype=dtype)
+    ws = [(torch.randn(*s, generator=gen, device='cuda') * s[1] ** -0.5).to(dtype).requires_grad_(not frozen) for s in ((hidden, dim), (hidden, dim), (dim, hidden))]
+    out = ff.gated_feed_forward(x, *ws, activation=act)
+    grads = torch.autograd.grad(out, [x] if frozen else [x, *ws], dy)
+    at = ends(rows)
+    want = ref.gated(x.detach()[at], *(w.detach() for w in ws), act, dy[at], dtype, sides=True)
+    near(out.detach()[at], want['out'], 'out'), near(grads[0][at], want['dx'], 'dx')
+    if not frozen:          # the gradients of the weights are linear in dy: of the ends alone, the rest zero
+        dy.zero_()[at] = torch.randn(len(at), dim, generator=gen, device='cuda', dtype=dtype)
+        want = ref.gated(x.detach()[at], *(w.detach() for w in ws), act, dy[at], dtype, sides=True)
+        for key, got in zip(('dw_gate', 'dw_up', 'dw_down'), torch.autograd.grad(ff.gated_feed_forward(x, *ws, activation=act), ws, dy)):
+            near(got, want[key], key)
+
+
+@pytest.mark.gpu
+def test_norm_and_8bit_offsets_beyond_32_bits():
+    rows, dim = (1 << 20) + 77, 2080
+    gen = torch.Generator(device='cuda').manual_seed(67)
+    x, r, dy = (torch.randn(rows, dim, generator=gen, device='cuda', dtype=BF16) for _ in range(3))
+    at = ends(rows)
+    x.requires_grad_(True)
+    y, h = ff.rms_norm(x, None, r)
+    want = ref.norm(x.detach()[at], None, r[at], 1e-6, dy[at], torch.zeros_like(dy[at]), BF16, lost=0.0)
+    near(y.detach()[at], want['y'], 'y'), near(h.detach()[at], want['h'], 'h')
+    near(torch.autograd.grad(y, x, dy)[0][at], want['dx'], 'dx')
+    del y, h, dy
+    x = x.detach()
+    q, s, _ = ff.rms_norm_8bit(x, None, r)
+    small = ff.rms_norm_8bit(x[at], None, r[at])
+    assert torch.equal(q[at].view(torch.uint8), small[0].view(torch.uint8)) and torch.equal(s[at].view(torch.uint8), small[1].view(torch.uint8))
+    pairs = [ff.quantize_8bit(torch.randn(*n, generator=gen, device='cuda') * 0.02) for n in ((64, dim), (64, dim), (dim, 64))]
+    out = ff.gated_feed_forward_8bit((q, s), *pairs, dtype=BF16)
+    # (fewer rows may take another form, whose sums are in another order: the bound of check_8bit_norm)
+    small = ff.gated_feed_forward_8bit((q[torch.cat([at] * 4)], s[torch.cat([at] * 4)]), *pairs, dtype=BF16)[:len(at)].double()
+    assert float((out[at].double() - small).norm() / small.norm()) <= (2.0 ** -18 + 2.0 ** -13.5) ** 0.5
