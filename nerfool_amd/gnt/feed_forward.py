@@ -21,8 +21,10 @@ gradients, or dim is above 64, the forward keeps x Wg^T and x Wu^T in float32 fo
 permitting: `ops.gated_ff_bwd_recomputes`).
 
 Any number of leading axes; a call's tensors are of one type and on one device; tensors that are not contiguous are copied.  Work is enqueued on the
-current stream; results do not depend on scheduling (no atomics).  In float32 an infinity in an operand of a product gives NaN where the exact sum
-would be infinite: operands are split into parts, and the parts that are zero meet the infinity."""
+current stream; results do not depend on scheduling (no atomics).  A row's result may depend on how many rows the call has, as the order of its sums does, and on 8 bits with a
+bfloat16 result a little more: see `gated_feed_forward_8bit`.  In float32 with more than 64 rows (or, in a gradient, any number) an infinity in an operand of a product gives NaN
+where the exact sum would be infinite: operands are split into parts, and the parts that are zero, or of the other sign, meet the infinity.  (Up to 64 rows the forward multiplies
+float32 values as they are.)"""
 import torch
 import torch.nn as nn
 from torch.autograd import forward_ad
@@ -149,7 +151,11 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation='silu'):
 
 def gated_feed_forward_8bit(x, w_gate, w_up, w_down, activation='silu', dtype=torch.bfloat16):
     """`gated_feed_forward` on 8-bit pairs (q, scale), dim and hidden multiples of 32: x [..., dim] -> [..., dim] in dtype.  The product in the
-    middle is brought to 8 bits by the same rule from its float32 values.  No backward pass."""
+    middle is brought to 8 bits by the same rule from its float32 values.  No backward pass.
+
+    float32 and float16 results, and all results of up to 64 rows, are of exact products in float32 sums.  With more rows a bfloat16 result is of the matrix instruction's own 8-bit
+    products, which drops what lies below 2^-12 of the largest of 16, at twice the rate (0.0020 from the exact sums where rounding alone is 0.0017): dtype=torch.float32 and
+    .to(torch.bfloat16) has the exact ones."""
     _no_gradient('gated_feed_forward_8bit', (*x, *w_gate, *w_up, *w_down))
     (q, scale), lead = x, x[0].shape[:-1]
     if scale.shape[:-1] != lead:
