@@ -293,6 +293,16 @@ __device__ __forceinline__ void ff_output(float* lds, const Acc (&acc)[TP][TQ], 
     }
 }
 
+// what an output stage reads once a thread: epi.ready(), where it has that
+template <typename Epi>
+__device__ __forceinline__ auto ff_ready(const Epi& e, int) -> decltype(e.ready()) {
+    return e.ready();
+}
+template <typename Epi>
+__device__ __forceinline__ const Epi& ff_ready(const Epi& e, long) {
+    return e;
+}
+
 // tile BP (rows of P) x BQ (rows of Q), WP x WQ waves
 template <typename E, int NP, int BP, int BQ, int WP, int WQ, int BK, bool PO, bool QO, bool GATED, typename Epi>
 __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand q, FfShape s, Epi epi) {
@@ -405,5 +415,5 @@ __global__ void __launch_bounds__(WP* WQ * 64) k_ff_gemm(FfOperand p, FfOperand 
         for (; k0 < k_hi; k0 += BK) step(std::false_type(), k0);
     }
     ff_dma_barrier<0>();          // no load may land in LDS that the workgroup has given back
-    ff_output<BP, BQ, WP, WQ, GATED>(reinterpret_cast<float*>(lds), acc, s, m0, n0, part, epi);
+    ff_output<BP, BQ, WP, WQ, GATED>(reinterpret_cast<float*>(lds), acc, s, m0, n0, part, ff_ready(epi, 0));
 }

@@ -158,8 +158,7 @@ __global__ void __launch_bounds__(64 * ff_rows_most(NT, SIDES)) k_ff_rows(const 
         ff_f32x4 u = v;
         if (GATED) u = ff_rows_total(part, waves, FRAGS, (NW - 1) * NT + t, lane);
         if constexpr (SIDES) {          // (as a branch at run time it costs one token 47 -> 50 us)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = ff_side<T>(sides, m < M && nn + c < N, m, nn + c, v[c]);
+ff_sides_settle4<T>(sides, m < M && nn < N, m, nn, N - nn, v);
         }
         if (m >= M) continue;
 #pragma unroll

@@ -17,7 +17,7 @@
 
 // nf_gated_ff_narrow.hip
 bool ff_narrow_fits(int64_t rows, int dim, int hidden);
-int64_t ff_narrow_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, bool backward);
+int64_t ff_narrow_workspace_bytes(int dim, int hidden, int dtype, bool backward);
 int ff_narrow(const void* x, const void* wg, const void* wu, const void* wd, const void* dy, int64_t rows, int dim, int hidden, int dtype, int act, void* out, void* workspace,
               hipStream_t st);
 
@@ -61,8 +61,15 @@ struct EpiStore {
     int64_t pitch;
     int len, split_m;          // rows m < len go to out, rows m >= split_m to out2, at most len of them
     const float* scale;          // [1] times the values (float16 gradients), or null
+    float by;
+    // (read once a thread, not with every store)
+    __device__ __forceinline__ EpiStore ready() const {
+        EpiStore e = *this;
+        if (std::is_same<T, ff_half>::value) e.by = scale ? scale[1] : 1.f;
+        return e;
+    }
     __device__ __forceinline__ void plain(int, int m, int n, int left, bool inside, ff_f32x4 v) const {
-        if (std::is_same<T, ff_half>::value && scale) v *= scale[1];
+        if (std::is_same<T, ff_half>::value) v *= by;
         const bool second = m >= split_m;
         const int r = second ? m - split_m : m;
         T* o = second ? out2 : out;
@@ -87,10 +94,7 @@ struct EpiGate {
     int act;
     FfSides sides;
     __device__ __forceinline__ void gated(int, int m, int n, int left, bool inside, ff_f32x4 g, const ff_f32x4& u) const {
-        if constexpr (SIDES) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) g[c] = ff_side<T>(sides, inside && c < left, m, n + c, g[c]);
-        }
+        if constexpr (SIDES) ff_sides_settle4<T>(sides, inside, m, n, left, g);
         if (!inside) return;
         ff_f32x4 v;
         float a, slope;
@@ -114,9 +118,14 @@ struct EpiGateBwd {
     int64_t F, Fp;
     int act, want_h;
     const float* scale;          // float16: [0] times dg and du
+    float by;
+    __device__ __forceinline__ EpiGateBwd ready() const {
+        EpiGateBwd e = *this;
+        if (std::is_same<T, ff_half>::value) e.by = scale[0];
+        return e;
+    }
     __device__ __forceinline__ void plain(int, int m, int n, int left, bool inside, const ff_f32x4& dh) const {
         if (!inside) return;
-        const float s = std::is_same<T, ff_half>::value ? scale[0] : 1.f;
         ff_f32x4 gv = {0.f, 0.f, 0.f, 0.f}, uv = gv, dg, du, hv;
         const float *gp = g + m * F + n, *up = u + m * F + n;
         if (left >= 4) {
@@ -132,7 +141,7 @@ struct EpiGateBwd {
             hv[c] = a * uv[c];
             dg[c] = dh[c] * uv[c] * slope;
             du[c] = dh[c] * a;
-            if (std::is_same<T, ff_half>::value) dg[c] *= s, du[c] *= s;
+            if (std::is_same<T, ff_half>::value) dg[c] *= by, du[c] *= by;
         }
         dgu.put(m, n, left, dg);
         dgu.put(m, (int)Fp + n, left, du);
@@ -146,13 +155,14 @@ template <typename Epi>
 __global__ void __launch_bounds__(256) k_ff_join(EpiPart parts, int n_parts, int64_t M, int N, Epi epi) {
     const int per_row = (int)(parts.pitch / 4);
     const int64_t items = M * per_row;
+    const Epi e = epi.ready();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
         const int64_t m = i / per_row;
         const int n = (int)(i - m * per_row) * 4;
         const float* p = parts.out + m * parts.pitch + n;
         ff_f32x4 v = *reinterpret_cast<const ff_f32x4*>(p);
         for (int k = 1; k < n_parts; ++k) v += *reinterpret_cast<const ff_f32x4*>(p + k * parts.stride);
-        epi.plain(0, (int)m, n, N - n, n < N, v);
+        e.plain(0, (int)m, n, N - n, n < N, v);
     }
 }
 
@@ -187,14 +197,14 @@ __global__ void __launch_bounds__(256) k_ff_pack(FfPackJobs<T> jobs) {
     }
 }
 
-// ---- float16 gradients: the power of two by which dg and du are held (ff_grad_scale), of the largest |dy|.  Two launches: 4096 x 2048 x 8192 with all gradients 1244 -> 1273 us,
-//      40 x 2048 x 5504 149 -> 159
+// ---- float16 gradients: the power of two by which dg and du are held (ff_grad_scale), of the largest |dy|.  Two launches; backward pass with all gradients, us without and with them: 40 x
+//      2048 x 5504 96 and 104, 64 x 4096 x 8192 204 and 208, 1024 x 1024 x 2048 91 and 98.  (One workgroup for all of a short dy saves 1.5 at 32768 values and loses from 80000 on.)
 constexpr int FF_SCALE_PARTS = 256;
-__global__ void __launch_bounds__(256) k_ff_grad_top(const ff_half* __restrict__ dy, int64_t n, float* __restrict__ part) {
+__global__ void __launch_bounds__(1024) k_ff_grad_top(const ff_half* __restrict__ dy, int64_t n, float* __restrict__ part) {
     constexpr int N = FfVec<ff_half>::N;
-    __shared__ float tops[4];
+    __shared__ float tops[16];
     float top = 0.f;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N; i < n; i += (int64_t)gridDim.x * 256 * N) {
+    for (int64_t i = ((int64_t)blockIdx.x * 1024 + threadIdx.x) * N; i < n; i += (int64_t)gridDim.x * 1024 * N) {
         float v[N];
         ff_load_row(dy + i, 0, n - i < N ? (int)(n - i) : N, v);
 #pragma unroll
@@ -203,7 +213,9 @@ __global__ void __launch_bounds__(256) k_ff_grad_top(const ff_half* __restrict__
     top = nf_wave_max(top);
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+#pragma unroll
+    for (int w = 0; w < 16; ++w) top = fmaxf(top, tops[w]);
+    if (threadIdx.x == 0) part[blockIdx.x] = top;
 }
 // out[0] = the scale, out[1] = 1 / it
 __global__ void __launch_bounds__(64) k_ff_grad_scale(const float* __restrict__ part, float* __restrict__ out) {
@@ -477,7 +489,7 @@ int ff_fwd(const void* x, const void* wg, const void* wu, const void* wd, int M,
     const FfChoice c = ff_choice_of<T>(FF_GATE_UP, M, D, F);
     if (border) FF_TRY((product<T, false, false, true>(c, p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, true>{f.h, g_save, u_save, F, act, sides}, st)));
     else FF_TRY((product<T, false, false, true>(c, p, q, M, F, (int)f.h.pitch, (int)f.x.mid.pitch, EpiGate<T, false>{f.h, g_save, u_save, F, act, sides}, st)));
-    const EpiStore<T> store = {(T*)out, nullptr, D, M, 0x7fffffff, nullptr};
+    const EpiStore<T> store = {(T*)out, nullptr, D, M, 0x7fffffff, nullptr, 1.f};
     FF_TRY((product_split<T, false, false>(ff_choice_of<T>(FF_DOWN, M, D, F), as_operand(f.wd.mid, D), as_operand(f.h, M), M, D, (int)f.h.pitch, store, f.parts, st)));
     return 0;
 }
@@ -529,27 +541,27 @@ int ff_bwd(const void* x, const void* wg, const void* wu, const void* wd, const 
     // dh[m][f] = sum over d of dy[m][d] Wd[d][f]
     const float* scale = nullptr;
     if (std::is_same<T, ff_half>::value) {
-        hipLaunchKernelGGL(k_ff_grad_top, dim3(FF_SCALE_PARTS), dim3(256), 0, st, (const ff_half*)dy, (int64_t)M * D, f.scale + 2);
+        hipLaunchKernelGGL(k_ff_grad_top, dim3(FF_SCALE_PARTS), dim3(1024), 0, st, (const ff_half*)dy, (int64_t)M * D, f.scale + 2);
         hipLaunchKernelGGL(k_ff_grad_scale, dim3(1), dim3(64), 0, st, (const float*)f.scale + 2, f.scale);
         scale = f.scale;
     }
-    const EpiGateBwd<T> gate = {f.dgu, f.h, g, u, F, Fp, act, dwd != nullptr, scale};
+    const EpiGateBwd<T> gate = {f.dgu, f.h, g, u, F, Fp, act, dwd != nullptr, scale, 1.f};
     FfOperand p = as_operand(f.wd.mid, (int)f.wd.mid.pitch);
     FF_TRY((product<T, true, false, false>(ff_choice_of<T>(FF_DH, M, D, F), p, as_operand(f.dy.mid, M), M, F, Fp, D, gate, st)));
     if (dx) {          // dx[m][d] = sum over k of dgu[m][k] [Wg; zeros up to Fp; Wu][k][d]
         p = as_operand(f.wg.mid, (int)f.wg.mid.pitch);
         p.b = (const uint16_t*)f.wu.mid.p;
         p.len = F, p.seg = Fp;
-        const EpiStore<T> store = {(T*)dx, nullptr, D, M, 0x7fffffff, scale};
+        const EpiStore<T> store = {(T*)dx, nullptr, D, M, 0x7fffffff, scale, 1.f};
         FF_TRY((product_split<T, true, false>(ff_choice_of<T>(FF_DX, M, D, F), p, as_operand(f.dgu, M), M, D, Fp + F, store, f.parts, st)));
     }
     if (dwgu) {          // [dWg; dWu][f][d] = sum over m of dgu[m][f] x[m][d]
-        const EpiStore<T> store = {(T*)dwg, (T*)dwu, D, F, Fp, scale};
+        const EpiStore<T> store = {(T*)dwg, (T*)dwu, D, F, Fp, scale, 1.f};
         FF_TRY((product_split<T, true, true>(ff_choice_of<T>(FF_DW_GATE_UP, M, D, F), as_operand(f.x.mid, (int)f.x.mid.pitch), as_operand(f.dgu, 2 * Fp), 2 * Fp, D, M, store,
                                                   f.parts, st)));
     }
     if (dwd) {          // dWd[d][f] = sum over m of dy[m][d] h[m][f]
-        const EpiStore<T> store = {(T*)dwd, nullptr, F, D, 0x7fffffff, nullptr};
+        const EpiStore<T> store = {(T*)dwd, nullptr, F, D, 0x7fffffff, nullptr, 1.f};
         FF_TRY((product_split<T, true, true>(ff_choice_of<T>(FF_DW_DOWN, M, D, F), as_operand(f.h, Fp), as_operand(f.dy.mid, (int)f.dy.mid.pitch), D, F, M, store, f.parts,
                                                   st)));
     }
@@ -570,7 +582,7 @@ extern "C" int64_t nf_gated_ff_fwd_workspace_bytes(int64_t rows, int dim, int hi
     if (!ff_sizes_ok("nf_gated_ff_fwd_workspace_bytes", rows, dim, hidden, dtype, 0)) return -1;
     if (rows <= FF_ROWS_MAX) return ff_few_rows_h_bytes(rows, hidden, dtype == FF_F32 ? 4 : 2) + (rows + hidden) * 4;
     const int64_t n = dtype == FF_F32 ? FwdPlan<float>(nullptr, rows, dim, hidden).bytes : FwdPlan<ff_bf16>(nullptr, rows, dim, hidden).bytes;
-    const int64_t narrow = ff_narrow_fits(rows, dim, hidden) ? ff_narrow_workspace_bytes(rows, dim, hidden, dtype, false) : 0;
+    const int64_t narrow = ff_narrow_fits(rows, dim, hidden) ? ff_narrow_workspace_bytes(dim, hidden, dtype, false) : 0;
     return n > narrow ? n : narrow;          // (which of the two runs depends on whether g and u are saved)
 }
 
@@ -593,7 +605,7 @@ extern "C" int nf_gated_ff_bwd_recomputes(int64_t rows, int dim, int hidden) { r
 
 extern "C" int64_t nf_gated_ff_bwd_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, int want_dx, int want_dw_gate_up, int want_dw_down) {
     if (!ff_sizes_ok("nf_gated_ff_bwd_workspace_bytes", rows, dim, hidden, dtype, 0)) return -1;
-    if (want_dx && !want_dw_gate_up && !want_dw_down && ff_narrow_fits(rows, dim, hidden)) return ff_narrow_workspace_bytes(rows, dim, hidden, dtype, true);
+    if (want_dx && !want_dw_gate_up && !want_dw_down && ff_narrow_fits(rows, dim, hidden)) return ff_narrow_workspace_bytes(dim, hidden, dtype, true);
     if (dtype == FF_F32) return BwdPlan<float>(nullptr, rows, dim, hidden, want_dx, want_dw_gate_up, want_dw_down).bytes;
     return BwdPlan<ff_bf16>(nullptr, rows, dim, hidden, want_dx, want_dw_gate_up, want_dw_down).bytes;
 }

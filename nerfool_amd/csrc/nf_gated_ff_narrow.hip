@@ -33,11 +33,20 @@ struct NarrowParts<float> {
 // one wave a record: lane l holds row l mod 16, k = 8 (l / 16) + j, j = 0 .. 7 -> [chunk][record][part][lane][8]
 template <typename T>
 __global__ void __launch_bounds__(256) k_ff_narrow_pack(const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ wd, int D, int F, int kd, int backward,
-                                                        typename NarrowParts<T>::E* __restrict__ out) {
+                                                        typename NarrowParts<T>::E* __restrict__ out, float* __restrict__ norms) {
     typedef NarrowParts<T> P;
     const int per = narrow_records(kd, backward), chunks = (F + 31) / 32;
     const int rec = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, row = lane & 15, q = lane >> 4;
-    if (rec >= per * chunks) return;
+    if (rec >= per * chunks) {          // behind the records: a wave per gate row, whose norm relu's sides ask for
+        const int f = rec - per * chunks;
+        if (!norms || f >= 32 * chunks) return;
+        const double v = f < F && lane < D ? (double)(float)wg[(int64_t)f * D + lane] : 0.0;
+        double sq = v * v;
+#pragma unroll
+        for (int k = 32; k >= 1; k >>= 1) sq += __shfl_xor(sq, k, NF_WAVE);
+        if (lane == 0) norms[f] = (float)sqrt(sq);
+        return;
+    }
     const int chunk = rec / per, n = rec - chunk * per;
     typename P::E part[8][P::NP];
     for (int j = 0; j < 8; ++j) {
@@ -73,7 +82,7 @@ struct Narrow {
     static constexpr int NP = P::NP, RECORDS = narrow_records(KD, BWD), PIECES = RECORDS * NP, CHUNK = PIECES * 1024;
 
     // this lane's 8 values of a token's row as an operand: k = 32 kd + 8 (l / 16) ..
-    static __device__ __forceinline__ void row(const T* x, int64_t m, int64_t M, int D, int k, V (&v)[NP]) {
+    static __device__ __forceinline__ void row(const T* x, int64_t m, int64_t M, int D, int k, V (&v)[NP], double* squares = nullptr) {
         float f[8];
         const T* r = x + (m < M ? m : M - 1) * D;
         constexpr int N = FfVec<T>::N;
@@ -83,6 +92,10 @@ struct Narrow {
             ff_load_row(r, k + c, D, t);
 #pragma unroll
             for (int j = 0; j < N; ++j) f[c + j] = t[j];
+        }
+        if (squares) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) *squares = fma((double)f[j], (double)f[j], *squares);
         }
         operand(f, v);
     }
@@ -122,10 +135,17 @@ __global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, cons
     };
     load_chunk(0);
     V xb[KD][NP], yb[BWD ? KD : 1][NP];
+    double squares = 0;
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
-        N::row(x, m, M, D, 32 * k + 8 * q, xb[k]);
+        N::row(x, m, M, D, 32 * k + 8 * q, xb[k], SIDES ? &squares : nullptr);
         if (BWD) N::row(dy, m, M, D, 32 * k + 8 * q, yb[BWD ? k : 0]);
+    }
+    float bound = 0.f;          // of the token's units, per |row of Wg|; the token lies on 4 lanes
+    if constexpr (SIDES) {
+        squares += __shfl_xor(squares, 16, NF_WAVE);
+        squares += __shfl_xor(squares, 32, NF_WAVE);
+        bound = sides.scale * (float)sqrt(squares);
     }
     float scale = 1.f;          // float16: of the token's dg and du (ff_grad_scale; its dy lies on 4 lanes)
     if constexpr (BWD && std::is_same<T, ff_half>::value) {
@@ -159,11 +179,22 @@ __global__ void __launch_bounds__(512) k_ff_narrow(const T* __restrict__ x, cons
             }
         }
         if constexpr (SIDES) {
+            bool ask[8];
+            int f[8];
+            float gs[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int f = 32 * c + 16 * (j / 4) + 4 * q + j % 4;
-                g[j / 4][j % 4] = ff_side<T>(sides, m < M && f < F, m, f, g[j / 4][j % 4]);
+            for (int i = 0; i < 2; ++i) {
+                const ff_f32x4 wn = *reinterpret_cast<const ff_f32x4*>(sides.wn + 32 * c + 16 * i + 4 * q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f[4 * i + j] = 32 * c + 16 * i + 4 * q + j;
+                    gs[4 * i + j] = g[i][j];
+                    ask[4 * i + j] = m < M && f[4 * i + j] < F && fabsf(g[i][j]) <= bound * wn[j];
+                }
             }
+            ff_sides_settle<T>(sides, ask, m, f, gs);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j / 4][j % 4] = gs[j];
         }
         V hb[NP], ub[NP];          // forward: h; backward: dg and du
         float v[8], v2[8];
@@ -211,10 +242,11 @@ int narrow_run(const void* x, const void* wg, const void* wu, const void* wd, co
         }
         set[dev] = true;
     }
-    const int records = N::RECORDS * ((F + 31) / 32);
-    FfSides sides = {};
-    if (SIDES) sides = ff_sides<T>(x, wg, M, F, D, N::NP == 3 ? 12 : 2, (float*)((char*)workspace + (int64_t)records * N::NP * 1024), st);
-    hipLaunchKernelGGL((k_ff_narrow_pack<T>), dim3((records + 3) / 4), dim3(256), 0, st, (const T*)wg, (const T*)wu, (const T*)wd, D, F, KD, (int)BWD, (typename N::E*)workspace);
+    const int chunks = (F + 31) / 32, records = N::RECORDS * chunks;
+    float* norms = SIDES ? (float*)((char*)workspace + (int64_t)records * N::NP * 1024) : nullptr;
+    const FfSides sides = {x, wg, nullptr, norms, D, ff_sides_scale(N::NP == 3 ? 12 : 2)};
+    hipLaunchKernelGGL((k_ff_narrow_pack<T>), dim3((records + (SIDES ? 32 * chunks : 0) + 3) / 4), dim3(256), 0, st, (const T*)wg, (const T*)wu, (const T*)wd, D, F, KD, (int)BWD,
+                       (typename N::E*)workspace, norms);
     hipLaunchKernelGGL((k_ff_narrow<T, KD, BWD, SIDES>), dim3((unsigned)((M + 127) / 128)), dim3(512), LDS, st, (const T*)x, (const T*)dy, (const char*)workspace, M, D, F, act,
                        (T*)out, sides);
     return 0;
@@ -236,8 +268,8 @@ int narrow_kd(const void* x, const void* wg, const void* wu, const void* wd, con
 // A chunk takes 2 to 4 us, so 16 of them what the products' launches take at their smallest; from 16384 rows on half the CUs are busy here.
 bool ff_narrow_fits(int64_t rows, int dim, int hidden) { return dim <= 64 && (hidden <= 512 || rows >= 16384); }
 
-int64_t ff_narrow_workspace_bytes(int64_t rows, int dim, int hidden, int dtype, bool backward) {
-    return (int64_t)((hidden + 31) / 32) * narrow_records(dim <= 32 ? 1 : 2, backward) * (dtype == FF_F32 ? 3 : 1) * 1024 + (backward ? (rows + hidden) * 4 : 0);
+int64_t ff_narrow_workspace_bytes(int dim, int hidden, int dtype, bool backward) {
+    return (int64_t)((hidden + 31) / 32) * (narrow_records(dim <= 32 ? 1 : 2, backward) * (dtype == FF_F32 ? 3 : 1) * 1024 + (backward ? 128 : 0));
 }
 
 // dy null: out = the block of x; else out = dx

@@ -450,3 +450,34 @@ def test_norm_and_8bit_offsets_beyond_32_bits():
     # (fewer rows may take another form, whose sums are in another order: the bound of check_8bit_norm)
     small = ff.gated_feed_forward_8bit((q[torch.cat([at] * 4)], s[torch.cat([at] * 4)]), *pairs, dtype=BF16)[:len(at)].double()
     assert float((out[at].double() - small).norm() / small.norm()) <= (2.0 ** -18 + 2.0 ** -13.5) ** 0.5
+
+
+def check_relu_zeros(device, rows, dim, hidden, dtype, frozen):
+    """rows of zeros, and gate rows of zeros: g is 0 exactly, and so is relu's slope there"""
+    gen = torch.Generator().manual_seed(71)
+    x = normal(gen, rows, dim, dtype=dtype, device=device)
+    ws = [normal(gen, *s, dtype=dtype, device=device, scale=s[1] ** -0.5) for s in ((hidden, dim), (hidden, dim), (dim, hidden))]
+    x[::3], ws[0][::2] = 0, 0
+    dy = normal(gen, rows, dim, dtype=dtype, device=device)
+    want = ref.gated(x, *ws, 'relu', dy, dtype, sides=True)
+    ws = [w.requires_grad_(not frozen) for w in ws]
+    out = ff.gated_feed_forward(x.requires_grad_(True), *ws, activation='relu')
+    grads = torch.autograd.grad(out, [x] if frozen else [x, *ws], dy)
+    near(out.detach(), want['out'], 'out')
+    for key, got in zip(('dx', 'dw_gate', 'dw_up', 'dw_down'), grads):
+        near(got, want[key], key)
+    assert (grads[0][::3] == 0).all() and (frozen or (grads[1][::2] == 0).all())
+
+
+ZEROS = [(5, 41, 24, F32, False), (70, 37, 40, BF16, False), (70, 40, 33, F32, True), (66, 64, 50, F16, True)]
+
+
+@pytest.mark.parametrize('rows,dim,hidden,dtype,frozen', ZEROS)
+def test_relu_zeros_standin(emu, rows, dim, hidden, dtype, frozen):  # noqa: F811
+    check_relu_zeros(emu, rows, dim, hidden, dtype, frozen)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,dim,hidden,dtype,frozen', ZEROS + [(700, 200, 300, F32, False), (1300, 64, 257, F32, True)])
+def test_relu_zeros(rows, dim, hidden, dtype, frozen):
+    check_relu_zeros('cuda', rows, dim, hidden, dtype, frozen)
